@@ -82,6 +82,9 @@ SIGNATURES = {
     "fc3d_capture_fwd": (c_int, [P, P, P, P, P, P, P, P, I64, P, P, P, c_int, c_int, c_int, P, P, P, P, P, c_int, c_int,
                                  P, P, P]),
     "fc3d_box_filter": (c_int, [P, P, c_int, c_int, c_int, c_int, c_int, c_float, P]),
+    "fc3d_layer_norm_fwd": (c_int, [P, P, c_int, P, P, c_int, I64, I64, I64, I64, c_float, c_int, P, P, P]),
+    "fc3d_layer_norm_bwd_workspace": (c_size_t, [c_int, I64, I64, I64]),
+    "fc3d_layer_norm_bwd": (c_int, [P, P, P, c_int, P, P, c_int, P, P, I64, I64, I64, I64, I64, c_int, P, P, P, P]),
     "fc3d_profile_enable": (c_int, [c_int]),
     "fc3d_profile_report": (c_int, [c_char_p, c_size_t]),
 }

@@ -17,13 +17,17 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(os.path.dirname(HERE))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libfc3d_hip.so")
-SOURCES = ["optics.hip", "geometry.hip", "capture.hip", "profile.hip"]
+SOURCES = ["optics.hip", "geometry.hip", "capture.hip", "profile.hip", "norm.hip"]
 
 # -ffp-contract=off                         index/mask decisions need the reference's separately rounded ops
 # -fhip-fp32-correctly-rounded-divide-sqrt  IEEE fp32 division (torch's CPU kernels divide exactly)
 # -munsafe-fp-atomics                       hardware float atomic add instead of a compare-and-swap loop
 FLAGS = ["-O3", "--offload-arch=gfx950", "-fPIC", "-shared", "-std=c++17", "-ffp-contract=off",
          "-fhip-fp32-correctly-rounded-divide-sqrt", "-munsafe-fp-atomics", "-fno-gpu-rdc"]
+# The training operators' sources keep to one fp32 operation per lane and instruction: the packed forms are taken out
+# of the code generator's choice (the host pass warns that it does not know the feature: harmless).
+_SCALAR_F32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+SOURCE_FLAGS = {"norm.hip": _SCALAR_F32}
 
 
 def _hipcc() -> str:
@@ -43,7 +47,7 @@ def source_hash(extra_flags=()) -> str:
         h.update(os.path.basename(path).encode() + b"\0")
         with open(path, "rb") as f:
             h.update(f.read())
-    h.update(" ".join([*FLAGS, *extra_flags, *SOURCES]).encode())
+    h.update(" ".join([*FLAGS, *extra_flags, *SOURCES, *(f"{k} {v}" for k, v in SOURCE_FLAGS.items())]).encode())
     try:
         h.update(subprocess.run([_hipcc(), "--version"], capture_output=True, timeout=60).stdout)
     except Exception:
@@ -74,7 +78,7 @@ def build(force: bool = False, verbose: bool = True, extra_flags=(), out: str = 
     with tempfile.TemporaryDirectory(prefix="fc3d_build_") as tmp:
         def compile_one(src):
             obj = os.path.join(tmp, src + ".o")
-            cmd = [_hipcc(), *cflags, *extra_flags, "-I", os.path.join(ROOT, "include"), "-I", CSRC, "-c",
+            cmd = [_hipcc(), *cflags, *SOURCE_FLAGS.get(src, ()), *extra_flags, "-I", os.path.join(ROOT, "include"), "-I", CSRC, "-c",
                    os.path.join(CSRC, src), "-o", obj]
             if verbose:
                 print(" ".join(cmd), flush=True)

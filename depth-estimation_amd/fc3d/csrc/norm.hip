@@ -1,0 +1,917 @@
+// Layer norm, forward and backward, for activations held in 32 or 16 bits.
+//
+//   y = act((x - mu) r w + b),   mu = mean_c x,   r = 1 / sqrt(mean_c (x - mu)^2 + eps)
+//
+// over `channels` values of each position; act is the identity or max(., 0).  With g = dy where the activation
+// passes it and h = (x - mu) r:
+//
+//   dx = r (g w - mean_c(g w) - h mean_c(g w h)),   dw = sum_positions g h,   db = sum_positions g.
+//
+// Two memory orders: "rows" (the normalised axis is contiguous: inner == 1) and "planes" (a channel's positions are
+// contiguous, the channels of one position lie `inner` values apart: images with the channel axis before the
+// spatial ones).  Both are bound by memory: a value is read once, kept in registers while its position's
+// statistics are formed (mean first, then the squares of the differences: no cancellation), and written once.
+// Statistics, sums over positions and all arithmetic are 32 bits; a 16-bit result is rounded once, at its store.
+// Sums over positions are kept per workgroup, written as partial sums and added in a fixed order by a second,
+// small launch: no atomics, the same bits on every run.
+#include "fc3d_common.h"
+
+namespace fc3d {
+namespace {
+
+typedef __bf16 bf16;
+typedef _Float16 f16;
+
+constexpr int kVec = 4;              // values of one vector access: 16 bytes of fp32, 8 of a 16-bit type
+
+template <typename T, int V>
+struct Vec {
+    T e[V];
+};
+template <typename T>
+struct Word {
+    typedef uint32_t type __attribute__((ext_vector_type(2), aligned(2)));
+};
+template <>
+struct Word<float> {
+    typedef uint32_t type __attribute__((ext_vector_type(4), aligned(4)));
+};
+// Vector accesses at the element's own alignment: rows of odd length and planes of odd size start anywhere, and
+// global loads and stores take any address on this chip.
+template <typename T, int V>
+__device__ __forceinline__ Vec<T, V> ldv(const T* p) {
+    Vec<T, V> r;
+    if constexpr (V == 1) {
+        r.e[0] = *p;
+    } else {
+        typedef typename Word<T>::type word;
+        const word w = *reinterpret_cast<const word*>(p);
+        __builtin_memcpy(&r, &w, sizeof(r));
+    }
+    return r;
+}
+template <typename T, int V>
+__device__ __forceinline__ void stv(T* p, const Vec<T, V>& v) {
+    if constexpr (V == 1) {
+        *p = v.e[0];
+    } else {
+        typename Word<T>::type w;
+        __builtin_memcpy(&w, &v, sizeof(v));
+        *reinterpret_cast<typename Word<T>::type*>(p) = w;
+    }
+}
+// The first n of V values (n <= 0: none); the rest reads as zero.
+template <typename T, int V>
+__device__ __forceinline__ Vec<T, V> ldv_n(const T* p, int n) {
+    if (n >= V) return ldv<T, V>(p);
+    Vec<T, V> r;
+#pragma unroll
+    for (int j = 0; j < V; ++j) r.e[j] = (T)0.0f;
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+        if (j < n) r.e[j] = p[j];
+    return r;
+}
+template <typename T, int V>
+__device__ __forceinline__ void stv_n(T* p, const Vec<T, V>& v, int n) {
+    if (n >= V) {
+        stv<T, V>(p, v);
+        return;
+    }
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+        if (j < n) p[j] = v.e[j];
+}
+
+// A weight or bias: fp32 or the activations' 16-bit type (the same branch in every lane), `absent` without one
+template <typename T>
+__device__ __forceinline__ float param(const void* p, bool f32, long i, float absent) {
+    if (!p) return absent;
+    return f32 ? static_cast<const float*>(p)[i] : (float)static_cast<const T*>(p)[i];
+}
+__device__ __forceinline__ void put_param(void* p, int type, long i, float v) {
+    if (type == FC3D_F32) static_cast<float*>(p)[i] = v;
+    else if (type == FC3D_BF16) static_cast<bf16*>(p)[i] = (bf16)v;
+    else static_cast<f16*>(p)[i] = (f16)v;
+}
+
+// Whether max(pre, 0) hands pre on; a NaN passes, in both directions
+__device__ __forceinline__ bool passes(float pre) { return !(pre <= 0.0f); }
+
+// Sum over the LPR lanes that share a row, the same bits in every lane.  Above one wavefront the wavefronts' sums
+// meet in LDS; `slot` alternates between two areas, so that one barrier per sum is enough.
+template <int LPR>
+__device__ __forceinline__ float group_sum(float v, float* red, int slot) {
+#pragma unroll
+    for (int o = (LPR < 64 ? LPR : 64) / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+    if constexpr (LPR > 64) {
+        constexpr int nw = LPR / 64;
+        float* a = red + slot * nw;
+        if ((threadIdx.x & 63) == 0) a[threadIdx.x >> 6] = v;
+        __syncthreads();
+        v = a[0];
+#pragma unroll
+        for (int i = 1; i < nw; ++i) v += a[i];
+    }
+    return v;
+}
+
+constexpr int kRowElems = 16;        // values of a row that one lane holds
+
+// ---- rows -------------------------------------------------------------------------------------------------
+// LPR lanes per row, kRowElems values each; a workgroup takes rows blockIdx.x * (BLOCK / LPR) + k * gridDim.x * ...,
+// its lanes keep their columns' weights.
+template <typename T, int LPR, int BLOCK>
+__global__ __launch_bounds__(BLOCK) void ln_rows_fwd(const T* __restrict__ x, const void* __restrict__ w, const void* __restrict__ b, bool w_f32, long rows, int C, long x_stride,
+                                                     float eps, int relu, T* __restrict__ y, float* __restrict__ mean,
+                                                     float* __restrict__ rstd) {
+    constexpr int V = kVec, NV = kRowElems / V;
+    constexpr int RPB = BLOCK / LPR;
+    __shared__ float red[LPR > 64 ? 2 * (LPR / 64) : 1];
+    const int lane = threadIdx.x % LPR, sub = threadIdx.x / LPR;
+    const float fc = (float)C;
+    float wv[NV * V], bv[NV * V];
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+        const int c0 = (lane + k * LPR) * V;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            wv[k * V + j] = c0 + j < C ? param<T>(w, w_f32, c0 + j, 1.0f) : 0.0f;
+            bv[k * V + j] = c0 + j < C ? param<T>(b, w_f32, c0 + j, 0.0f) : 0.0f;
+        }
+    }
+    // every lane of a workgroup runs the same number of rounds: the sums above one wavefront hold barriers
+    for (long r0 = (long)blockIdx.x * RPB; r0 < rows; r0 += (long)gridDim.x * RPB) {
+        const long r = r0 + sub;
+        const bool live = r < rows;
+        const T* xr = x + (live ? r : r0) * x_stride;
+        Vec<T, V> xv[NV];
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            const int c0 = (lane + k * LPR) * V;
+            xv[k] = ldv_n<T, V>(xr + (c0 < C ? c0 : 0), C - c0);
+        }
+        float s = 0.0f;
+#pragma unroll
+        for (int k = 0; k < NV; ++k)
+#pragma unroll
+            for (int j = 0; j < V; ++j) s += (float)xv[k].e[j];
+        const float mu = group_sum<LPR>(s, red, 0) / fc;
+        s = 0.0f;
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            const int n = C - (lane + k * LPR) * V;
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const float d = j < n ? (float)xv[k].e[j] - mu : 0.0f;
+                s = fmaf(d, d, s);
+            }
+        }
+        const float rs = 1.0f / sqrtf(group_sum<LPR>(s, red, 1) / fc + eps);
+        if (live) {
+            T* yr = y + r * C;
+#pragma unroll
+            for (int k = 0; k < NV; ++k) {
+                const int c0 = (lane + k * LPR) * V;
+                if (c0 < C) {
+                    Vec<T, V> o;
+#pragma unroll
+                    for (int j = 0; j < V; ++j) {
+                        float v = fmaf(((float)xv[k].e[j] - mu) * rs, wv[k * V + j], bv[k * V + j]);
+                        if (relu) v = passes(v) ? v : 0.0f;
+                        o.e[j] = (T)v;
+                    }
+                    stv_n<T, V>(yr + c0, o, C - c0);
+                }
+            }
+            if (mean && lane == 0) {
+                mean[r] = mu;
+                rstd[r] = rs;
+            }
+        }
+    }
+}
+
+// partial: [gridDim.x][2][C] sums of g h and of g over the workgroup's rows, or NULL when no parameter asks for them
+template <typename T, int LPR, int BLOCK>
+__global__ __launch_bounds__(BLOCK) void ln_rows_bwd(const T* __restrict__ dy, const T* __restrict__ x,
+                                                     const void* __restrict__ w, const void* __restrict__ b, bool w_f32,
+                                                     const float* __restrict__ mean, const float* __restrict__ rstd,
+                                                     long rows, int C, long dy_stride, long x_stride, int relu,
+                                                     T* __restrict__ dx, float* __restrict__ partial) {
+    constexpr int V = kVec, NV = kRowElems / V, E = kRowElems;
+    constexpr int RPB = BLOCK / LPR;
+    __shared__ float red[LPR > 64 ? 4 * (LPR / 64) : 1];
+    __shared__ float cols[RPB > 1 ? BLOCK * E : 1];
+    const int lane = threadIdx.x % LPR, sub = threadIdx.x / LPR;
+    const float fc = (float)C;
+    float wv[E], bv[E], aw[E], ab[E];
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+        const int c0 = (lane + k * LPR) * V;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            wv[k * V + j] = c0 + j < C ? param<T>(w, w_f32, c0 + j, 1.0f) : 0.0f;
+            bv[k * V + j] = c0 + j < C ? param<T>(b, w_f32, c0 + j, 0.0f) : 0.0f;
+            aw[k * V + j] = 0.0f;
+            ab[k * V + j] = 0.0f;
+        }
+    }
+    int turn = 0;
+    for (long r0 = (long)blockIdx.x * RPB; r0 < rows; r0 += (long)gridDim.x * RPB, turn ^= 1) {
+        const long r = r0 + sub;
+        const bool live = r < rows;
+        const T* xr = x + (live ? r : r0) * x_stride;
+        const T* gr = dy + (live ? r : r0) * dy_stride;
+        Vec<T, V> xv[NV], gv[NV];
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            const int c0 = (lane + k * LPR) * V;
+            xv[k] = ldv_n<T, V>(xr + (c0 < C ? c0 : 0), C - c0);
+            gv[k] = ldv_n<T, V>(gr + (c0 < C ? c0 : 0), live ? C - c0 : 0);
+        }
+        const float mu = mean[live ? r : r0], rs = rstd[live ? r : r0];
+        float s1 = 0.0f, s2 = 0.0f;
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            const int n = C - (lane + k * LPR) * V;
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const int i = k * V + j;
+                const float h = ((float)xv[k].e[j] - mu) * rs;
+                float g = (float)gv[k].e[j];
+                if (relu) {
+                    g = passes(fmaf(h, wv[i], bv[i])) ? g : 0.0f;
+                    gv[k].e[j] = (T)g;
+                }
+                if (j < n && live) {
+                    const float gw = g * wv[i];
+                    s1 += gw;
+                    s2 = fmaf(gw, h, s2);
+                    aw[i] = fmaf(g, h, aw[i]);
+                    ab[i] += g;
+                }
+            }
+        }
+        const float m1 = group_sum<LPR>(s1, red, 2 * turn) / fc;
+        const float m2 = group_sum<LPR>(s2, red, 2 * turn + 1) / fc;
+        if (live && dx) {
+            T* dr = dx + r * C;
+#pragma unroll
+            for (int k = 0; k < NV; ++k) {
+                const int c0 = (lane + k * LPR) * V;
+                if (c0 < C) {
+                    Vec<T, V> o;
+#pragma unroll
+                    for (int j = 0; j < V; ++j) {
+                        const float h = ((float)xv[k].e[j] - mu) * rs;
+                        o.e[j] = (T)(rs * (fmaf((float)gv[k].e[j], wv[k * V + j], -m1) - h * m2));
+                    }
+                    stv_n<T, V>(dr + c0, o, C - c0);
+                }
+            }
+        }
+    }
+    if (!partial) return;
+    float* pw = partial + (long)blockIdx.x * 2 * C;
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+        float* a = which ? ab : aw;
+        if constexpr (RPB > 1) {
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < E; ++i) cols[(sub * E + i) * LPR + lane] = a[i];
+            __syncthreads();
+            for (int t = threadIdx.x; t < LPR * E; t += BLOCK) {
+                float s = 0.0f;
+#pragma unroll 4
+                for (int q = 0; q < RPB; ++q) s += cols[q * E * LPR + t];
+                const int i = t / LPR, c = (t % LPR + (i / V) * LPR) * V + i % V;
+                if (c < C) pw[which * C + c] = s;
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < NV; ++k) {
+                const int c0 = (lane + k * LPR) * V;
+#pragma unroll
+                for (int j = 0; j < V; ++j)
+                    if (c0 + j < C) pw[which * C + c0 + j] = a[k * V + j];
+            }
+        }
+    }
+}
+
+// ---- planes -----------------------------------------------------------------------------------------------
+// A workgroup is CL channel groups x PL positions; a lane holds E channels (cg, cg + CL, ...) of V neighbouring
+// positions.  Lanes next to each other take neighbouring positions, so every load covers PL * V * sizeof(T)
+// contiguous bytes of one channel.  Positions are counted in vectors over the whole batch (q = image * nvec + vector).
+template <int CL, int PL>
+constexpr int channel_groups() {      // sums that are left after the lanes of a wavefront have added theirs
+    return PL >= 64 ? CL : CL > 64 / PL ? CL / (64 / PL) : 1;
+}
+template <int CL, int PL, int V>
+__device__ __forceinline__ void channel_sums(float (&s)[V], float* red) {
+    if constexpr (CL > 1) {
+        const int pl = threadIdx.x % PL, cg = threadIdx.x / PL;
+        constexpr int NG = channel_groups<CL, PL>(), GW = CL / NG;
+#pragma unroll
+        for (int o = PL; o < PL * GW; o <<= 1)
+#pragma unroll
+            for (int v = 0; v < V; ++v) s[v] += __shfl_xor(s[v], o, 64);
+        if constexpr (NG > 1) {
+            __syncthreads();                                  // the readers of the last sums are through
+            if (cg % GW == 0)
+#pragma unroll
+                for (int v = 0; v < V; ++v) red[((cg / GW) * V + v) * PL + pl] = s[v];
+            __syncthreads();
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                float a = red[v * PL + pl];
+#pragma unroll
+                for (int g = 1; g < NG; ++g) a += red[(g * V + v) * PL + pl];
+                s[v] = a;
+            }
+        }
+    }
+}
+
+template <typename T, int V, int CL, int PL, int E>
+__global__ __launch_bounds__(CL* PL) void ln_planes_fwd(const T* __restrict__ x, const void* __restrict__ w, const void* __restrict__ b, bool w_f32, unsigned nq, unsigned nvec, int C,
+                                                        long inner, long x_stride, float eps, int relu, T* __restrict__ y,
+                                                        float* __restrict__ mean, float* __restrict__ rstd) {
+    __shared__ float red[CL > 1 ? channel_groups<CL, PL>() * PL * V : 1];
+    const int pl = threadIdx.x % PL, cg = threadIdx.x / PL;
+    const float fc = (float)C;
+    float wv[E], bv[E];
+#pragma unroll
+    for (int k = 0; k < E; ++k) {
+        const int c = cg + k * CL;
+        wv[k] = c < C ? param<T>(w, w_f32, c, 1.0f) : 0.0f;
+        bv[k] = c < C ? param<T>(b, w_f32, c, 0.0f) : 0.0f;
+    }
+    for (unsigned long q0 = (unsigned long)blockIdx.x * PL; q0 < nq; q0 += (unsigned long)gridDim.x * PL) {
+        const bool live = q0 + pl < nq;
+        const unsigned q = live ? (unsigned)(q0 + pl) : 0u;
+        const unsigned img = q / nvec;
+        const long p = (long)(q - img * nvec) * V;
+        const int n = live ? (int)(inner - p < V ? inner - p : V) : 0;
+        const T* xp = x + (long)img * x_stride + p;
+        Vec<T, V> xv[E];
+#pragma unroll
+        for (int k = 0; k < E; ++k) {
+            const int c = cg + k * CL;
+            xv[k] = ldv_n<T, V>(xp + (c < C ? c : 0) * inner, c < C ? n : 0);
+        }
+        float mu[V], rs[V];
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            mu[v] = 0.0f;
+#pragma unroll
+            for (int k = 0; k < E; ++k) mu[v] += (float)xv[k].e[v];
+        }
+        channel_sums<CL, PL, V>(mu, red);
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            mu[v] /= fc;
+            rs[v] = 0.0f;
+#pragma unroll
+            for (int k = 0; k < E; ++k) {
+                const float d = cg + k * CL < C ? (float)xv[k].e[v] - mu[v] : 0.0f;
+                rs[v] = fmaf(d, d, rs[v]);
+            }
+        }
+        channel_sums<CL, PL, V>(rs, red);
+#pragma unroll
+        for (int v = 0; v < V; ++v) rs[v] = 1.0f / sqrtf(rs[v] / fc + eps);
+        T* yp = y + (long)img * inner * C + p;
+#pragma unroll
+        for (int k = 0; k < E; ++k) {
+            const int c = cg + k * CL;
+            if (c < C) {
+                Vec<T, V> o;
+#pragma unroll
+                for (int v = 0; v < V; ++v) {
+                    float a = fmaf(((float)xv[k].e[v] - mu[v]) * rs[v], wv[k], bv[k]);
+                    if (relu) a = passes(a) ? a : 0.0f;
+                    o.e[v] = (T)a;
+                }
+                stv_n<T, V>(yp + c * inner, o, n);
+            }
+        }
+        if (mean && cg == 0) {
+#pragma unroll
+            for (int v = 0; v < V; ++v)
+                if (v < n) {
+                    mean[(long)img * inner + p + v] = mu[v];
+                    rstd[(long)img * inner + p + v] = rs[v];
+                }
+        }
+    }
+}
+
+template <typename T, int V, int CL, int PL, int E>
+__global__ __launch_bounds__(CL* PL) void ln_planes_bwd(const T* __restrict__ dy, const T* __restrict__ x,
+                                                        const void* __restrict__ w, const void* __restrict__ b, bool w_f32,
+                                                        const float* __restrict__ mean, const float* __restrict__ rstd,
+                                                        unsigned nq, unsigned nvec, int C, long inner, long dy_stride,
+                                                        long x_stride, int relu, T* __restrict__ dx,
+                                                        float* __restrict__ partial) {
+    __shared__ float red[CL > 1 ? channel_groups<CL, PL>() * PL * V : 1];
+    __shared__ float wave_part[PL > 64 ? CL * (PL / 64) * E : 1];
+    const int pl = threadIdx.x % PL, cg = threadIdx.x / PL;
+    const float fc = (float)C;
+    float wv[E], bv[E], aw[E], ab[E];
+#pragma unroll
+    for (int k = 0; k < E; ++k) {
+        const int c = cg + k * CL;
+        wv[k] = c < C ? param<T>(w, w_f32, c, 1.0f) : 0.0f;
+        bv[k] = c < C ? param<T>(b, w_f32, c, 0.0f) : 0.0f;
+        aw[k] = 0.0f;
+        ab[k] = 0.0f;
+    }
+    for (unsigned long q0 = (unsigned long)blockIdx.x * PL; q0 < nq; q0 += (unsigned long)gridDim.x * PL) {
+        const bool live = q0 + pl < nq;
+        const unsigned q = live ? (unsigned)(q0 + pl) : 0u;
+        const unsigned img = q / nvec;
+        const long p = (long)(q - img * nvec) * V;
+        const int n = live ? (int)(inner - p < V ? inner - p : V) : 0;
+        const T* xp = x + (long)img * x_stride + p;
+        const T* gp = dy + (long)img * dy_stride + p;
+        Vec<T, V> xv[E], gv[E];
+#pragma unroll
+        for (int k = 0; k < E; ++k) {
+            const int c = cg + k * CL;
+            xv[k] = ldv_n<T, V>(xp + (c < C ? c : 0) * inner, c < C ? n : 0);
+            gv[k] = ldv_n<T, V>(gp + (c < C ? c : 0) * inner, c < C ? n : 0);
+        }
+        float mu[V], rs[V], s1[V], s2[V];
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            const long at = (long)img * inner + p + (v < n ? v : 0);
+            mu[v] = mean[at];
+            rs[v] = rstd[at];
+            s1[v] = 0.0f;
+            s2[v] = 0.0f;
+        }
+#pragma unroll
+        for (int k = 0; k < E; ++k) {
+            const bool on = cg + k * CL < C;
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                const float h = ((float)xv[k].e[v] - mu[v]) * rs[v];
+                float g = (float)gv[k].e[v];
+                if (relu) {
+                    g = passes(fmaf(h, wv[k], bv[k])) ? g : 0.0f;
+                    gv[k].e[v] = (T)g;
+                }
+                if (on && v < n) {
+                    const float gw = g * wv[k];
+                    s1[v] += gw;
+                    s2[v] = fmaf(gw, h, s2[v]);
+                    aw[k] = fmaf(g, h, aw[k]);
+                    ab[k] += g;
+                }
+            }
+        }
+        channel_sums<CL, PL, V>(s1, red);
+        channel_sums<CL, PL, V>(s2, red);
+        if (dx) {
+            T* dp = dx + (long)img * inner * C + p;
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                s1[v] /= fc;
+                s2[v] /= fc;
+            }
+#pragma unroll
+            for (int k = 0; k < E; ++k) {
+                const int c = cg + k * CL;
+                if (c < C) {
+                    Vec<T, V> o;
+#pragma unroll
+                    for (int v = 0; v < V; ++v) {
+                        const float h = ((float)xv[k].e[v] - mu[v]) * rs[v];
+                        o.e[v] = (T)(rs[v] * (fmaf((float)gv[k].e[v], wv[k], -s1[v]) - h * s2[v]));
+                    }
+                    stv_n<T, V>(dp + c * inner, o, n);
+                }
+            }
+        }
+    }
+    if (!partial) return;
+    float* pw = partial + (long)blockIdx.x * 2 * C;
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+        float* a = which ? ab : aw;
+#pragma unroll
+        for (int k = 0; k < E; ++k)
+#pragma unroll
+            for (int o = (PL < 64 ? PL : 64) / 2; o > 0; o >>= 1) a[k] += __shfl_xor(a[k], o, 64);
+        if constexpr (PL > 64) {
+            constexpr int NW = PL / 64;
+            __syncthreads();
+            if ((threadIdx.x & 63) == 0)
+#pragma unroll
+                for (int k = 0; k < E; ++k) wave_part[(cg * NW + pl / 64) * E + k] = a[k];
+            __syncthreads();
+            for (int t = threadIdx.x; t < CL * E; t += CL * PL) {
+                const int g = t / E, k = t % E, c = g + k * CL;
+                float s = 0.0f;
+#pragma unroll
+                for (int i = 0; i < NW; ++i) s += wave_part[(g * NW + i) * E + k];
+                if (c < C) pw[which * C + c] = s;
+            }
+        } else {
+            if (pl == 0)
+#pragma unroll
+                for (int k = 0; k < E; ++k)
+                    if (cg + k * CL < C) pw[which * C + cg + k * CL] = a[k];
+        }
+    }
+}
+
+// ---- channels beyond what a workgroup's registers hold ------------------------------------------------------
+// One workgroup per row (rows) or per PLL positions (planes), the values read once per sum and once for the
+// result; the repeats come from the caches.  Strides: consecutive channels lie `cs` values apart.
+constexpr int kLongBlock = 1024;
+constexpr int kLongPos = 16;         // planes: positions a workgroup takes
+
+template <bool PLANES>
+__device__ __forceinline__ float long_sum(float v, float* red) {
+    __syncthreads();
+    if constexpr (PLANES) {
+        v += __shfl_xor(v, 16, 64);
+        v += __shfl_xor(v, 32, 64);
+        if ((threadIdx.x & 63) < kLongPos) red[(threadIdx.x >> 6) * kLongPos + (threadIdx.x & 15)] = v;
+        __syncthreads();
+        v = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kLongBlock / 64; ++i) v += red[i * kLongPos + (threadIdx.x & 15)];
+    } else {
+        v = wave_sum(v);
+        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+        __syncthreads();
+        v = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kLongBlock / 64; ++i) v += red[i];
+    }
+    return v;
+}
+
+template <typename T, bool PLANES>
+__global__ __launch_bounds__(kLongBlock) void ln_long_fwd(const T* __restrict__ x, const void* __restrict__ w, const void* __restrict__ b, bool w_f32, long positions, long C, long inner,
+                                                          long x_stride, float eps, int relu, T* __restrict__ y,
+                                                          float* __restrict__ mean, float* __restrict__ rstd) {
+    __shared__ float red[kLongBlock / 64 * kLongPos];
+    constexpr int NP = PLANES ? kLongPos : 1, STEP = kLongBlock / NP;
+    const int pl = threadIdx.x % NP, c0 = threadIdx.x / NP;
+    for (long q0 = (long)blockIdx.x * NP; q0 < positions; q0 += (long)gridDim.x * NP) {
+        const bool live = q0 + pl < positions;
+        const long q = live ? q0 + pl : q0, img = q / inner, p = q - img * inner;
+        const T* xp = x + img * x_stride + p;
+        T* yp = y + img * inner * C + p;
+        float s = 0.0f;
+        for (long c = c0; c < C; c += STEP) s += (float)xp[c * inner];
+        const float mu = long_sum<PLANES>(s, red) / (float)C;
+        s = 0.0f;
+        for (long c = c0; c < C; c += STEP) {
+            const float d = (float)xp[c * inner] - mu;
+            s = fmaf(d, d, s);
+        }
+        const float rs = 1.0f / sqrtf(long_sum<PLANES>(s, red) / (float)C + eps);
+        if (live) {
+            for (long c = c0; c < C; c += STEP) {
+                float v = fmaf(((float)xp[c * inner] - mu) * rs, param<T>(w, w_f32, c, 1.0f), param<T>(b, w_f32, c, 0.0f));
+                if (relu) v = passes(v) ? v : 0.0f;
+                yp[c * inner] = (T)v;
+            }
+            if (mean && c0 == 0) {
+                mean[q] = mu;
+                rstd[q] = rs;
+            }
+        }
+    }
+}
+
+template <typename T, bool PLANES>
+__global__ __launch_bounds__(kLongBlock) void ln_long_bwd(const T* __restrict__ dy, const T* __restrict__ x,
+                                                          const void* __restrict__ w, const void* __restrict__ b, bool w_f32,
+                                                          const float* __restrict__ mean, const float* __restrict__ rstd,
+                                                          long positions, long C, long inner, long dy_stride,
+                                                          long x_stride, int relu, T* __restrict__ dx) {
+    __shared__ float red[kLongBlock / 64 * kLongPos];
+    constexpr int NP = PLANES ? kLongPos : 1, STEP = kLongBlock / NP;
+    const int pl = threadIdx.x % NP, c0 = threadIdx.x / NP;
+    for (long q0 = (long)blockIdx.x * NP; q0 < positions; q0 += (long)gridDim.x * NP) {
+        const bool live = q0 + pl < positions;
+        const long q = live ? q0 + pl : q0, img = q / inner, p = q - img * inner;
+        const T* xp = x + img * x_stride + p;
+        const T* gp = dy + img * dy_stride + p;
+        const float mu = mean[q], rs = rstd[q];
+        float s1 = 0.0f, s2 = 0.0f;
+        for (long c = c0; c < C; c += STEP) {
+            const float wc = param<T>(w, w_f32, c, 1.0f), h = ((float)xp[c * inner] - mu) * rs;
+            float g = (float)gp[c * inner];
+            if (relu) g = passes(fmaf(h, wc, param<T>(b, w_f32, c, 0.0f))) ? g : 0.0f;
+            s1 += g * wc;
+            s2 = fmaf(g * wc, h, s2);
+        }
+        const float m1 = long_sum<PLANES>(s1, red) / (float)C, m2 = long_sum<PLANES>(s2, red) / (float)C;
+        if (live) {
+            T* dp = dx + img * inner * C + p;
+            for (long c = c0; c < C; c += STEP) {
+                const float wc = param<T>(w, w_f32, c, 1.0f), h = ((float)xp[c * inner] - mu) * rs;
+                float g = (float)gp[c * inner];
+                if (relu) g = passes(fmaf(h, wc, param<T>(b, w_f32, c, 0.0f))) ? g : 0.0f;
+                dp[c * inner] = (T)(rs * (fmaf(g, wc, -m1) - h * m2));
+            }
+        }
+    }
+}
+
+// Sums over positions for the same case: a workgroup takes one share of the positions (blockIdx.y of gridDim.y) and
+// 256 channels (rows: a lane per channel) or one channel (planes: a lane per position).
+template <typename T, bool PLANES>
+__global__ __launch_bounds__(256) void ln_long_params(const T* __restrict__ dy, const T* __restrict__ x,
+                                                      const void* __restrict__ w, const void* __restrict__ b, bool w_f32,
+                                                      const float* __restrict__ mean, const float* __restrict__ rstd,
+                                                      long positions, long C, long inner, long dy_stride, long x_stride,
+                                                      int relu, float* __restrict__ partial) {
+    __shared__ float red[2][4];
+    const long c = PLANES ? (long)blockIdx.x : (long)blockIdx.x * 256 + threadIdx.x;
+    const long share = (positions + gridDim.y - 1) / gridDim.y;
+    const long lo = (long)blockIdx.y * share, hi = lo + share < positions ? lo + share : positions;
+    float sw = 0.0f, sb = 0.0f;
+    if (c < C) {
+        const float wc = param<T>(w, w_f32, c, 1.0f), bc = param<T>(b, w_f32, c, 0.0f);
+        for (long q = lo + (PLANES ? threadIdx.x : 0); q < hi; q += PLANES ? 256 : 1) {
+            const long img = q / inner, p = q - img * inner;
+            const float h = ((float)x[img * x_stride + c * inner + p] - mean[q]) * rstd[q];
+            float g = (float)dy[img * dy_stride + c * inner + p];
+            if (relu) g = passes(fmaf(h, wc, bc)) ? g : 0.0f;
+            sw = fmaf(g, h, sw);
+            sb += g;
+        }
+    }
+    float* pw = partial + (long)blockIdx.y * 2 * C;
+    if constexpr (PLANES) {
+        sw = wave_sum(sw);
+        sb = wave_sum(sb);
+        if ((threadIdx.x & 63) == 0) {
+            red[0][threadIdx.x >> 6] = sw;
+            red[1][threadIdx.x >> 6] = sb;
+        }
+        __syncthreads();
+        if (threadIdx.x < 2) pw[threadIdx.x * C + c] = (red[threadIdx.x][0] + red[threadIdx.x][1]) + (red[threadIdx.x][2] + red[threadIdx.x][3]);
+    } else if (c < C) {
+        pw[c] = sw;
+        pw[C + c] = sb;
+    }
+}
+
+// dw, db = sums of the n partial sums, 32 columns per workgroup and n shared out over 32 lanes of each
+__global__ __launch_bounds__(1024) void ln_params_sum(const float* __restrict__ partial, int n, long C, int type,
+                                                      void* __restrict__ dw, void* __restrict__ db) {
+    __shared__ float red[32][33];
+    const int col = threadIdx.x & 31, part = threadIdx.x >> 5;
+    const long at = (long)blockIdx.x * 32 + col;                  // over [2][C]
+    float s = 0.0f;
+    if (at < 2 * C)
+        for (int i = part; i < n; i += 32) s += partial[(long)i * 2 * C + at];
+    red[part][col] = s;
+    __syncthreads();
+    if (part == 0 && at < 2 * C) {
+        s = red[0][col];
+#pragma unroll
+        for (int i = 1; i < 32; ++i) s += red[i][col];
+        if (at < C) {
+            if (dw) put_param(dw, type, at, s);
+        } else if (db) {
+            put_param(db, type, at - C, s);
+        }
+    }
+}
+
+// ---- which kernel, how many workgroups ----------------------------------------------------------------------
+constexpr int kRowsMax = kRowElems * 1024;        // rows: the widest that 1024 lanes hold
+constexpr int kPlanesMax = 1024;                  // planes: 128 channel groups of 8
+
+// Workgroups of a launch that loops over its positions: four per compute unit.  A backward launch leaves one row
+// of partial sums per workgroup, which the second launch reads: no more of them than that pays for.
+constexpr long kGroups = 1024;
+
+struct Plan {
+    bool rows, wide;      // wide: vectors along the positions (planes)
+    bool fits;            // the register kernels hold a position's channels
+    int lpr;              // rows: lanes per row
+    int cl, pl;           // planes: channel groups, positions (or vectors of positions) side by side
+    long units;           // workgroups that the positions fill once
+};
+
+int elem_size(int type) { return type == FC3D_F32 ? 4 : 2; }
+
+Plan plan_of(int64_t outer, int64_t C, int64_t inner) {
+    Plan p = {};
+    p.rows = inner == 1;
+    if (p.rows) {
+        p.fits = C <= kRowsMax;
+        p.lpr = C <= 8 * kRowElems ? 8 : C <= 32 * kRowElems ? 32 : C <= 64 * kRowElems ? 64 : C <= 256 * kRowElems ? 256 : 1024;
+        const int rpb = p.lpr < 256 ? 256 / p.lpr : 1;
+        p.units = p.fits ? (outer + rpb - 1) / rpb : outer;
+    } else {
+        p.fits = C <= kPlanesMax;
+        // a plane that is no multiple of the vector leaves part of its last vector empty: single values where that
+        // would idle a quarter of the lanes
+        const int64_t nv = (inner + kVec - 1) / kVec;
+        p.wide = inner * 4 >= nv * kVec * 3;
+        p.cl = C <= 8 ? 1 : C <= 32 ? 4 : C <= 128 ? 16 : C <= 512 ? 64 : 128;
+        p.pl = p.cl <= 16 ? 256 / p.cl : p.cl == 64 ? 8 : 4;
+        const int64_t nq = p.wide ? outer * nv : outer * inner;
+        p.units = p.fits ? (nq + p.pl - 1) / p.pl : (outer * inner + kLongPos - 1) / kLongPos;
+    }
+    return p;
+}
+
+unsigned groups_of(const Plan& p) {
+    const long most = p.fits ? kGroups : 4096;
+    return (unsigned)(p.units < most ? p.units : most);
+}
+constexpr int kLongShares = 64;
+int64_t partials_of(const Plan& p) { return p.fits ? (int64_t)groups_of(p) : kLongShares; }
+
+int check_sizes(int x_type, int w_type, int64_t outer, int64_t C, int64_t inner) {
+    if (x_type < FC3D_F32 || x_type > FC3D_F16) return FC3D_EINVAL;
+    if (w_type != x_type && w_type != FC3D_F32) return FC3D_EINVAL;
+    if (outer < 0 || C <= 0 || inner <= 0) return FC3D_EINVAL;
+    const int64_t most = (int64_t)1 << 31;
+    if (C >= (1 << 24) || inner >= most || outer >= most || (outer > 0 && outer * inner >= most)) return FC3D_ERANGE;
+    return FC3D_OK;
+}
+
+bool aligned_to(const void* p, int bytes) { return (reinterpret_cast<uintptr_t>(p) & (uintptr_t)(bytes - 1)) == 0; }
+
+struct FwdArgs {
+    hipStream_t s;
+    const void *x, *w, *b;
+    bool w_f32;
+    int64_t outer, C, inner, x_stride;
+    float eps;
+    int relu;
+    void* y;
+    float *mean, *rstd;
+};
+struct BwdArgs {
+    hipStream_t s;
+    const void *dy, *x, *w, *b;
+    bool w_f32;
+    const float *mean, *rstd;
+    int64_t outer, C, inner, dy_stride, x_stride;
+    int relu;
+    void* dx;
+    float* partial;       // NULL: no parameter asks for a gradient
+};
+
+template <typename T, int LPR, int BLOCK>
+int rows_launch(const FwdArgs& a, unsigned groups) {
+    FC3D_LAUNCH("layer_norm_fwd", (ln_rows_fwd<T, LPR, BLOCK>), dim3(groups), dim3(BLOCK), 0, a.s, (const T*)a.x, a.w, a.b,
+                a.w_f32, (long)a.outer, (int)a.C, (long)a.x_stride, a.eps, a.relu, (T*)a.y, a.mean, a.rstd);
+    return FC3D_OK;
+}
+template <typename T, int LPR, int BLOCK>
+int rows_launch(const BwdArgs& a, unsigned groups) {
+    FC3D_LAUNCH("layer_norm_bwd", (ln_rows_bwd<T, LPR, BLOCK>), dim3(groups), dim3(BLOCK), 0, a.s, (const T*)a.dy,
+                (const T*)a.x, a.w, a.b, a.w_f32, a.mean, a.rstd, (long)a.outer, (int)a.C, (long)a.dy_stride,
+                (long)a.x_stride, a.relu, (T*)a.dx, a.partial);
+    return FC3D_OK;
+}
+template <typename T, int V, int CL, int PL>
+int planes_launch(const FwdArgs& a, unsigned groups) {
+    const unsigned nvec = (unsigned)((a.inner + V - 1) / V), nq = (unsigned)(a.outer * nvec);
+    FC3D_LAUNCH("layer_norm_fwd", (ln_planes_fwd<T, V, CL, PL, 8>), dim3(groups), dim3(CL * PL), 0, a.s, (const T*)a.x, a.w,
+                a.b, a.w_f32, nq, nvec, (int)a.C, (long)a.inner, (long)a.x_stride, a.eps, a.relu, (T*)a.y, a.mean, a.rstd);
+    return FC3D_OK;
+}
+template <typename T, int V, int CL, int PL>
+int planes_launch(const BwdArgs& a, unsigned groups) {
+    const unsigned nvec = (unsigned)((a.inner + V - 1) / V), nq = (unsigned)(a.outer * nvec);
+    FC3D_LAUNCH("layer_norm_bwd", (ln_planes_bwd<T, V, CL, PL, 8>), dim3(groups), dim3(CL * PL), 0, a.s, (const T*)a.dy,
+                (const T*)a.x, a.w, a.b, a.w_f32, a.mean, a.rstd, nq, nvec, (int)a.C, (long)a.inner, (long)a.dy_stride,
+                (long)a.x_stride, a.relu, (T*)a.dx, a.partial);
+    return FC3D_OK;
+}
+template <typename T, int V, typename A>
+int planes_of(const A& a, const Plan& p, unsigned groups) {
+    switch (p.cl) {
+        case 1: return planes_launch<T, V, 1, 256>(a, groups);
+        case 4: return planes_launch<T, V, 4, 64>(a, groups);
+        case 16: return planes_launch<T, V, 16, 16>(a, groups);
+        case 64: return planes_launch<T, V, 64, 8>(a, groups);
+        default: return planes_launch<T, V, 128, 4>(a, groups);
+    }
+}
+// The register kernel of a plan, forward or backward by the arguments' type
+template <typename T, typename A>
+int registers_of(const A& a, const Plan& p) {
+    const unsigned groups = groups_of(p);
+    if (!p.rows) return p.wide ? planes_of<T, kVec>(a, p, groups) : planes_of<T, 1>(a, p, groups);
+    switch (p.lpr) {
+        case 8: return rows_launch<T, 8, 256>(a, groups);
+        case 32: return rows_launch<T, 32, 256>(a, groups);
+        case 64: return rows_launch<T, 64, 256>(a, groups);
+        case 256: return rows_launch<T, 256, 256>(a, groups);
+        default: return rows_launch<T, 1024, 1024>(a, groups);
+    }
+}
+
+template <typename T, bool PLANES>
+int long_of(const FwdArgs& a, const Plan& p) {
+    FC3D_LAUNCH("layer_norm_fwd", (ln_long_fwd<T, PLANES>), dim3(groups_of(p)), dim3(kLongBlock), 0, a.s, (const T*)a.x, a.w,
+                a.b, a.w_f32, (long)(a.outer * a.inner), (long)a.C, (long)a.inner, (long)a.x_stride, a.eps, a.relu, (T*)a.y,
+                a.mean, a.rstd);
+    return FC3D_OK;
+}
+template <typename T, bool PLANES>
+int long_of(const BwdArgs& a, const Plan& p) {
+    const T *dy = (const T*)a.dy, *x = (const T*)a.x;
+    const long positions = (long)(a.outer * a.inner);
+    if (a.dx)
+        FC3D_LAUNCH("layer_norm_bwd", (ln_long_bwd<T, PLANES>), dim3(groups_of(p)), dim3(kLongBlock), 0, a.s, dy, x, a.w, a.b,
+                    a.w_f32, a.mean, a.rstd, positions, (long)a.C, (long)a.inner, (long)a.dy_stride, (long)a.x_stride,
+                    a.relu, (T*)a.dx);
+    if (a.partial)
+        FC3D_LAUNCH("layer_norm_params", (ln_long_params<T, PLANES>),
+                    dim3((unsigned)(PLANES ? a.C : (a.C + 255) / 256), kLongShares), dim3(256), 0, a.s, dy, x, a.w, a.b,
+                    a.w_f32, a.mean, a.rstd, positions, (long)a.C, (long)a.inner, (long)a.dy_stride, (long)a.x_stride,
+                    a.relu, a.partial);
+    return FC3D_OK;
+}
+
+template <typename T, typename A>
+int kernel_of(const A& a, const Plan& p) {
+    if (p.fits) return registers_of<T>(a, p);
+    return p.rows ? long_of<T, false>(a, p) : long_of<T, true>(a, p);
+}
+template <typename A>
+int type_of(const A& a, const Plan& p, int x_type) {
+    return x_type == FC3D_F32 ? kernel_of<float>(a, p) : x_type == FC3D_BF16 ? kernel_of<bf16>(a, p) : kernel_of<f16>(a, p);
+}
+
+__global__ __launch_bounds__(256) void ln_params_clear(long C, int type, void* __restrict__ dw, void* __restrict__ db) {
+    const long i = (long)blockIdx.x * 256 + threadIdx.x;
+    if (i < C) {
+        if (dw) put_param(dw, type, i, 0.0f);
+        if (db) put_param(db, type, i, 0.0f);
+    }
+}
+
+}  // namespace
+}  // namespace fc3d
+
+using namespace fc3d;
+
+extern "C" int fc3d_layer_norm_fwd(void* stream, const void* x, int x_type, const void* weight, const void* bias, int w_type,
+                                   int64_t outer, int64_t channels, int64_t inner, int64_t x_stride, float eps, int relu,
+                                   void* y, float* mean, float* rstd) {
+    if (const int rc = check_sizes(x_type, w_type, outer, channels, inner)) return rc;
+    if (!(eps >= 0.0f) || (mean == nullptr) != (rstd == nullptr)) return FC3D_EINVAL;
+    if (outer == 0) return FC3D_OK;
+    if (!x || !y || x_stride < 0) return FC3D_EINVAL;
+    if (!aligned_to(x, elem_size(x_type)) || !aligned_to(y, elem_size(x_type)) || !aligned_to(weight, elem_size(w_type)) ||
+        !aligned_to(bias, elem_size(w_type)) || !aligned_to(mean, 4) || !aligned_to(rstd, 4))
+        return FC3D_EALIGN;
+    const FwdArgs a = {(hipStream_t)stream, x, weight, bias, w_type == FC3D_F32, outer, channels, inner, x_stride, eps, relu,
+                       y, mean, rstd};
+    return type_of(a, plan_of(outer, channels, inner), x_type);
+}
+
+extern "C" size_t fc3d_layer_norm_bwd_workspace(int x_type, int64_t outer, int64_t channels, int64_t inner) {
+    if (check_sizes(x_type, x_type, outer, channels, inner) != FC3D_OK || outer == 0) return 0;
+    return (size_t)partials_of(plan_of(outer, channels, inner)) * 2 * (size_t)channels * sizeof(float);
+}
+
+extern "C" int fc3d_layer_norm_bwd(void* stream, const void* dy, const void* x, int x_type, const void* weight,
+                                   const void* bias, int w_type, const float* mean, const float* rstd, int64_t outer,
+                                   int64_t channels, int64_t inner, int64_t dy_stride, int64_t x_stride, int relu, void* dx,
+                                   void* dw, void* db, void* workspace) {
+    if (const int rc = check_sizes(x_type, w_type, outer, channels, inner)) return rc;
+    if (!dx && !dw && !db) return FC3D_OK;
+    if (!aligned_to(dw, elem_size(w_type)) || !aligned_to(db, elem_size(w_type))) return FC3D_EALIGN;
+    if (outer == 0) {
+        if (!dw && !db) return FC3D_OK;
+        FC3D_LAUNCH("layer_norm_params", ln_params_clear, dim3((unsigned)((channels + 255) / 256)), dim3(256), 0,
+                    (hipStream_t)stream, (long)channels, w_type, dw, db);
+        return FC3D_OK;
+    }
+    if (!dy || !x || !mean || !rstd || dy_stride < 0 || x_stride < 0 || ((dw || db) && !workspace)) return FC3D_EINVAL;
+    if (!aligned_to(dy, elem_size(x_type)) || !aligned_to(x, elem_size(x_type)) || !aligned_to(dx, elem_size(x_type)) ||
+        !aligned_to(weight, elem_size(w_type)) || !aligned_to(bias, elem_size(w_type)) || !aligned_to(mean, 4) ||
+        !aligned_to(rstd, 4) || !aligned_to(workspace, 4))
+        return FC3D_EALIGN;
+    const BwdArgs a = {(hipStream_t)stream, dy, x, weight, bias, w_type == FC3D_F32, mean, rstd, outer, channels, inner,
+                       dy_stride, x_stride, relu, dx, dw || db ? (float*)workspace : nullptr};
+    const Plan p = plan_of(outer, channels, inner);
+    const int rc = type_of(a, p, x_type);
+    if (rc != FC3D_OK || !a.partial) return rc;
+    FC3D_LAUNCH("layer_norm_params_sum", ln_params_sum, dim3((unsigned)((2 * channels + 31) / 32)), dim3(1024), 0, a.s,
+                a.partial, (int)partials_of(p), (long)channels, w_type, dw, db);
+    return FC3D_OK;
+}

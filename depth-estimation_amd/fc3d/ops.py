@@ -1140,3 +1140,180 @@ def box_filter(img: torch.Tensor, k: int, mode: str = "mean", c: float = 0.0) ->
         _check(_lib.fc3d_box_filter(_stream(), src.data_ptr(), B, H, W, int(k), m, float(c), out.data_ptr()),
                "fc3d_box_filter")
     return out
+
+
+# --------------------------------------------------------------------------- #
+# training the reconstruction networks
+# --------------------------------------------------------------------------- #
+_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}     # FC3D_F32 / FC3D_BF16 / FC3D_F16
+
+
+def _need_gpu_float(t, what):
+    """The element-type code of a GPU tensor in fp32, bf16 or fp16."""
+    if not t.is_cuda:
+        raise RuntimeError("fc3d operators run on the GPU only (got a tensor on %s); "
+                           "there is no CPU implementation" % t.device)
+    code = _TYPES.get(t.dtype)
+    if code is None:
+        raise TypeError(f"{what} must be float32, bfloat16 or float16 (got {t.dtype})")
+    return code
+
+
+def _one_stride(sizes, strides):
+    """The element stride of dimensions walked as one index in order, or None where no single stride does."""
+    step, span = None, 1
+    for n, st in zip(reversed(sizes), reversed(strides)):
+        if n == 1:
+            continue
+        if step is None:
+            step = st
+        elif st != step * span:
+            return None
+        span *= n
+    return 0 if step is None else step
+
+
+def _norm_layout(x, dim, last):
+    """(x as the kernels take it, outer, channels, inner, stride of the outer index).  last: the normalised axis is
+    the contiguous one (rows); otherwise the axes behind it are (planes).  Copied where the layout is neither."""
+    sizes, st = tuple(x.shape), x.stride()
+    C = sizes[dim]
+    if last:
+        rest = sizes[:dim] + sizes[dim + 1:]
+        step = _one_stride(rest, st[:dim] + st[dim + 1:]) if st[dim] == 1 or C == 1 else None
+        outer = 1
+        for n in rest:
+            outer *= n
+        if step is None:
+            return x.movedim(dim, -1).contiguous(), outer, C, 1, C
+        return x, outer, C, 1, step
+    outer = inner = 1
+    for n in sizes[:dim]:
+        outer *= n
+    dense = True
+    for n, s in zip(reversed(sizes[dim + 1:]), reversed(st[dim + 1:])):
+        dense = dense and (s == inner or n == 1)
+        inner *= n
+    dense = dense and (st[dim] == inner or C == 1)
+    step = _one_stride(sizes[:dim], st[:dim]) if dense else None
+    if step is None:
+        return x.contiguous(), outer, C, inner, C * inner
+    return x, outer, C, inner, step
+
+
+def _norm_last(x, dim):
+    """Whether the normalised axis is the contiguous one: sequences, channels-last images.  Dimensions of one value
+    say nothing about the order; a dense tensor is read as it is written down."""
+    if dim == x.dim() - 1:
+        return True
+    if x.is_contiguous():
+        return False
+    return x.stride(dim) == 1 and x.shape[dim] > 1
+
+
+def _norm_out(x, dim, last):
+    """An output in the memory order of the input."""
+    if not last or dim == x.dim() - 1:
+        return torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    perm = [i for i in range(x.dim()) if i != dim] + [dim]
+    return torch.empty_permuted(x.shape, perm, dtype=x.dtype, device=x.device)
+
+
+def _norm_forward(x, weight, bias, eps, dim, relu, want_stats):
+    last = _norm_last(x, dim)
+    xd, outer, C, inner, step = _norm_layout(x, dim, last)
+    y = _norm_out(x, dim, last)
+    stats = torch.empty((2, outer * inner), dtype=torch.float32, device=x.device) if want_stats else None
+    p = weight if weight is not None else bias
+    with _on_device(x.device):
+        status = _lib.fc3d_layer_norm_fwd(_stream(), xd.data_ptr(), _TYPES[x.dtype],
+                                          weight.data_ptr() if weight is not None else None,
+                                          bias.data_ptr() if bias is not None else None,
+                                          _TYPES[p.dtype] if p is not None else 0, outer, C, inner, step, eps, relu,
+                                          y.data_ptr(), stats.data_ptr() if want_stats else None,
+                                          stats.data_ptr() + 4 * outer * inner if want_stats else None)
+        if status:
+            _check(status, "fc3d_layer_norm_fwd")
+    return y, xd, stats, last
+
+
+class LayerNormFn(torch.autograd.Function):
+    """layer_norm with its gradients; x, weight [C] or None, bias [C] or None."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps, dim, relu):
+        y, xd, stats, last = _norm_forward(x, weight, bias, eps, dim, relu, True)
+        ctx.save_for_backward(xd, weight, bias if relu else None, stats)
+        ctx.meta = (dim, last, relu, xd is x, None if bias is None else bias.dtype)
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        xd, weight, bias, stats = ctx.saved_tensors
+        dim, last, relu, as_given, bias_dtype = ctx.meta
+        need_x, need_w, need_b = ctx.needs_input_grad[:3]
+        dev = xd.device
+        g, outer, C, inner, g_step = _norm_layout(dy, dim, last)
+        # a copy that the forward made is dense in the order the kernels read
+        x_step = _norm_layout(xd, dim, last)[4] if as_given else C * inner
+        p_dtype = weight.dtype if weight is not None else bias_dtype
+        dx = _norm_out(xd if as_given else dy, dim, last) if need_x else None
+        dw = torch.empty(C, dtype=weight.dtype, device=dev) if need_w else None
+        db = torch.empty(C, dtype=bias_dtype, device=dev) if need_b else None
+        ws = None
+        if need_w or need_b:
+            ws = torch.empty(_lib.fc3d_layer_norm_bwd_workspace(_TYPES[xd.dtype], outer, C, inner) // 4,
+                             dtype=torch.float32, device=dev)
+        with _on_device(dev):
+            _check(_lib.fc3d_layer_norm_bwd(_stream(), g.data_ptr(), xd.data_ptr(), _TYPES[xd.dtype],
+                                            weight.data_ptr() if weight is not None else None,
+                                            bias.data_ptr() if bias is not None else None,
+                                            _TYPES[p_dtype] if p_dtype is not None else 0, stats.data_ptr(),
+                                            stats.data_ptr() + 4 * outer * inner, outer, C, inner, g_step, x_step,
+                                            relu, dx.data_ptr() if need_x else None, dw.data_ptr() if need_w else None,
+                                            db.data_ptr() if need_b else None, ws.data_ptr() if ws is not None else None),
+                   "fc3d_layer_norm_bwd")
+        return dx, dw, db, None, None, None
+
+
+def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None,
+               eps: float = 1e-5, dim: int = -1, relu: bool = False) -> torch.Tensor:
+    """Normalises x over axis `dim` at every other position, then scales and shifts it:
+    y = (x - mean) / sqrt(var + eps) * weight + bias, and max(y, 0) with relu=True (in the same pass).
+
+    x: float32, bfloat16 or float16, any number of axes; dim=-1 for sequences, dim=1 for NCHW images (dense or
+    channels_last).  x is read through its strides where the other axes are walked with one stride, and copied
+    otherwise; y keeps the memory order.  weight, bias: [x.shape[dim]], in x's type or float32 (both alike), or None.
+    Statistics and sums are float32; differentiable once w.r.t. x, weight and bias, bit-reproducible."""
+    code = _need_gpu_float(x, "x")
+    nd = x.dim()
+    if nd == 0 or not -nd <= dim < nd:
+        raise ValueError(f"dim {dim} is no axis of a tensor of shape {tuple(x.shape)}")
+    dim %= nd
+    C = x.shape[dim]
+    if C == 0:
+        raise ValueError("layer_norm over an axis without values")
+    eps = float(eps)
+    if not eps >= 0.0:
+        raise ValueError(f"eps must not be negative (got {eps})")
+    grad = x.requires_grad
+    for t, what in ((weight, "weight"), (bias, "bias")):
+        if t is None:
+            continue
+        if t.device != x.device:
+            raise RuntimeError(f"tensors on different devices: {x.device} and {t.device}")
+        if tuple(t.shape) != (C,):
+            raise ValueError(f"{what} must be [{C}], got {tuple(t.shape)}")
+        if t.dtype != torch.float32 and _TYPES.get(t.dtype) != code:
+            raise TypeError(f"{what} must be float32 or {x.dtype}, got {t.dtype}")
+        grad = grad or t.requires_grad
+    if weight is not None:
+        if bias is not None and bias.dtype != weight.dtype:
+            raise TypeError(f"weight and bias must have the same type, got {weight.dtype} and {bias.dtype}")
+        weight = _dense(weight)
+    if bias is not None:
+        bias = _dense(bias)
+    if grad and torch.is_grad_enabled():
+        return LayerNormFn.apply(x, weight, bias, eps, dim, bool(relu))
+    return _norm_forward(x, weight, bias, eps, dim, bool(relu), False)[0]

@@ -428,6 +428,40 @@ int fc3d_capture_fwd(void *stream, const float *Ip, const float *z_p, const floa
 int fc3d_box_filter(void *stream, const float *in, int B, int H, int W, int k, int mode, float c, float *out);
 
 /* ------------------------------------------------------------------------ */
+/* training the reconstruction networks (no counterpart in the reference: its  */
+/* networks normalise over the batch and its optimiser is torch's Adam)        */
+/* ------------------------------------------------------------------------ */
+
+/* Element types of the entry points below (their tensors come as void*).      */
+#define FC3D_F32 0
+#define FC3D_BF16 1
+#define FC3D_F16 2
+
+/* Layer norm over `channels` values of each position, then optionally max(., 0):
+ *   y = act((x - mean) * rstd * weight + bias),  rstd = 1 / sqrt(mean((x - mean)^2) + eps).
+ * x is [outer][channels][inner] with dense inner dimensions and x_stride elements from one
+ * outer index to the next (0 allowed); y is dense.  inner == 1: the normalised axis is
+ * contiguous (sequences, channels-last images); inner = H*W: the channel axis of NCHW images.
+ * weight, bias: [channels] in w_type, which is x_type or FC3D_F32; either may be NULL (1, 0).
+ * mean, rstd: [outer][inner] fp32 for the backward pass, or both NULL.  Sums and statistics are
+ * fp32.  Pointers need the alignment of their element type only.  outer == 0: nothing is done.
+ * outer * inner < 2^31, channels < 2^24.                                                     */
+int fc3d_layer_norm_fwd(void *stream, const void *x, int x_type, const void *weight, const void *bias, int w_type,
+                        int64_t outer, int64_t channels, int64_t inner, int64_t x_stride, float eps, int relu,
+                        void *y, float *mean, float *rstd);
+
+/* Its backward pass.  dy has the layout of x with its own stride over the outer index; dx (dense),
+ * dw, db ([channels] in w_type) may each be NULL.  workspace: fc3d_layer_norm_bwd_workspace()
+ * bytes, 4-byte aligned, need not be initialised (NULL allowed without dw and db): partial sums per
+ * workgroup, added in a fixed order (bit-reproducible).  relu != 0: dy passes where the
+ * forward's value before the activation is not <= 0, recomputed from x.                      */
+size_t fc3d_layer_norm_bwd_workspace(int x_type, int64_t outer, int64_t channels, int64_t inner);
+int fc3d_layer_norm_bwd(void *stream, const void *dy, const void *x, int x_type, const void *weight, const void *bias,
+                        int w_type, const float *mean, const float *rstd, int64_t outer, int64_t channels,
+                        int64_t inner, int64_t dy_stride, int64_t x_stride, int relu, void *dx, void *dw, void *db,
+                        void *workspace);
+
+/* ------------------------------------------------------------------------ */
 /* optional per-kernel timing (no counterpart in the reference, which has no   */
 /* profiling hooks): while enabled every kernel launch of this library is       */
 /* bracketed by a HIP event pair on the launching stream.  fc3d_profile_report  */
