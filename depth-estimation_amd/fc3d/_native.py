@@ -6,7 +6,7 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import POINTER, c_char_p, c_float, c_int, c_int32, c_int64, c_size_t, c_void_p
+from ctypes import POINTER, c_char_p, c_double, c_float, c_int, c_int32, c_int64, c_size_t, c_void_p
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 # FC3D_LIB_PATH: another build of the same library (kernel tuning experiments)
@@ -85,6 +85,12 @@ SIGNATURES = {
     "fc3d_layer_norm_fwd": (c_int, [P, P, c_int, P, P, c_int, I64, I64, I64, I64, c_float, c_int, P, P, P]),
     "fc3d_layer_norm_bwd_workspace": (c_size_t, [c_int, I64, I64, I64]),
     "fc3d_layer_norm_bwd": (c_int, [P, P, P, c_int, P, P, c_int, P, P, I64, I64, I64, I64, I64, c_int, P, P, P, P]),
+    "fc3d_orthogonalize_workspace": (c_size_t, [c_int, POINTER(c_int64), POINTER(c_int64)]),
+    "fc3d_orthogonalize": (c_int, [P, c_int, POINTER(c_void_p), POINTER(c_void_p), POINTER(c_int64), POINTER(c_int64), c_int,
+                                   c_int, c_double, c_double, c_double, c_double, P]),
+    "fc3d_muon_step": (c_int, [P, c_int, POINTER(c_void_p), POINTER(c_void_p), POINTER(c_void_p), POINTER(c_int64),
+                               POINTER(c_int64), POINTER(c_float), c_int, c_int, c_double, c_int, c_double, c_int, c_double,
+                               c_double, c_double, c_double, P]),
     "fc3d_profile_enable": (c_int, [c_int]),
     "fc3d_profile_report": (c_int, [c_char_p, c_size_t]),
 }

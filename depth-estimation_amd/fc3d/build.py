@@ -17,7 +17,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(os.path.dirname(HERE))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libfc3d_hip.so")
-SOURCES = ["optics.hip", "geometry.hip", "capture.hip", "profile.hip", "norm.hip"]
+SOURCES = ["optics.hip", "geometry.hip", "capture.hip", "profile.hip", "norm.hip", "muon.hip"]
 
 # -ffp-contract=off                         index/mask decisions need the reference's separately rounded ops
 # -fhip-fp32-correctly-rounded-divide-sqrt  IEEE fp32 division (torch's CPU kernels divide exactly)
@@ -27,7 +27,7 @@ FLAGS = ["-O3", "--offload-arch=gfx950", "-fPIC", "-shared", "-std=c++17", "-ffp
 # The training operators' sources keep to one fp32 operation per lane and instruction: the packed forms are taken out
 # of the code generator's choice (the host pass warns that it does not know the feature: harmless).
 _SCALAR_F32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
-SOURCE_FLAGS = {"norm.hip": _SCALAR_F32}
+SOURCE_FLAGS = {"norm.hip": _SCALAR_F32, "muon.hip": _SCALAR_F32}
 
 
 def _hipcc() -> str:

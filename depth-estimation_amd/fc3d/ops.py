@@ -1317,3 +1317,172 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
     if grad and torch.is_grad_enabled():
         return LayerNormFn.apply(x, weight, bias, eps, dim, bool(relu))
     return _norm_forward(x, weight, bias, eps, dim, bool(relu), False)[0]
+
+
+NS_COEFFICIENTS = (3.4445, -4.7750, 2.0315)     # one step takes small singular values up by 3.4, large ones near one
+
+
+def _matrix_order(t):
+    """(rows, cols) of a tensor as a dense row-major matrix in memory: its first axis against all others, in whatever
+    order these lie (a permutation of columns goes through the products unchanged), a transposed matrix as its
+    transpose (so does a transposition); None where the memory is neither."""
+    if t.dim() < 2:
+        raise ValueError(f"a matrix has two axes at least, got a tensor of shape {tuple(t.shape)}")
+    rows = t.shape[0]
+    cols = t.numel() // rows if rows else 0
+    if t.is_contiguous() or rows == 0 or cols == 0:
+        return rows, cols
+    st = t.stride()
+    rest = sorted((s, n) for s, n in zip(st[1:], t.shape[1:]) if n > 1)
+    span = 1
+    for s, n in rest:
+        if s != span:
+            break
+        span *= n
+    else:
+        if rows == 1 or st[0] == cols:
+            return rows, cols
+    if t.dim() == 2 and st[0] == 1 and st[1] == rows:
+        return cols, rows
+    return None
+
+
+def _ns_arguments(steps, coefficients, eps):
+    a, b, c = (float(v) for v in coefficients)
+    steps, eps = int(steps), float(eps)
+    if not 1 <= steps <= 64:
+        raise ValueError(f"steps must be 1..64 (got {steps})")
+    if not eps >= 0.0:
+        raise ValueError(f"eps must not be negative (got {eps})")
+    if not np.isfinite((a, b, c)).all():
+        raise ValueError(f"coefficients must be finite (got {coefficients})")
+    return steps, a, b, c, eps
+
+
+def _pointers(tensors):
+    return (ctypes.c_void_p * len(tensors))(*[t.data_ptr() for t in tensors])
+
+
+def _ns_workspace(rows, cols, dev):
+    n = len(rows)
+    r, c = (ctypes.c_int64 * n)(*rows), (ctypes.c_int64 * n)(*cols)
+    nbytes = _lib.fc3d_orthogonalize_workspace(n, r, c)
+    if nbytes == 0:
+        raise ValueError("matrices beyond what the kernels index")
+    return r, c, torch.empty(nbytes, dtype=torch.uint8, device=dev)
+
+
+def _ns_status(status, what, coefficients):
+    if status == -2:
+        raise ValueError(f"{what}: coefficients {tuple(coefficients)} let the singular values grow, or sizes beyond the kernels'")
+    _check(status, what)
+
+
+def orthogonalize(g, steps: int = 5, coefficients=NS_COEFFICIENTS, eps: float = 1e-7):
+    """Newton-Schulz orthogonalisation of a matrix, or of each of a list of matrices in one sequence of launches:
+    X = g / (|g|_F + eps), then `steps` times X <- a X + (b A + c A A) X with A = X X^T, coefficients = (a, b, c).
+    With the default ones the singular values of g end near one, its singular vectors are kept.
+
+    g: float32, bfloat16 or float16 tensors of two axes or more on one GPU (a convolution's weight is
+    [out, in * kh * kw]), any sizes and strides; results in their shapes and types.  The products keep the accuracy
+    of fp32 whatever the type.  No gradient."""
+    single = isinstance(g, torch.Tensor)
+    mats = [g] if single else list(g)
+    steps, a, b, c, eps = _ns_arguments(steps, coefficients, eps)
+    groups: dict = {}
+    out = [None] * len(mats)
+    for i, t in enumerate(mats):
+        code = _need_gpu_float(t, "matrices")
+        if t.device != mats[0].device:
+            raise RuntimeError(f"tensors on different devices: {mats[0].device} and {t.device}")
+        t = t.detach()
+        order = _matrix_order(t)
+        if order is None:
+            t = t.contiguous()
+            order = _matrix_order(t)
+        out[i] = torch.empty_like(t)
+        if t.numel():
+            groups.setdefault(code, []).append((t, out[i], order))
+    for code, items in groups.items():
+        dev = mats[0].device
+        r, cl, ws = _ns_workspace([o[0] for _, _, o in items], [o[1] for _, _, o in items], dev)
+        with _on_device(dev):
+            status = _lib.fc3d_orthogonalize(_stream(), len(items), _pointers([t for t, _, _ in items]),
+                                             _pointers([o for _, o, _ in items]), r, cl, code, steps, a, b, c, eps,
+                                             ws.data_ptr())
+        _ns_status(status, "fc3d_orthogonalize", coefficients)
+    return out[0] if single else out
+
+
+def muon_scale(shape, scale: str) -> float:
+    """The factor on the learning rate of a weight of this shape (rows: the first axis, cols: all others):
+    "spectral" sqrt(max(1, rows / cols)), "rms" 0.2 sqrt(max(rows, cols)) (steps as large as Adam's usually are)."""
+    rows = shape[0]
+    cols = 1
+    for n in shape[1:]:
+        cols *= n
+    if scale == "spectral":
+        return max(1.0, rows / max(1, cols)) ** 0.5
+    if scale == "rms":
+        return 0.2 * max(rows, cols) ** 0.5
+    raise ValueError(f"unknown scale {scale!r} (spectral or rms)")
+
+
+@torch.no_grad()
+def muon_step(params, grads, momenta, lr: float = 0.02, momentum: float = 0.95, nesterov: bool = True,
+              weight_decay: float = 0.0, steps: int = 5, coefficients=NS_COEFFICIENTS, eps: float = 1e-7,
+              scale: str = "spectral") -> None:
+    """One Muon step, in place, for lists of weights, their gradients and fp32 momenta:
+    m <- momentum m + (1 - momentum) g;  u = (1 - momentum) g + momentum m with nesterov, else m;
+    w <- (1 - lr weight_decay) w - lr muon_scale(w.shape, scale) orthogonalize(u).
+
+    params: float32, bfloat16 or float16 tensors of two axes or more, dense in memory (the first axis outermost, or a
+    transposed matrix), on one GPU, each of them once.  grads: the same shapes, any of the three types; copied where
+    they lie in another order than their weight.  momenta: float32, in their weight's memory order."""
+    params, grads, momenta = list(params), list(grads), list(momenta)
+    if not len(params) == len(grads) == len(momenta):
+        raise ValueError(f"{len(params)} weights, {len(grads)} gradients, {len(momenta)} momenta")
+    steps, a, b, c, eps = _ns_arguments(steps, coefficients, eps)
+    lr, momentum, weight_decay = float(lr), float(momentum), float(weight_decay)
+    if not 0.0 <= momentum <= 1.0:
+        raise ValueError(f"momentum must be in [0, 1] (got {momentum})")
+    decay = 1.0 - lr * weight_decay
+    if not (np.isfinite(lr) and np.isfinite(decay)):
+        raise ValueError(f"lr and weight_decay must be finite (got {lr}, {weight_decay})")
+    written = set()
+    groups: dict = {}
+    for p, g, m in zip(params, grads, momenta):
+        code, g_code = _need_gpu_float(p, "weights"), _need_gpu_float(g, "gradients")
+        if m.dtype != torch.float32:
+            raise TypeError(f"momenta must be float32 (got {m.dtype})")
+        if not (p.device == g.device == m.device == params[0].device):
+            raise RuntimeError(f"tensors on different devices: {params[0].device}, {p.device}, {g.device}, {m.device}")
+        if not p.shape == g.shape == m.shape:
+            raise ValueError(f"a weight {tuple(p.shape)} with a gradient {tuple(g.shape)} and a momentum {tuple(m.shape)}")
+        order = _matrix_order(p)
+        if order is None:
+            raise ValueError(f"a weight of shape {tuple(p.shape)} and strides {p.stride()} is not dense")
+        factor = muon_scale(p.shape, scale)
+        if p.numel() == 0:
+            continue
+        if m.stride() != p.stride() and not (m.is_contiguous() and p.is_contiguous()):
+            raise ValueError(f"a momentum of strides {m.stride()} beside a weight of strides {p.stride()}")
+        if p.data_ptr() in written or m.data_ptr() in written:
+            raise ValueError("a weight or momentum is in the list twice")
+        written.update((p.data_ptr(), m.data_ptr()))
+        if g.stride() != p.stride() and not (g.is_contiguous() and p.is_contiguous()):
+            g = torch.empty_like(p, dtype=g.dtype).copy_(g)
+        groups.setdefault((code, g_code), []).append((p, g, m, order, lr * factor))
+    # nothing is written before every list has its workspace
+    spaces = [_ns_workspace([it[3][0] for it in items], [it[3][1] for it in items], params[0].device)
+              for items in groups.values()]
+    for ((code, g_code), items), (r, cl, ws) in zip(groups.items(), spaces):
+        dev = params[0].device
+        with _on_device(dev):
+            status = _lib.fc3d_muon_step(_stream(), len(items), _pointers([it[0] for it in items]),
+                                         _pointers([it[1] for it in items]), _pointers([it[2] for it in items]), r, cl,
+                                         (ctypes.c_float * len(items))(*[it[4] for it in items]), code, g_code, momentum,
+                                         int(bool(nesterov)), decay, steps, a, b, c, eps, ws.data_ptr())
+        _ns_status(status, "fc3d_muon_step", coefficients)
+        # the kernels wrote behind torch's back: autograd's check of saved tensors has to see it
+        torch.autograd.graph.increment_version([t for it in items for t in (it[0], it[2])])

@@ -461,6 +461,31 @@ int fc3d_layer_norm_bwd(void *stream, const void *dy, const void *x, int x_type,
                         int64_t inner, int64_t dy_stride, int64_t x_stride, int relu, void *dx, void *dw, void *db,
                         void *workspace);
 
+/* Orthogonalised updates by Newton-Schulz products, for `count` matrices at once:
+ *   X = G / (|G|_F + eps), then `steps` times  X <- a X + (b A + c A A) X  with A = X X^T
+ * (of the transpose where rows > cols), and out = X.  Evaluated in the Gram form with every
+ * operand a pair of fp16 values and fp32 sums: the accuracy of fp32 products.  HOST arrays:
+ * g, out (device pointers to dense row-major [rows][cols] tensors of `type`; out[i] may be
+ * g[i]), rows, cols; they may be freed after the call.  A matrix must have a row and a column.
+ * FC3D_ERANGE: sizes beyond 2^24, or coefficients that let singular values grow (beyond 16).
+ * workspace: fc3d_orthogonalize_workspace() bytes, 256-byte aligned, need not be initialised;
+ * calls that may run at the same time need one each.                                          */
+size_t fc3d_orthogonalize_workspace(int count, const int64_t *rows, const int64_t *cols);
+int fc3d_orthogonalize(void *stream, int count, const void *const *g, void *const *out, const int64_t *rows,
+                       const int64_t *cols, int type, int steps, double a, double b, double c, double eps,
+                       void *workspace);
+
+/* One optimiser step on `count` matrices:
+ *   m <- momentum m + (1 - momentum) g;  u = (1 - momentum) g + momentum m if nesterov, else m;
+ *   w <- decay w - lr[i] O(u),  O as in fc3d_orthogonalize.
+ * HOST arrays as there; params in param_type, grads in grad_type, momenta fp32, all dense
+ * row-major [rows][cols]; lr: one factor per matrix.  No matrix may appear twice.  The workspace
+ * is that of fc3d_orthogonalize for the same sizes.                                           */
+int fc3d_muon_step(void *stream, int count, void *const *params, const void *const *grads, float *const *momenta,
+                   const int64_t *rows, const int64_t *cols, const float *lr, int param_type, int grad_type,
+                   double momentum, int nesterov, double decay, int steps, double a, double b, double c, double eps,
+                   void *workspace);
+
 /* ------------------------------------------------------------------------ */
 /* optional per-kernel timing (no counterpart in the reference, which has no   */
 /* profiling hooks): while enabled every kernel launch of this library is       */

@@ -1,0 +1,400 @@
+"""Newton-Schulz orthogonalisation and the Muon step (fc3d.ops.orthogonalize / muon_step, fc3d.optim.Muon) against
+their definition in 64 bits.
+
+Bounds, in the 2-norm of the whole result relative to the result's.  The operands are pairs of fp16 values: an operand
+is off by 2^-23 of itself at most, the dropped product of the two lo planes by 2^-24 of the product: five half steps of
+fp32 where fp32 products take their operands as they are and round in the sums alike.  So the error may be that of the
+fp32 evaluation, taken on the same input, four times (its own share included), plus 2^-20 where that happens to be zero.
+A 16-bit result adds its rounding, half a step, and the Gram form in one segment: a value of A is off by 2^-23 of
+itself, A's spectrum by at most 2 * 2^-23 times a row's norm, which is 1 / sqrt(m) where the rows share the norm; a
+singular value s of the result by s dP/dlambda <= 2.6e4 times that (the default polynomial's five steps): 6e-3 / sqrt(m)."""
+import math
+
+import pytest
+import torch
+
+COEFFS = (3.4445, -4.7750, 2.0315)
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+
+
+def ns(g, dt, steps=5, coeffs=COEFFS, eps=1e-7):
+    """The definition, evaluated in type dt on the CPU."""
+    a, b, c = coeffs
+    x = g.to(dt).reshape(g.shape[0], -1)
+    x = x / (x.norm() + eps)
+    tall = x.shape[0] > x.shape[1]
+    if tall:
+        x = x.t()
+    for _ in range(steps):
+        s = x @ x.t()
+        x = a * x + (b * s + c * (s @ s)) @ x
+    return (x.t() if tall else x).reshape(g.shape)
+
+
+def update(shape, kind, seed, dt=F32):
+    g = torch.Generator().manual_seed(seed)
+    m, n = shape[0], math.prod(shape[1:])
+    x = torch.randn(m, n, generator=g)
+    if kind == "low":                                # a few strong directions over a noise floor
+        k = min(m, n, 4)
+        x = torch.randn(m, k, generator=g) @ torch.randn(k, n, generator=g) + 0.01 * x
+    return (1e-3 * x).reshape(shape).to(dt)
+
+
+def bound(g, ref, steps=5, coeffs=COEFFS, eps=1e-7, dt=None):
+    dt = g.dtype if dt is None else dt
+    e32 = (ns(g, F32, steps, coeffs, eps).double() - ref).norm() / ref.norm()
+    tol = 4 * float(e32) + 2.0 ** -20
+    if dt != F32:
+        tol += torch.finfo(dt).eps / 2 + 6e-3 / math.sqrt(min(g.shape[0], math.prod(g.shape[1:])))
+    return tol
+
+
+def near(got, g, what, steps=5, coeffs=COEFFS, eps=1e-7):
+    ref = ns(g, torch.float64, steps, coeffs, eps)
+    assert got.shape == ref.shape and got.dtype == g.dtype, what
+    off = float((got.cpu().double() - ref).norm() / ref.norm())
+    tol = bound(g, ref, steps, coeffs, eps)
+    assert off <= tol, f"{what}: {off:.2e} of the result, {tol:.2e} allowed"
+
+
+# ---- on the CPU -------------------------------------------------------------------------------------------------
+
+def test_refusals():
+    import ctypes
+    from fc3d import _native, ops, optim
+    with pytest.raises(RuntimeError, match="GPU only"):
+        ops.orthogonalize(torch.zeros(4, 4))
+    with pytest.raises(RuntimeError, match="GPU only"):
+        ops.muon_step([torch.zeros(4, 4)], [torch.zeros(4, 4)], [torch.zeros(4, 4)])
+    with pytest.raises(ValueError):
+        ops.muon_step([torch.zeros(4, 4)], [], [])
+    assert ops.orthogonalize([]) == []
+    ops.muon_step([], [], [])
+    for bad in (dict(steps=0), dict(steps=65), dict(eps=-1.0), dict(coefficients=(float("nan"), 0, 0))):
+        with pytest.raises(ValueError):
+            ops.orthogonalize([], **bad)
+    for bad in (dict(momentum=1.5), dict(lr=float("inf")), dict(weight_decay=float("nan"))):
+        with pytest.raises(ValueError):
+            ops.muon_step([], [], [], **bad)
+    p = torch.nn.Parameter(torch.zeros(4, 4))
+    for bad in (dict(lr=-1.0), dict(momentum=-0.1), dict(weight_decay=-1.0), dict(steps=0), dict(scale="other")):
+        with pytest.raises(ValueError):
+            optim.Muon([p], **bad)
+    with pytest.raises(ValueError, match="two axes"):
+        optim.Muon([torch.nn.Parameter(torch.zeros(4))])
+    lib = _native.load()
+    I64, VP = ctypes.c_int64, ctypes.c_void_p
+    one = 256
+
+    def call(g=one, out=one, rows=4, cols=4, t=0, steps=5, co=COEFFS, eps=1e-7, ws=one, count=1):
+        return lib.fc3d_orthogonalize(None, count, (VP * 1)(g), (VP * 1)(out), (I64 * 1)(rows), (I64 * 1)(cols), t, steps, *co, eps, ws)
+    assert call(count=0) == 0 and call(count=-1) == -1
+    assert call(g=None) == -1 and call(out=None) == -1 and call(ws=None) == -1 and call(rows=0) == -1 and call(cols=-3) == -1
+    assert call(t=3) == -1 and call(steps=0) == -1 and call(steps=65) == -1 and call(eps=-1.0) == -1 and call(eps=float("nan")) == -1
+    assert call(co=(float("inf"), 0, 0)) == -1
+    assert call(co=(30.0, 0.0, 0.0)) == -2 and call(co=(2.0, 2.0, 2.0)) == -2           # singular values grow
+    assert call(rows=1 << 24) == -2 and call(rows=1 << 20, cols=1 << 20) == -2
+    assert call(g=one + 2) == -3 and call(out=one + 1, t=1) == -3 and call(ws=one + 16) == -3
+
+    def step(mom=one, lr=0.1, beta=0.95, decay=1.0):
+        return lib.fc3d_muon_step(None, 1, (VP * 1)(one), (VP * 1)(one), (VP * 1)(mom) if mom != 0 else None, (I64 * 1)(4), (I64 * 1)(4),
+                                  (ctypes.c_float * 1)(lr), 0, 0, beta, 1, decay, 5, *COEFFS, 1e-7, None)
+    assert step(mom=0) == -1 and step(mom=None) == -1 and step(beta=1.1) == -1 and step(beta=float("nan")) == -1
+    assert step(decay=float("inf")) == -1 and step() == -1                               # no workspace
+    ws = lambda r, c: lib.fc3d_orthogonalize_workspace(1, (I64 * 1)(r), (I64 * 1)(c))  # noqa: E731
+    assert ws(0, 4) == 0 and ws(1 << 24, 4) == 0 and ws(4, 4) > 0 and ws(64, 64) == ws(4, 4)
+    assert lib.fc3d_orthogonalize_workspace(0, None, None) == 0
+
+
+def test_memory_orders_of_matrices():
+    from fc3d.ops import _matrix_order, muon_scale
+    t = torch.zeros(6, 5, 3, 3)
+    assert _matrix_order(t) == (6, 45)
+    assert _matrix_order(t.contiguous(memory_format=torch.channels_last)) == (6, 45)
+    assert _matrix_order(torch.zeros(6, 4).t()) == (6, 4)                    # as the matrix that lies in memory
+    assert _matrix_order(torch.zeros(6, 8)[:, :4]) is None and _matrix_order(torch.zeros(1, 4).expand(6, 4)) is None
+    assert _matrix_order(torch.zeros(6, 1, 4).transpose(0, 2)) is None
+    assert _matrix_order(torch.zeros(0, 4)) == (0, 0) and _matrix_order(torch.zeros(1, 4).t()) == (4, 1)
+    with pytest.raises(ValueError):
+        _matrix_order(torch.zeros(4))
+    assert muon_scale((64, 16), "spectral") == 2.0 and muon_scale((16, 4, 4), "spectral") == 1.0
+    assert muon_scale((4, 25, 4), "rms") == 2.0
+    with pytest.raises(ValueError):
+        muon_scale((4, 4), "x")
+
+
+def test_five_steps_bring_singular_values_near_one():
+    """What the definition is for; the coefficients' polynomial stays within 0.67 .. 1.21 from 0.02 on."""
+    s = torch.linspace(0.02, 1, 1000, dtype=torch.float64)
+    a, b, c = COEFFS
+    for _ in range(5):
+        s = a * s + b * s ** 3 + c * s ** 5
+    assert 0.66 < float(s.min()) and float(s.max()) < 1.21
+    x = ns(update((24, 60), "gauss", 0), torch.float64)
+    assert torch.linalg.svdvals(x).min() > 0.6
+
+
+# ---- on the GPU -------------------------------------------------------------------------------------------------
+
+gpu = pytest.mark.gpu
+
+SHAPES = [(1, 1), (1, 7), (7, 1), (2, 3), (9, 32), (32, 9), (64, 64), (64, 65), (65, 64), (63, 129), (130, 500), (300, 77),
+          (100, 1000), (256, 256), (32, 32, 3, 3), (512, 700), (128, 128, 3, 3), (700, 65, 2)]
+
+
+@gpu
+@pytest.mark.parametrize("dt", [F32, BF16, F16], ids=lambda t: str(t).replace("torch.", ""))
+@pytest.mark.parametrize("kind", ["gauss", "low"])
+def test_orthogonalize_against_definition(dt, kind):
+    from fc3d import ops
+    gs = [update(s, kind, 100 + i, dt) for i, s in enumerate(SHAPES)]
+    together = ops.orthogonalize([g.cuda() for g in gs])
+    for g, x, shape in zip(gs, together, SHAPES):
+        near(x, g, f"{shape} {dt} {kind}")
+        assert torch.equal(ops.orthogonalize(g.cuda()), x), shape      # alone: the same bits
+
+
+@gpu
+@pytest.mark.parametrize("dt", [F32, BF16])
+@pytest.mark.parametrize("steps", [1, 2, 3, 4, 6, 7, 12])
+def test_other_step_counts_and_coefficients(dt, steps):
+    from fc3d import ops
+    for shape in ((48, 60), (40, 200)):
+        for coeffs in (COEFFS, (1.875, -1.25, 0.375)):                 # the second: cubic convergence to one
+            g = update(shape, "gauss", steps, dt)
+            near(ops.orthogonalize(g.cuda(), steps=steps, coefficients=coeffs), g, f"{shape} {steps} {coeffs}", steps, coeffs)
+
+
+@gpu
+def test_scales_zeros_and_special_values():
+    from fc3d import ops
+    g = update((40, 100), "gauss", 5)
+    x = ops.orthogonalize(g.cuda())
+    for f in (2.0 ** 100, 2.0 ** 40, 2.0 ** -10):                       # only the eps feels the scale
+        assert float((ops.orthogonalize((g * f).cuda(), eps=0.0) - ops.orthogonalize(g.cuda(), eps=0.0)).abs().max()) <= 2.0 ** -20
+    h = update((40, 100), "gauss", 5, BF16)
+    assert torch.equal(ops.orthogonalize((h * 2.0 ** 90).cuda(), eps=0.0), ops.orthogonalize(h.cuda(), eps=0.0))
+    for dt in (F32, BF16, F16):
+        z = torch.zeros(33, 70, dtype=dt, device="cuda")
+        assert not ops.orthogonalize(z).any()
+        assert bool(torch.isnan(ops.orthogonalize(z, eps=0.0)).all())
+        for bad in (float("nan"), float("inf")):
+            t = update((33, 70), "gauss", 6, dt).cuda()
+            t[3, 4] = bad
+            two = ops.orthogonalize([t, update((33, 70), "gauss", 6, dt).cuda()])
+            assert bool(torch.isnan(two[0]).all()) and bool(torch.isfinite(two[1]).all())      # its own matrix alone
+    assert torch.equal(ops.orthogonalize(g.cuda()), x)
+
+
+@gpu
+def test_lists_orders_and_empty_matrices():
+    from fc3d import ops
+    g = update((70, 40, 3, 3), "gauss", 7)
+    plain = ops.orthogonalize(g.cuda())
+    cl = ops.orthogonalize(g.cuda().contiguous(memory_format=torch.channels_last))
+    assert cl.is_contiguous(memory_format=torch.channels_last)
+    near(cl, g, "channels_last")
+    near(plain, g, "dense")
+    m = update((50, 90), "gauss", 8)
+    t = ops.orthogonalize(m.cuda().t())
+    near(t, m.t(), "transposed view")
+    wide = torch.zeros(50, 100, device="cuda")
+    wide[:, 5:95] = m.cuda()
+    near(ops.orthogonalize(wide[:, 5:95]), m, "columns of a wider matrix")
+    out = ops.orthogonalize([torch.zeros(0, 5, device="cuda"), m.cuda(), torch.zeros(5, 0, device="cuda", dtype=F16), m.bfloat16().cuda()])
+    assert out[0].shape == (0, 5) and out[2].shape == (5, 0) and out[2].dtype == F16
+    near(out[1], m, "among empty ones")
+    near(out[3], m.bfloat16(), "among other types")
+    # more than one group of launches takes
+    many = [update((3 + i % 7, 5 + i % 11), "gauss", 200 + i) for i in range(101)]
+    for x, v in zip(ops.orthogonalize([v.cuda() for v in many]), many):
+        near(x, v, "one of many")
+    with pytest.raises(ValueError, match="grow"):
+        ops.orthogonalize(m.cuda(), coefficients=(30.0, 0.0, 0.0))
+    with pytest.raises(TypeError):
+        ops.orthogonalize(m.double().cuda())
+    with pytest.raises(ValueError):
+        ops.orthogonalize(torch.zeros(5, device="cuda"))
+
+
+@gpu
+def test_writes_nothing_beyond_its_outputs_and_works_in_place():
+    import ctypes
+    from fc3d import _native
+    lib = _native.load()
+    I64, VP = ctypes.c_int64, ctypes.c_void_p
+    pad = 64
+    for dt, code in ((F32, 0), (BF16, 1)):
+        for shape in ((33, 70), (70, 33), (1, 129), (64, 64)):
+            g = update(shape, "gauss", 9, dt)
+            buf = torch.full((g.numel() + 2 * pad,), 512.0, dtype=dt, device="cuda")
+            buf[pad:-pad] = g.reshape(-1).cuda()
+            r, c = (I64 * 1)(shape[0]), (I64 * 1)(shape[1])
+            n = lib.fc3d_orthogonalize_workspace(1, r, c)
+            ws = torch.full((n + 512,), 77, dtype=torch.uint8, device="cuda")
+            at = (VP * 1)(buf.data_ptr() + pad * buf.element_size())
+            base = ws.data_ptr() + 256
+            assert base % 256 == 0
+            assert lib.fc3d_orthogonalize(torch.cuda.current_stream().cuda_stream, 1, at, at, r, c, code, 5, *COEFFS, 1e-7, base) == 0
+            torch.cuda.synchronize()
+            assert bool((buf[:pad] == 512.0).all()) and bool((buf[-pad:] == 512.0).all())
+            assert bool((ws[:256] == 77).all()) and bool((ws[256 + n:] == 77).all())
+            near(buf[pad:-pad].reshape(shape), g, f"in place {shape}")
+
+
+def step_formula(w, g, m, lr, beta, nesterov, wd, scale_f, dt=torch.float64):
+    w, g, m = w.to(dt), g.to(dt), m.to(dt)
+    m = beta * m + (1 - beta) * g
+    u = (1 - beta) * g + beta * m if nesterov else m
+    return (1 - lr * wd) * w - lr * scale_f * ns(u, dt), m, u
+
+
+@gpu
+@pytest.mark.parametrize("types", [(F32, F32), (BF16, BF16), (F16, F16), (F32, BF16), (BF16, F32)],
+                         ids=lambda t: "-".join(str(v).replace("torch.", "") for v in t))
+@pytest.mark.parametrize("nesterov,scale", [(True, "spectral"), (False, "rms")])
+def test_step_against_definition(types, nesterov, scale):
+    from fc3d import ops
+    pt, gt = types
+    shapes = [(40, 24, 3, 3), (24, 100), (100, 24), (65, 65), (1, 9), (128, 640)]
+    w = [(torch.randn(s, generator=torch.Generator().manual_seed(i)) / 8).to(pt) for i, s in enumerate(shapes)]
+    g = [update(s, "low", 30 + i, gt) for i, s in enumerate(shapes)]
+    m = [update(s, "gauss", 60 + i) for i, s in enumerate(shapes)]
+    wd, md = [t.cuda() for t in w], [t.cuda() for t in m]
+    lr, beta, decay = 0.02, 0.9, 0.1
+    ops.muon_step(wd, [t.cuda() for t in g], md, lr=lr, momentum=beta, nesterov=nesterov, weight_decay=decay, scale=scale)
+    for i, s in enumerate(shapes):
+        f = ops.muon_scale(s, scale)
+        ref_w, ref_m, u = step_formula(w[i], g[i], m[i], lr, beta, nesterov, decay, f)
+        # beta and 1 - beta rounded to fp32, a product and an fma: four half steps of the terms
+        off = (md[i].cpu().double() - ref_m).abs()
+        assert bool((off <= 4 * 2.0 ** -24 * (beta * m[i].double().abs() + (1 - beta) * g[i].double().abs()) + 2.0 ** -149).all()), s
+        o = ns(u, torch.float64)
+        # the update u comes with the same four half steps, which the steps amplify as they do fp32's own roundings
+        tol = lr * f * float(o.norm()) * (bound(u.float(), o, dt=pt) + 2.0 ** -20)
+        tol += (torch.finfo(pt).eps / 2 + 4 * 2.0 ** -24) * float(ref_w.norm() + (w[i].double() - ref_w).norm())
+        assert float((wd[i].cpu().double() - ref_w).norm()) <= tol, s
+
+
+@gpu
+def test_step_checks():
+    from fc3d import ops
+    w, g, m = (torch.zeros(4, 6, device="cuda") for _ in range(3))
+    v0 = w._version
+    ops.muon_step([w], [g], [m])
+    assert w._version > v0 and m._version > v0                        # seen by autograd's check of saved tensors
+    for bad, err in ((([w, w], [g, g], [m, m.clone()]), ValueError), (([w, w.clone()], [g, g], [m, m]), ValueError),
+                     (([w], [g], [m.half()]), TypeError), (([w], [g.t()], [m]), ValueError),
+                     (([w], [g.cpu()], [m]), RuntimeError), (([w[:, :3]], [g[:, :3]], [m[:, :3]]), ValueError),
+                     (([w.double()], [g], [m]), TypeError), (([w.t()], [g.t()], [m.t().contiguous()]), ValueError)):
+        with pytest.raises(err):
+            ops.muon_step(*bad)
+    with pytest.raises(ValueError, match="grow"):
+        ops.muon_step([w, w.half()], [g, g], [m, m.clone()], coefficients=(30.0, 0.0, 0.0))
+    ops.muon_step([torch.zeros(0, 4, device="cuda")], [torch.zeros(0, 4, device="cuda")], [torch.zeros(0, 4, device="cuda")])
+
+
+@gpu
+def test_step_of_weights_in_other_memory_orders():
+    from fc3d import ops
+    w, g, m = (update((24, 16, 3, 3), "gauss", 40 + i) for i in range(3))
+    ref = [t.cuda() for t in (w, g, m)]
+    ops.muon_step([ref[0]], [ref[1]], [ref[2]], weight_decay=0.1)
+    cl = [t.cuda().contiguous(memory_format=torch.channels_last) for t in (w, g, m)]
+    dense_g = g.cuda()                                                # the gradient in another order than its weight
+    ops.muon_step([cl[0]], [dense_g], [cl[2]], weight_decay=0.1)
+    assert float((cl[0] - ref[0]).abs().max()) <= 2.0 ** -18 * 0.02 and torch.equal(cl[2], ref[2])
+    a, b, c = (update((60, 24), "gauss", 50 + i).cuda() for i in range(3))
+    ta, tb, tc = a.clone(), b.clone(), c.clone()
+    ops.muon_step([a], [b], [c], scale="rms")
+    ops.muon_step([ta.t()], [tb.t()], [tc.t()], scale="rms")           # the factor is the same both ways round
+    assert torch.equal(a, ta) and torch.equal(c, tc)
+
+
+@gpu
+def test_optimizer():
+    from fc3d import ops, optim
+    torch.manual_seed(0)
+    make = lambda: [torch.nn.Parameter(update(s, "gauss", 70 + i, dt).cuda()) for i, (s, dt) in  # noqa: E731
+                    enumerate((((16, 8, 3, 3), F32), ((32, 20), BF16), ((5, 6), F32)))]
+    ps, qs = make(), make()
+    opt = optim.Muon([{"params": ps[:2], "lr": 0.1}, {"params": ps[2:], "nesterov": False}], lr=0.05, weight_decay=0.1)
+    mom = [torch.zeros_like(q, dtype=F32) for q in qs]
+    for turn in range(3):
+        gs = [update(tuple(p.shape), "gauss", 80 + 3 * turn + i, p.dtype).cuda() for i, p in enumerate(ps)]
+        for p, g in zip(ps, gs):
+            p.grad = g.clone()
+        if turn == 1:
+            ps[2].grad = None                                          # stays as it is
+        assert opt.step(lambda: 7.0) == 7.0
+        with torch.no_grad():
+            ops.muon_step(qs[:2], gs[:2], mom[:2], lr=0.1, weight_decay=0.1)
+            if turn != 1:
+                ops.muon_step(qs[2:], gs[2:], mom[2:], lr=0.05, nesterov=False, weight_decay=0.1)
+        for p, q in zip(ps, qs):
+            assert torch.equal(p, q)
+    # saved and loaded: the momenta come back bit for bit, those of 16-bit weights in 32 bits
+    again = optim.Muon([{"params": [torch.nn.Parameter(p.detach().clone()) for p in ps[:2]]},
+                        {"params": [torch.nn.Parameter(ps[2].detach().clone())]}])
+    again.load_state_dict(opt.state_dict())
+    for g, h in zip(again.param_groups, opt.param_groups):
+        assert g["lr"] == h["lr"] and g["nesterov"] == h["nesterov"]
+        for p, q in zip(g["params"], h["params"]):
+            a, b = again.state[p]["momentum_buffer"], opt.state[q]["momentum_buffer"]
+            assert a.dtype == F32 and torch.equal(a, b) and a.data_ptr() != b.data_ptr()
+            p.grad = torch.ones_like(p)
+            q.grad = torch.ones_like(q)
+    again.step()
+    opt.step()
+    for g, h in zip(again.param_groups, opt.param_groups):
+        for p, q in zip(g["params"], h["params"]):
+            assert torch.equal(p, q)
+
+
+@gpu
+def test_steps_in_graphs_and_on_streams():
+    """Two captured steps replayed on new gradients, with eager steps of others in between; two streams at once."""
+    from fc3d import ops
+
+    def capture(shapes, seed):
+        w = [update(s, "gauss", seed + i).cuda() for i, s in enumerate(shapes)]
+        g = [torch.zeros_like(t) for t in w]
+        m = [torch.zeros_like(t) for t in w]
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            ops.muon_step([t.clone() for t in w], g, [t.clone() for t in m])
+        torch.cuda.current_stream().wait_stream(side)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side, capture_error_mode="thread_local"):
+            ops.muon_step(w, g, m)
+        return graph, w, g, m
+    shapes = ([(40, 90), (64, 64)], [(30, 200), (9, 9), (70, 70)])
+    graphs = [capture(s, 300 + 10 * i) for i, s in enumerate(shapes)]
+    eager = [([t.clone() for t in w], [t.clone() for t in m]) for _, w, _, m in graphs]
+    for turn in range(4):
+        for (_, w, g, m), s in zip(graphs, shapes):
+            for i, t in enumerate(g):
+                t.copy_(update(s[i], "low", 400 + 10 * turn + i).cuda())
+        for graph, _, _, _ in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        for (_, w, g, m), (ew, em) in zip(graphs, eager):
+            ops.muon_step(ew, g, em)
+            torch.cuda.synchronize()
+            for a, b in zip(w + m, ew + em):
+                assert torch.equal(a, b)
+    gs = [update((200, 300), "gauss", 500 + i).cuda() for i in range(2)]
+    alone = [ops.orthogonalize(g) for g in gs]
+    streams = [torch.cuda.Stream() for _ in gs]
+    got = []
+    torch.cuda.synchronize()
+    for _ in range(3):
+        for g, s in zip(gs, streams):
+            with torch.cuda.stream(s):
+                got.append(ops.orthogonalize(g))
+    torch.cuda.synchronize()
+    for i, x in enumerate(got):
+        assert torch.equal(x, alone[i % 2])
