@@ -18,7 +18,9 @@
 // directions whose share of A is below its rounding, amplified a^(2L)-fold: five steps at once cost 1e-4 of the
 // result in bad cases (measured in emulation, low rank plus noise), which is below the rounding of a 16-bit result;
 // for fp32 results the segments are of two and three steps, or of one for matrices that are nearly square
-// (n < 2 m, where the smallest singular values sit near zero), as accurate as step by step.
+// (n < 2 m, where the smallest singular values sit near zero) and for those of one tile (where the squares saved are
+// cheap), as accurate as step by step.  Against 64 bits: 512 x 4608 1.2e-6 of the result (fp32 matrix products
+// 4.2e-6), 256 x 256 6e-7 (1.8e-6), 64 x 288 1.4e-6 (1.4e-6).
 #include "fc3d_common.h"
 
 #include <cmath>
@@ -29,62 +31,91 @@ namespace {
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef float float16v __attribute__((ext_vector_type(16)));
 
-constexpr int kTile = 64;             // products: output tile, and depth of one staged slice
-constexpr int kMaxItems = 48;         // matrices of one launch (their descriptions travel as kernel arguments)
-constexpr int kMaxJobs = 2 * kMaxItems;
+constexpr int kSlice = 64;            // depth of one staged slice of a product, and the unit that sizes are padded to
+constexpr int kMaxItems = 48;         // matrices of one group (their descriptions travel as kernel arguments once)
 constexpr int kChunk = 16384;         // elements of one workgroup of the norm pass
 
 // A matrix's buffers, each a plane of hi values and one of lo values: X in two orders (the transpose twice: a segment
 // reads one and writes the other), then the m x m matrices of the Gram form.
 enum Buffer : uint8_t { BUF_X, BUF_XT0, BUF_XT1, BUF_A, BUF_Q, BUF_R, BUF_P0, BUF_P1, BUF_COUNT };
 
-struct Job {                          // one product (or one matrix) of a launch
-    int64_t base;                     // halves from the start of the workspace's planes to the matrix's buffers
-    int m, n;                         // m <= n
-    int first;                        // the launch's first workgroup that works on it
-    uint8_t src1, src2, dst, op;      // buffers, and which of the launch's scales is the result's
-    int slot;                         // the matrix's number in the call
-};
-template <int N>
-struct Jobs {
-    int count;
-    Job e[N];
-};
-struct Io {                           // a matrix's tensors
-    const void* g;
-    float* mom;
-    void* out;
-    float lr;                         // learning rate times the shape's factor
-    int tall;                         // the tensor is n x m
-    int part0;                        // its first partial sum of squares
-};
-struct Ios {
-    Io e[kMaxItems];
-};
-
-__host__ __device__ inline int padded(int v) { return (v + kTile - 1) / kTile * kTile; }
-
-// The entry whose workgroups hold `block`
-template <int N>
-__device__ __forceinline__ int find_job(const Jobs<N>& t, int block) {
-    int lo = 0, hi = t.count - 1;
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (t.e[mid].first <= block) lo = mid;
-        else hi = mid - 1;
-    }
-    return lo;
+__host__ __device__ inline int64_t plane_of(int id, int64_t mp, int64_t np) {     // values of one plane of a buffer
+    return id < BUF_A ? mp * np : mp * mp;
 }
+__host__ __device__ inline int64_t before(int id, int64_t mp, int64_t np) {       // values in front of it
+    return id < BUF_A ? 2 * id * mp * np : 2 * BUF_A * mp * np + 2 * (id - BUF_A) * mp * mp;
+}
+
+struct Matrix {
+    const void* g;
+    float* mom;                       // NULL: g itself is orthogonalised
+    void* out;
+    int64_t base;                     // halves from the start of the workspace's planes to its buffers
+    int m, n, mp, np;                 // m <= n, and both padded
+    float lr;                         // learning rate times the shape's factor
+    int part0;                        // its first partial sum of squares
+    int split, sums0;                 // workgroups that share the depth of a Gram tile, its first tile of their sums
+    int tall, plan;                   // the tensor is n x m; which sequence of products it goes through
+
+    __device__ __forceinline__ void from_lane(int w) {        // this lane's entry becomes lane w's, in all lanes
+        static_assert(sizeof(Matrix) % 4 == 0, "copied as words");
+        int words[sizeof(Matrix) / 4];
+        __builtin_memcpy(words, this, sizeof(Matrix));
+#pragma unroll
+        for (unsigned i = 0; i < sizeof(Matrix) / 4; ++i) words[i] = __builtin_amdgcn_readlane(words[i], w);
+        __builtin_memcpy(this, words, sizeof(Matrix));
+    }
+};
+struct Table {
+    int count;
+    Matrix e[kMaxItems];
+};
 
 __device__ __forceinline__ float ld_any(const void* p, int type, size_t i) {
     if (type == FC3D_F32) return static_cast<const float*>(p)[i];
     if (type == FC3D_BF16) return (float)static_cast<const __bf16*>(p)[i];
     return (float)static_cast<const _Float16*>(p)[i];
 }
+// four values, at the element's own alignment
+typedef float float4a __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint32_t word2a __attribute__((ext_vector_type(2), aligned(2)));
+__device__ __forceinline__ void ld4_any(const void* p, int type, size_t i, float (&v)[4]) {
+    if (type == FC3D_F32) {
+        const float4a w = *reinterpret_cast<const float4a*>(static_cast<const float*>(p) + i);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = w[j];
+        return;
+    }
+    const word2a w = *reinterpret_cast<const word2a*>(static_cast<const uint16_t*>(p) + i);
+    if (type == FC3D_BF16) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = __uint_as_float(j & 1 ? w[j >> 1] & 0xffff0000u : w[j >> 1] << 16);
+    } else {
+        _Float16 h[4];
+        __builtin_memcpy(h, &w, 8);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = (float)h[j];
+    }
+}
 __device__ __forceinline__ void st_any(void* p, int type, size_t i, float v) {
     if (type == FC3D_F32) static_cast<float*>(p)[i] = v;
     else if (type == FC3D_BF16) static_cast<__bf16*>(p)[i] = (__bf16)v;
     else static_cast<_Float16*>(p)[i] = (_Float16)v;
+}
+
+// Which matrix this workgroup works on: lane l counts the workgroups of matrix l, a scan over the wavefront numbers
+// them.  Returns the matrix, and the workgroup's number within it in `block` (the same in all lanes).
+__device__ __forceinline__ int find_matrix(int mine, int& block) {
+    int sum = mine;
+    sum += __builtin_amdgcn_update_dpp(0, sum, 0x111, 0xf, 0xf, true);       // the lane 1, 2, 4, 8 below, in rows of 16
+    sum += __builtin_amdgcn_update_dpp(0, sum, 0x112, 0xf, 0xf, true);
+    sum += __builtin_amdgcn_update_dpp(0, sum, 0x114, 0xf, 0xf, true);
+    sum += __builtin_amdgcn_update_dpp(0, sum, 0x118, 0xf, 0xf, true);
+    sum += __builtin_amdgcn_update_dpp(0, sum, 0x142, 0xa, 0xf, false);      // the last lane of the row, of the half below
+    sum += __builtin_amdgcn_update_dpp(0, sum, 0x143, 0xc, 0xf, false);
+    const int w = __builtin_ctzll(ballot64(sum > block) | (1ull << 63));
+    block -= __builtin_amdgcn_readlane(sum - mine, w);
+    return w;
 }
 
 struct Blend {                        // m' = beta m + (1 - beta) g;  u = (1 - beta) g + beta m' (nesterov) or m'
@@ -95,55 +126,93 @@ __device__ __forceinline__ float blend(const Blend& k, float g, float mom_new) {
     return k.nesterov ? fmaf(k.beta, mom_new, k.rest * g) : mom_new;
 }
 
+__device__ __forceinline__ int parts_of(const Matrix& e) { return (int)(((size_t)e.m * e.n + kChunk - 1) / kChunk); }
+
 // Sums of squares of the update per workgroup (64 bits: any fp32 input stays in range), and the momentum's update.
-__global__ __launch_bounds__(256) void ns_norm_kernel(Jobs<kMaxItems> t, Ios io, int type, Blend k, double* __restrict__ parts) {
+// The first workgroup leaves the table in device memory for the launches that follow: kernel arguments may lie in host
+// memory, where a search through them costs microseconds.
+__global__ __launch_bounds__(256) void ns_norm_kernel(Table t, int type, Blend k, double* __restrict__ parts,
+                                                      Matrix* __restrict__ table) {
     __shared__ double red[4];
-    const int i = find_job(t, blockIdx.x);
-    const Io& o = io.e[i];
-    const size_t count = (size_t)t.e[i].m * t.e[i].n;
-    const size_t lo = (size_t)((int)blockIdx.x - t.e[i].first) * kChunk;
+    const int lane = threadIdx.x & 63;
+    if (blockIdx.x == 0) {
+        const int words = t.count * (int)(sizeof(Matrix) / 4);
+        const uint32_t* from = reinterpret_cast<const uint32_t*>(&t.e[0]);
+        for (int q = threadIdx.x; q < words; q += 256) reinterpret_cast<uint32_t*>(table)[q] = from[q];
+    }
+    int block = blockIdx.x;
+    const int w = find_matrix(lane < t.count ? parts_of(t.e[lane < t.count ? lane : 0]) : 0, block);
+    const Matrix& e = t.e[w];
+    const size_t count = (size_t)e.m * e.n;
+    const size_t lo = (size_t)block * kChunk;
     const size_t hi = lo + kChunk < count ? lo + kChunk : count;
     double s = 0.0;
-    for (size_t j = lo + threadIdx.x; j < hi; j += 256) {
-        float u = ld_any(o.g, type, j);
-        if (o.mom) {
-            const float mn = fmaf(k.beta, o.mom[j], k.rest * u);
-            o.mom[j] = mn;
+    const auto one = [&](size_t j) {
+        float u = ld_any(e.g, type, j);
+        if (e.mom) {
+            const float mn = fmaf(k.beta, e.mom[j], k.rest * u);
+            e.mom[j] = mn;
             u = blend(k, u, mn);
         }
         s = fma((double)u, (double)u, s);
+    };
+    const size_t whole = lo + (hi - lo) / 4 * 4;
+#pragma unroll 4
+    for (size_t j = lo + 4 * threadIdx.x; j < whole; j += 1024) {
+        float u[4];
+        ld4_any(e.g, type, j, u);
+        if (e.mom) {
+            float m[4];
+            ld4_any(e.mom, FC3D_F32, j, m);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                m[q] = fmaf(k.beta, m[q], k.rest * u[q]);
+                u[q] = blend(k, u[q], m[q]);
+            }
+            float4a v;
+            __builtin_memcpy(&v, m, 16);
+            *reinterpret_cast<float4a*>(e.mom + j) = v;
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q) s = fma((double)u[q], (double)u[q], s);
     }
+    if (whole + threadIdx.x < hi) one(whole + threadIdx.x);
 #pragma unroll
     for (int q = 32; q > 0; q >>= 1) s += __shfl_xor(s, q, 64);
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+    if (lane == 0) red[threadIdx.x >> 6] = s;
     __syncthreads();
-    if (threadIdx.x == 0) parts[o.part0 + (int)blockIdx.x - t.e[i].first] = (red[0] + red[1]) + (red[2] + red[3]);
+    if (threadIdx.x == 0) parts[e.part0 + block] = (red[0] + red[1]) + (red[2] + red[3]);
 }
 
-__device__ __forceinline__ void split_store(_Float16* p, size_t plane, size_t at, float v) {
-    const _Float16 h = (_Float16)v;
-    p[at] = h;
-    p[plane + at] = (_Float16)(v - (float)h);
+__device__ __forceinline__ void split8(_Float16* p, size_t plane, const float (&v)[8]) {
+    half8 h, l;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        h[j] = (_Float16)v[j];
+        l[j] = (_Float16)(v[j] - (float)h[j]);
+    }
+    *reinterpret_cast<half8*>(p) = h;
+    *reinterpret_cast<half8*>(p + plane) = l;
 }
 
 // X and its transpose, scaled by sx / (norm + eps), zero beyond the matrix, one 64 x 64 tile per workgroup.
 // `exact` (16-bit input taken as it is): one plane that holds the input times a power of two, without rounding; the
 // remaining factor in [1, 2) goes to rho and into the products that read X.
-__global__ __launch_bounds__(256) void ns_prepare_kernel(Jobs<kMaxItems> t, Ios io, int type, Blend k, const double* __restrict__ parts,
-                                                         double eps, float sx, int exact, _Float16* __restrict__ planes,
-                                                         float* __restrict__ rho) {
-    __shared__ float tile[kTile][kTile + 1];
+__global__ __launch_bounds__(256) void ns_prepare_kernel(const Matrix* __restrict__ t, int matrices, int type, Blend k,
+                                                         const double* __restrict__ parts, double eps, float sx, int exact,
+                                                         _Float16* __restrict__ planes, float* __restrict__ rho) {
+    __shared__ float tile[64][65];
     __shared__ double red[4];
-    const int i = find_job(t, blockIdx.x);
-    const Job& e = t.e[i];
-    const Io& o = io.e[i];
-    const int mp = padded(e.m), np = padded(e.n);
-    const int count = (int)(((size_t)e.m * e.n + kChunk - 1) / kChunk);
+    const int lane = threadIdx.x & 63;
+    int block = blockIdx.x;
+    const int w = find_matrix(lane < matrices ? (t[lane].mp / 64) * (t[lane].np / 64) : 0, block);
+    const Matrix& e = t[w];
+    const int count = parts_of(e);
     double s = 0.0;
-    for (int q = threadIdx.x; q < count; q += 256) s += parts[o.part0 + q];
+    for (int q = threadIdx.x; q < count; q += 256) s += parts[e.part0 + q];
 #pragma unroll
     for (int q = 32; q > 0; q >>= 1) s += __shfl_xor(s, q, 64);
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+    if (lane == 0) red[threadIdx.x >> 6] = s;
     __syncthreads();
     const double factor = (double)sx / (sqrt((red[0] + red[1]) + (red[2] + red[3])) + eps);
     int shift = 0;
@@ -151,173 +220,441 @@ __global__ __launch_bounds__(256) void ns_prepare_kernel(Jobs<kMaxItems> t, Ios 
     if (exact) {
         rest = 2.0f * (float)frexp(factor, &shift);          // factor = rest * 2^(shift - 1), rest in [1, 2)
         shift -= 1;
-        if (!(factor < 1e300)) shift = 0;                    // a zero matrix with eps 0, or a NaN: 0 * inf below
-        if (!(factor < 1e300) || factor == 0.0) rest = (float)factor;
+        if (!(factor < 1e300) || factor == 0.0) {            // a zero matrix with eps 0, an infinity or a NaN: 0 * inf below
+            shift = 0;
+            rest = (float)factor;
+        }
     }
-    const int block = (int)blockIdx.x - e.first, tn = np / kTile;
-    const int i0 = block / tn * kTile, j0 = block % tn * kTile;
-    if (block == 0 && threadIdx.x == 0) rho[e.slot] = rest;
-    const int tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
+    const int tn = e.np / 64;
+    const int i0 = block / tn * 64, j0 = block % tn * 64;
+    if (block == 0 && threadIdx.x == 0) rho[w] = rest;
+    const int ty = threadIdx.x >> 6;
 #pragma unroll
     for (int q = 0; q < 16; ++q) {
-        const int fast = tx, slow = q * 4 + ty;              // fast: along the tensor's rows
-        const int r = o.tall ? fast : slow, c = o.tall ? slow : fast;
+        const int fast = lane, slow = q * 4 + ty;            // fast: along the tensor's rows
+        const int r = e.tall ? fast : slow, c = e.tall ? slow : fast;
         float v = 0.0f;
         if (i0 + r < e.m && j0 + c < e.n) {
-            const size_t at = o.tall ? (size_t)(j0 + c) * e.m + (i0 + r) : (size_t)(i0 + r) * e.n + (j0 + c);
-            v = ld_any(o.g, type, at);
-            if (o.mom) v = blend(k, v, o.mom[at]);
+            const size_t at = e.tall ? (size_t)(j0 + c) * e.m + (i0 + r) : (size_t)(i0 + r) * e.n + (j0 + c);
+            v = ld_any(e.g, type, at);
+            if (e.mom) v = blend(k, v, e.mom[at]);
             v = exact ? ldexpf(v, shift) : (float)((double)v * factor);
         }
         tile[r][c] = v;
     }
     __syncthreads();
-    const size_t plane = (size_t)mp * np;
+    const size_t plane = plane_of(BUF_X, e.mp, e.np);
     _Float16* x = planes + e.base;
-    _Float16* xt = x + 2 * plane;
+    _Float16* xt = x + before(BUF_XT0, e.mp, e.np);
 #pragma unroll
-    for (int q = 0; q < 16; ++q) {
-        const int r = q * 4 + ty;
-        split_store(x, plane, (size_t)(i0 + r) * np + j0 + tx, tile[r][tx]);
-        split_store(xt, plane, (size_t)(j0 + r) * mp + i0 + tx, tile[tx][r]);
+    for (int q = 0; q < 2; ++q) {
+        const int id = threadIdx.x + 256 * q, r = id >> 3, c = (id & 7) * 8;
+        float v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = tile[r][c + j];
+        split8(x + (size_t)(i0 + r) * e.np + j0 + c, plane, v);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = tile[c + j][r];
+        split8(xt + (size_t)(j0 + r) * e.mp + i0 + c, plane, v);
     }
 }
 
 // ---- products -----------------------------------------------------------------------------------------------
 // D[i][j] = sum_k S1[i][k] S2[j][k]: both operands run along the depth in memory (a symmetric matrix is its own
-// transpose, and X is kept in both orders), so one kernel serves every product.
-enum Kind { GRAM, POLY, MUL, APPLY };
-
-struct Product {
-    _Float16* planes;
-    const float* rho;
-    float alpha[2];                   // sum -> stored value (scales of the operands and of the result), by Job::op
-    float a, b;                       // POLY: Q = a I + b A + c A^2, in units of the stored result
-    int use_rho;                      // the first segment of an input taken as it is
-    // APPLY
-    int last;                         // to the tensors, else back to X and its transpose
+// transpose, and X is kept in both orders), so one kernel serves every product:
+//   GRAM   A = X X^T           POLY  Q = a I + b A + c A A        MUL  R = A Q, A = R Q, P = P Q  (symmetric: the upper
+//   APPLY  X = P X                                                     triangle's tiles, mirrored)
+// A launch does the next product of every matrix, whatever its kind: matrices of different shapes go through
+// different sequences (plans) side by side.
+enum Kind : uint8_t { NONE, GRAM, POLY, MUL, APPLY };
+struct Op {
+    uint8_t kind, src1, src2, dst;
+    float alpha;                      // sum -> stored value (scales of the operands and of the result)
+    uint8_t use_rho, last;            // the first segment of an input taken as it is; APPLY: to the tensors
+};
+constexpr int kPlans = 2;
+struct Launch {
+    Op op[kPlans][2];                 // up to two products of a matrix that do not need each other
+    float a, b;                       // POLY: Q = a I + b A + c A A, in units of the stored result
     int out_type, step;               // step: weights := decay * weights - lr * result
     float decay;
+    int matrices;
+    const Matrix* table;
+    _Float16* planes;
+    const float* rho;
+    float* sums;                      // Gram tiles of shared depth: [tile][share][TILE * TILE]
 };
 
-__device__ __forceinline__ _Float16* buffer(const Job& e, _Float16* planes, int id, int& ld, size_t& plane) {
-    const int mp = padded(e.m), np = padded(e.n);
-    const size_t xn = (size_t)mp * np, an = (size_t)mp * mp;
-    if (id < BUF_A) {
-        ld = id == BUF_X ? np : mp;
-        plane = xn;
-        return planes + e.base + (size_t)id * 2 * xn;
-    }
-    ld = mp;
-    plane = an;
-    return planes + e.base + 6 * xn + (size_t)(id - BUF_A) * 2 * an;
+__device__ __forceinline__ _Float16* buffer(const Matrix& e, _Float16* planes, int id, int& ld, size_t& plane) {
+    ld = id == BUF_X ? e.np : e.mp;
+    plane = (size_t)plane_of(id, e.mp, e.np);
+    return planes + e.base + before(id, e.mp, e.np);
 }
 
-struct NoIos {};
-// P1, P2: planes of the operands that count (1: the lo plane is zero)
-template <int KIND, int P1, int P2, int N, typename IO>
-__global__ __launch_bounds__(256) void ns_product_kernel(Jobs<N> t, IO io, Product a) {
-    __shared__ half8 lds[(P1 + P2) * kTile * kTile / 8];
-    const int w = find_job(t, blockIdx.x);
-    const Job& e = t.e[w];
-    const int block = (int)blockIdx.x - e.first;
+__host__ __device__ inline int tiles_of(int kind, int mp, int np, int split, int tile) {
+    const int tm = (mp + tile - 1) / tile, tn = (np + tile - 1) / tile;
+    return kind == NONE ? 0 : kind == APPLY ? tm * tn : tm * (tm + 1) / 2 * (kind == GRAM ? split : 1);
+}
+
+// Workgroups next to each other, which run at the same time behind one L2, take tiles in strips of kStrip: 4 x 8 tiles
+// read 12 different operand slices where a row of 32 reads 33.
+constexpr int kStrip = 8;
+
+__device__ __forceinline__ int column_of(int block) {         // the column of a triangle numbered column by column
+    int tj = (int)((sqrtf(8.0f * (float)block + 1.0f) - 1.0f) * 0.5f);
+    while ((long)tj * (tj + 1) / 2 > block) --tj;
+    while ((long)(tj + 1) * (tj + 2) / 2 <= block) ++tj;
+    return tj;
+}
+// The upper triangle of t x t tiles: strips of kStrip columns, each by rows, its own triangle last
+__device__ __forceinline__ void upper_tile(int block, int t, int& ti, int& tj) {
+    const int left = column_of(block) / kStrip * kStrip, wide = t - left < kStrip ? t - left : kStrip;
+    int l = block - (int)((long)left * (left + 1) / 2);
+    if (l < left * wide) {
+        ti = l / wide;
+        tj = left + l % wide;
+    } else {
+        l -= left * wide;
+        const int c = column_of(l);
+        ti = left + l - c * (c + 1) / 2;
+        tj = left + c;
+    }
+}
+
+// A workgroup computes a TILE x TILE tile.  A wavefront holds BLK x BLK of the 32 x 32 matrix instruction's sums, so that
+// an operand read from LDS feeds 3 BLK of them: TILE 64 and 96: every wavefront the whole tile, its part of the depth;
+// TILE 128: two wavefronts per quadrant.  Their sums meet at the end.  Stages are fetched ahead into registers (what
+// another compute unit has just written comes from behind the L2: most of a microsecond) and go through two LDS
+// buffers, one barrier per stage.  P1, P2: planes of the operands that count (1: the lo plane is zero).
+template <int TILE, int WAVES, int P1, int P2>
+__global__ __launch_bounds__(WAVES * 64, TILE == 64 && WAVES == 4 ? 2 : 1) void ns_product_kernel(Launch a) {
+    constexpr bool QUADS = TILE == 128;
+    constexpr int THREADS = WAVES * 64, BLK = QUADS ? 2 : TILE / 32;
+    constexpr int NP = P1 + P2;
+    constexpr int DEPTH = kSlice, ROW = DEPTH / 8;           // of a stage, in values and in 16-byte pieces
+    constexpr int AHEAD = QUADS ? 1 : 2;                     // stages in flight in registers
+    static_assert(QUADS || WAVES * 16 == DEPTH, "every wavefront has 16 values of a stage's depth");
+    constexpr int PIECES = TILE * ROW / THREADS;             // pieces of a stage per lane and plane
+    constexpr int ROWS = THREADS / ROW;                      // rows that the workgroup's lanes cover at once
+    constexpr int SHARES = QUADS ? 2 : WAVES, LD = TILE + 1;
+    constexpr int STAGE = NP * TILE * ROW;                   // pieces of one stage
+    constexpr int SUMS = SHARES * TILE * LD;                 // floats of the workgroup's result
+    constexpr int BYTES = 2 * STAGE * 16 > SUMS * 4 ? 2 * STAGE * 16 : SUMS * 4;
+    __shared__ __attribute__((aligned(16))) char shared[BYTES];
+    half8* lds = reinterpret_cast<half8*>(shared);
+    float* out = reinterpret_cast<float*>(shared);
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    int block = (int)block_x();
+    // every lane reads one matrix of the table: what the workgroup needs of its own comes from that lane's registers
+    Matrix e = a.table[lane < a.matrices ? lane : 0];
+    const Op o00 = a.op[0][0], o01 = a.op[0][1], o10 = a.op[1][0], o11 = a.op[1][1];
+    const int k0 = e.plan ? o10.kind : o00.kind, k1 = e.plan ? o11.kind : o01.kind;
+    int n0 = tiles_of(k0, e.mp, e.np, e.split, TILE);
+    const int w = find_matrix(lane < a.matrices ? n0 + tiles_of(k1, e.mp, e.np, e.split, TILE) : 0, block);
+    e.from_lane(w);
+    n0 = __builtin_amdgcn_readlane(n0, w);
+    Op o = e.plan ? o10 : o00;
+    if (block >= n0) {
+        block -= n0;
+        o = e.plan ? o11 : o01;
+    }
+    int share = 0;
+    if (o.kind == GRAM && e.split > 1) {
+        const int tiles = tiles_of(MUL, e.mp, 0, 1, TILE);
+        share = block / tiles;
+        block -= share * tiles;
+    }
     int ti, tj;
-    if constexpr (KIND == APPLY) {
-        const int tn = padded(e.n) / kTile;
-        ti = block / tn;
-        tj = block % tn;
-    } else {                                                  // the upper triangle, column by column
-        tj = (int)((sqrtf(8.0f * (float)block + 1.0f) - 1.0f) * 0.5f);
-        while ((long)tj * (tj + 1) / 2 > block) --tj;
-        while ((long)(tj + 1) * (tj + 2) / 2 <= block) ++tj;
-        ti = block - (int)((long)tj * (tj + 1) / 2);
+    if (o.kind == APPLY) {
+        const int tm = (e.mp + TILE - 1) / TILE, tn = (e.np + TILE - 1) / TILE, strip = block / (kStrip * tn);
+        const int wide = tm - strip * kStrip < kStrip ? tm - strip * kStrip : kStrip;
+        const int l = block - strip * kStrip * tn;
+        ti = strip * kStrip + l % wide;
+        tj = l / wide;
+    } else {
+        upper_tile(block, (e.mp + TILE - 1) / TILE, ti, tj);
     }
     int ld1, ld2;
     size_t pl1, pl2;
-    const _Float16* s1 = buffer(e, a.planes, e.src1, ld1, pl1) + (size_t)ti * kTile * ld1;
-    const _Float16* s2 = buffer(e, a.planes, e.src2, ld2, pl2) + (size_t)tj * kTile * ld2;
-    const int depth = KIND == GRAM ? padded(e.n) : padded(e.m);
+    const _Float16* s1 = buffer(e, a.planes, o.src1, ld1, pl1) + (size_t)ti * TILE * ld1;
+    const _Float16* s2 = buffer(e, a.planes, o.src2, ld2, pl2) + (size_t)tj * TILE * ld2;
+    const int rows1 = e.mp - ti * TILE, rows2 = (o.kind == APPLY ? e.np : e.mp) - tj * TILE;       // from this tile on
+    int slices = (o.kind == GRAM ? e.np : e.mp) / kSlice;
+    if (o.kind == GRAM && e.split > 1) {
+        const int each = (slices + e.split - 1) / e.split, from = share * each;
+        slices = from + each < slices ? each : slices - from;
+        s1 += (size_t)from * kSlice;
+        s2 += (size_t)from * kSlice;
+    }
 
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int wi = (wave >> 1) * 32, wj = (wave & 1) * 32;
-    // 16-byte pieces of a row of 64 values are stored at piece ^ (row & 7): eight rows read at one depth then lie in
-    // different banks
-    half8 next[(P1 + P2) * 2];
-    const auto fetch = [&](int k0) {
+    // A row's pieces are stored in an order of its own (piece ^ key), so that 16 rows read at one depth, 256 bytes, lie in
+    // different banks (a row is 128 bytes long).
+    const auto key = [](int row) { return (row >> 1) & 7; };
+    const int row0 = tid / ROW, piece0 = tid % ROW;
+    const int stages = slices;
+    unsigned at1[PIECES], at2[PIECES];                        // bytes from the tile's first row; rows behind the matrix: its last
 #pragma unroll
-        for (int p = 0; p < P1 + P2; ++p)
+    for (int q = 0; q < PIECES; ++q) {
+        const int row = row0 + ROWS * q;
+        at1[q] = ((unsigned)(row < rows1 ? row : rows1 - 1) * (unsigned)ld1 + piece0 * 8) * 2u;
+        at2[q] = ((unsigned)(row < rows2 ? row : rows2 - 1) * (unsigned)ld2 + piece0 * 8) * 2u;
+    }
+    half8 next[AHEAD][NP * PIECES];
+    const auto fetch = [&](int s, half8 (&to)[NP * PIECES]) {
 #pragma unroll
-            for (int q = 0; q < 2; ++q) {
-                const int id = tid + 256 * q, row = id >> 3, piece = id & 7;
-                const _Float16* src = p < P1 ? s1 + p * pl1 + (size_t)row * ld1 : s2 + (p - P1) * pl2 + (size_t)row * ld2;
-                next[p * 2 + q] = *reinterpret_cast<const half8*>(src + k0 + piece * 8);
+        for (int p = 0; p < NP; ++p) {
+            const char* src = reinterpret_cast<const char*>((p < P1 ? s1 + p * pl1 : s2 + (p - P1) * pl2) + (size_t)s * DEPTH);
+#pragma unroll
+            for (int q = 0; q < PIECES; ++q)
+                to[p * PIECES + q] = *reinterpret_cast<const half8*>(src + (p < P1 ? at1[q] : at2[q]));
+        }
+    };
+    const auto stage = [&](int s, const half8 (&from)[NP * PIECES]) {
+#pragma unroll
+        for (int p = 0; p < NP; ++p)
+#pragma unroll
+            for (int q = 0; q < PIECES; ++q) {
+                const int row = row0 + ROWS * q;
+                lds[(s & 1) * STAGE + (p * TILE + row) * ROW + (piece0 ^ key(row))] = from[p * PIECES + q];
             }
     };
-    const auto stage = [&]() {
-#pragma unroll
-        for (int p = 0; p < P1 + P2; ++p)
-#pragma unroll
-            for (int q = 0; q < 2; ++q) {
-                const int id = tid + 256 * q, row = id >> 3, piece = id & 7;
-                lds[p * 512 + row * 8 + (piece ^ (row & 7))] = next[p * 2 + q];
-            }
+    const int quad = wave >> 1;
+    const int bi = QUADS ? (quad >> 1) * 64 : 0, bj = QUADS ? (quad & 1) * 64 : 0;
+    const int own = QUADS ? (wave & 1) * 2 : wave;            // this wavefront's first 16 values of a stage's depth, in 16s
+    // The matrix units' sums lose up to a unit of the running sum's last place per instruction: that the wavefronts
+    // share the depth keeps the chains short (a depth of 4608: 108 instructions; one wavefront's 864 would double
+    // the error of the result).
+    float16v acc[BLK][BLK] = {};
+    struct Part {                                             // both operands at 16 values of the depth
+        half8 f1[BLK][P1], f2[BLK][P2];
     };
-    float16v acc = {};
-    fetch(0);
-    for (int k0 = 0; k0 < depth; k0 += kTile) {
+    const auto load = [&](int s, int kk, Part& f) {
+        const int piece = kk * 2 + (lane >> 5);
+#pragma unroll
+        for (int h = 0; h < BLK; ++h) {
+            const int r1 = bi + h * 32 + (lane & 31), r2 = bj + h * 32 + (lane & 31);
+#pragma unroll
+            for (int p = 0; p < P1; ++p) f.f1[h][p] = lds[(s & 1) * STAGE + (p * TILE + r1) * ROW + (piece ^ key(r1))];
+#pragma unroll
+            for (int p = 0; p < P2; ++p) f.f2[h][p] = lds[(s & 1) * STAGE + ((P1 + p) * TILE + r2) * ROW + (piece ^ key(r2))];
+        }
+    };
+    const auto multiply = [&](const Part& f) {
+#pragma unroll
+        for (int pass = 0; pass < 3; ++pass) {                // lo hi, hi lo, hi hi
+            const int p1 = pass == 0 ? 1 : 0, p2 = pass == 1 ? 1 : 0;
+            if (p1 >= P1 || p2 >= P2) continue;
+#pragma unroll
+            for (int q = 0; q < BLK * BLK; ++q)
+                acc[q / BLK][q % BLK] =
+                    __builtin_amdgcn_mfma_f32_32x32x16_f16(f.f1[q / BLK][p1], f.f2[q % BLK][p2], acc[q / BLK][q % BLK], 0, 0, 0);
+        }
+    };
+    // Stage s: behind the barrier that makes it visible, its operands are read while the matrix units still work on what
+    // was read before; stage s + 1 goes from registers to the other LDS buffer, s + 1 + AHEAD into the registers.
+    // `whole`: no branch around the loads, so that the compiler knows how many are in flight and waits for the oldest
+    // alone.
+    const auto step = [&](int s, half8 (&regs)[NP * PIECES], Part& x, Part& y, bool first, bool whole) {
         __syncthreads();
-        stage();
-        __syncthreads();
-        if (k0 + kTile < depth) fetch(k0 + kTile);
+        load(s, own, x);
+        if (!first) multiply(y);
+        if constexpr (QUADS) load(s, own + 1, y);
+        if (whole || s + 1 < stages) stage(s + 1, regs);
+        if (whole || s + 1 + AHEAD < stages) fetch(s + 1 + AHEAD, regs);
+        if constexpr (QUADS) multiply(x);
+        // LDS and memory instructions one by one between the matrix instructions: issued in a row they would fill the LDS
+        // queue, and the matrix units would wait for it
+        if (whole && P1 == 2 && P2 == 2) {
+            constexpr int READS = 4 * BLK, MOVES = NP * PIECES, EACH = QUADS || BLK == 3 ? 1 : 2;
 #pragma unroll
-        for (int kk = 0; kk < 4; ++kk) {
-            const int r1 = wi + (lane & 31), r2 = wj + (lane & 31), piece = kk * 2 + (lane >> 5);
-            half8 f1[P1], f2[P2];
+            for (int half = 0; half < (QUADS ? 2 : 1); ++half) {
 #pragma unroll
-            for (int p = 0; p < P1; ++p) f1[p] = lds[p * 512 + r1 * 8 + (piece ^ (r1 & 7))];
+                for (int q = 0; q < READS; ++q) {
+                    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);        // LDS read
+                    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);        // matrix
+                }
 #pragma unroll
-            for (int p = 0; p < P2; ++p) f2[p] = lds[(P1 + p) * 512 + r2 * 8 + (piece ^ (r2 & 7))];
-            if constexpr (P2 > 1) acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(f1[0], f2[1], acc, 0, 0, 0);
-            if constexpr (P1 > 1) acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(f1[1], f2[0], acc, 0, 0, 0);
-            acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(f1[0], f2[0], acc, 0, 0, 0);
+                for (int q = 0; q < MOVES / EACH / (QUADS ? 2 : 1); ++q) {
+                    __builtin_amdgcn_sched_group_barrier(0x200, EACH, 0);     // LDS write
+                    __builtin_amdgcn_sched_group_barrier(0x020, EACH, 0);     // load
+                    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                }
+            }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    Part fa, fb;                                              // even and odd stages; quadrants: the two halves of one
+    Part& odd = QUADS ? fa : fb;
+    Part& other = QUADS ? fb : fa;
+    fetch(0, next[0]);
+    if constexpr (AHEAD == 2) fetch(stages > 1 ? 1 : 0, next[1]);
+    stage(0, next[0]);
+    if (stages > AHEAD) fetch(AHEAD, next[0]);
+    half8 (&second)[NP * PIECES] = next[AHEAD - 1];
+    step(0, second, fa, fb, true, false);
+    int s = 1;
+    for (; s + 2 + AHEAD < stages; s += 2) {
+        step(s, next[0], odd, other, false, true);
+        step(s + 1, second, fa, fb, false, true);
+    }
+    for (; s < stages; ++s) {                                  // the last ones, by turns through copies
+        step(s, next[0], odd, other, false, false);
+        if constexpr (AHEAD == 2) {
+#pragma unroll
+            for (int q = 0; q < NP * PIECES; ++q) {
+                const half8 t = next[0][q];
+                next[0][q] = next[1][q];
+                next[1][q] = t;
+            }
+        }
+        if constexpr (!QUADS) {
+            const Part t = fa;
+            fa = fb;
+            fb = t;
         }
     }
-    // lane: column (lane & 31) of its wavefront's 32 x 32, rows 8 (r / 4) + 4 (lane / 32) + r % 4
-    float alpha = a.alpha[e.op];
-    if constexpr (KIND == GRAM || KIND == APPLY)
-        if (a.use_rho) alpha *= KIND == GRAM ? a.rho[e.slot] * a.rho[e.slot] : a.rho[e.slot];
-    const int j = tj * kTile + wj + (lane & 31);
+    multiply(QUADS ? fb : other);
+
+    // ---- the result through LDS, so that it leaves in whole rows of either order.  Lane: column (lane & 31) of a
+    // 32 x 32 block, rows 8 (r / 4) + 4 (lane / 32) + r % 4
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < BLK * BLK; ++q)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const int i = bi + q / BLK * 32 + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3), j = bj + q % BLK * 32 + (lane & 31);
+            out[(QUADS ? wave & 1 : wave) * TILE * LD + i * LD + j] = acc[q / BLK][q % BLK][r];
+        }
+    __syncthreads();
+    const auto sum_at = [&](int at) {                         // the wavefronts' shares of one value
+        float v = out[at];
+#pragma unroll
+        for (int h = 1; h < SHARES; ++h) v += out[h * TILE * LD + at];
+        return v;
+    };
+    if (o.kind == GRAM && e.split > 1) {
+        float* to = a.sums + ((size_t)e.sums0 + (size_t)block * e.split + share) * TILE * TILE;
+#pragma unroll 4
+        for (int id = tid; id < TILE * TILE; id += THREADS) to[id] = sum_at(id / TILE * LD + id % TILE);
+        return;
+    }
+    float alpha = o.alpha;
+    if (o.use_rho) alpha *= o.kind == GRAM ? a.rho[w] * a.rho[w] : a.rho[w];
+    const int i0 = ti * TILE, j0 = tj * TILE;
+    if (o.kind == APPLY && o.last) {
+#pragma unroll 4
+        for (int id = tid; id < TILE * TILE; id += THREADS) {
+            const int fast = id % TILE, slow = id / TILE;     // fast: along the tensor's rows
+            const int r = e.tall ? fast : slow, c = e.tall ? slow : fast;
+            if (i0 + r < e.m && j0 + c < e.n) {
+                const size_t at = e.tall ? (size_t)(j0 + c) * e.m + (i0 + r) : (size_t)(i0 + r) * e.n + (j0 + c);
+                float v = sum_at(r * LD + c) * alpha;
+                if (a.step) v = fmaf(a.decay, ld_any(e.out, a.out_type, at), -e.lr * v);
+                st_any(e.out, a.out_type, at, v);
+            }
+        }
+        return;
+    }
+    // To the buffers, eight values of a row at a time: the tile, and its mirror image (or, of X, the transpose).  A tile
+    // on the diagonal holds every pair twice, its cross terms summed in two orders: the upper one counts for both.
+    const bool diagonal = o.kind != APPLY && ti == tj;
+    constexpr int G = TILE / 8;
+    for (int side = 0; side < (diagonal ? 1 : 2); ++side) {
+        int ld;
+        size_t plane;
+        _Float16* d = buffer(e, a.planes, o.kind == APPLY && side == 0 ? (int)BUF_X : o.dst, ld, plane);
+        const int to_i = side ? j0 : i0, to_j = side ? i0 : j0, rows = side ? rows2 : rows1, cols = side ? rows1 : rows2;
+#pragma unroll 2
+        for (int id = tid; id < TILE * G; id += THREADS) {
+            const int r = id / G, c = id % G * 8;
+            if (r >= rows || c >= cols) continue;
+            const size_t at = (size_t)(to_i + r) * ld + to_j + c;
+            float v[8];
+            half8 hi, lo;
+            if (o.kind == POLY) {                             // (A is its own mirror image)
+                int lda;
+                size_t pa;
+                const _Float16* A = buffer(e, a.planes, o.src1, lda, pa) + at;
+                hi = *reinterpret_cast<const half8*>(A);
+                lo = *reinterpret_cast<const half8*>(A + pa);
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = sum_at(side || (diagonal && r > c + j) ? (c + j) * LD + r : r * LD + c + j) * alpha;
+            if (o.kind == POLY) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    v[j] = fmaf(a.b, (float)hi[j] + (float)lo[j], v[j]);
+                    if (to_i + r == to_j + c + j && to_i + r < e.m) v[j] += a.a;
+                }
+            }
+            split8(d + at, plane, v);
+        }
+    }
+}
+
+// The shares of the Gram tiles' depth, added in order, to A (one TILE x TILE tile per workgroup, upper triangle)
+template <int TILE>
+__global__ __launch_bounds__(256) void ns_gram_sum_kernel(Launch a) {
+    constexpr int LD = TILE + 1;
+    __shared__ float out[TILE * LD];
+    const int tid = threadIdx.x, lane = tid & 63;
+    int block = blockIdx.x;
+    int mine = 0;
+    if (lane < a.matrices && a.op[a.table[lane].plan][0].kind == GRAM && a.table[lane].split > 1)
+        mine = tiles_of(MUL, a.table[lane].mp, 0, 1, TILE);
+    const int w = find_matrix(mine, block);
+    const Matrix& e = a.table[w];
+    const Op& o = a.op[e.plan][0];
+    int ti, tj;
+    upper_tile(block, (e.mp + TILE - 1) / TILE, ti, tj);
+    const float4* from = reinterpret_cast<const float4*>(a.sums + ((size_t)e.sums0 + (size_t)block * e.split) * TILE * TILE);
+    float alpha = o.alpha;
+    if (o.use_rho) alpha *= a.rho[w] * a.rho[w];
+    constexpr int QUARTS = TILE * TILE / 4, EACH = QUARTS / 256 % 4 == 0 ? 4 : 3;
+    static_assert(QUARTS % (256 * EACH) == 0, "loads in flight per lane");
+    for (int g = 0; g < QUARTS / 256; g += EACH) {
+        float4 v[EACH];
+#pragma unroll
+        for (int q = 0; q < EACH; ++q) v[q] = from[tid + 256 * (g + q)];
+#pragma unroll 4
+        for (int h = 1; h < e.split; ++h)
+#pragma unroll
+            for (int q = 0; q < EACH; ++q) {
+                const float4 u = from[(size_t)h * QUARTS + tid + 256 * (g + q)];
+                v[q].x += u.x;
+                v[q].y += u.y;
+                v[q].z += u.z;
+                v[q].w += u.w;
+            }
+#pragma unroll
+        for (int q = 0; q < EACH; ++q) {
+            const int id = 4 * (tid + 256 * (g + q)), at = id / TILE * LD + id % TILE;
+            out[at] = v[q].x * alpha;
+            out[at + 1] = v[q].y * alpha;
+            out[at + 2] = v[q].z * alpha;
+            out[at + 3] = v[q].w * alpha;
+        }
+    }
+    __syncthreads();
     int ld;
     size_t plane;
+    _Float16* d = buffer(e, a.planes, o.dst, ld, plane);
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-        const int i = ti * kTile + wi + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3);
-        float v = acc[r] * alpha;
-        if constexpr (KIND == APPLY) {
-            if (a.last) {
-                if (i < e.m && j < e.n) {
-                    const Io& o = io.e[w];
-                    const size_t at = o.tall ? (size_t)j * e.m + i : (size_t)i * e.n + j;
-                    if (a.step) v = fmaf(a.decay, ld_any(o.out, a.out_type, at), -o.lr * v);
-                    st_any(o.out, a.out_type, at, v);
-                }
-            } else {
-                _Float16* x = buffer(e, a.planes, BUF_X, ld, plane);
-                split_store(x, plane, (size_t)i * ld + j, v);
-                x = buffer(e, a.planes, e.dst, ld, plane);
-                split_store(x, plane, (size_t)j * ld + i, v);
+    for (int side = 0; side < 2; ++side) {
+        if (side == 1 && ti == tj) break;
+        const int i0 = (side ? tj : ti) * TILE, j0 = (side ? ti : tj) * TILE;
+#pragma unroll 2
+        for (int id = tid; id < TILE * TILE / 8; id += 256) {
+            const int r = id / (TILE / 8), c = id % (TILE / 8) * 8;
+            if (i0 + r >= e.mp || j0 + c >= e.mp) continue;
+            float v[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const bool other = side || (ti == tj && r > c + j);
+                v[j] = other ? out[(c + j) * LD + r] : out[r * LD + c + j];
             }
-        } else {
-            if constexpr (KIND == POLY) {
-                const _Float16* A = buffer(e, a.planes, e.src1, ld, plane);
-                const size_t at = (size_t)i * ld + j;
-                v = fmaf(a.b, (float)A[at] + (float)A[plane + at], v);
-                if (i == j && i < e.m) v += a.a;
-            }
-            _Float16* d = buffer(e, a.planes, e.dst, ld, plane);
-            // a tile on the diagonal computes each pair twice, with its cross terms in two orders: one of them counts
-            if (ti != tj || i <= j) split_store(d, plane, (size_t)i * ld + j, v);
-            if (ti != tj || i < j) split_store(d, plane, (size_t)j * ld + i, v);
+            split8(d + (size_t)(i0 + r) * ld + j0 + c, plane, v);
         }
     }
 }
@@ -341,20 +678,15 @@ struct Call {
 struct Shape {
     int64_t m, n, mp, np;
     int64_t parts() const { return (m * n + kChunk - 1) / kChunk; }
-    int64_t halves() const { return 6 * mp * np + (int64_t)(BUF_COUNT - BUF_A) * 2 * mp * mp; }
+    int64_t halves() const { return before(BUF_COUNT, mp, np); }
 };
 bool shape_of(int64_t rows, int64_t cols, Shape& s) {
-    const int64_t most = 1 << 24;
+    const int64_t most = 1 << 23;
     if (rows < 0 || cols < 0 || rows >= most || cols >= most) return false;
     s.m = rows < cols ? rows : cols;
     s.n = rows < cols ? cols : rows;
-    s.mp = (s.m + kTile - 1) / kTile * kTile;
-    s.np = (s.n + kTile - 1) / kTile * kTile;
-    return (s.mp / kTile) * (s.np / kTile) < (1 << 22);       // workgroups of a launch
+    return (s.m / 64 + 2) * (s.n / 64 + 2) < (1 << 22);       // workgroups of a launch
 }
-
-// Bytes of the workspace's head: the partial sums and one factor per matrix
-int64_t head_bytes(int64_t parts) { return (parts * 8 + kMaxItems * 4 + 255) / 256 * 256; }
 
 float pow2_below(double bound) { return (float)std::exp2(14.0 - std::ceil(std::log2(bound))); }     // bound * it <= 2^14
 
@@ -367,8 +699,8 @@ bool scales_of(const Call& k, int longest, Scales& s) {
     double top = 1.0, all = 1.0;
     for (int i = 0; i < k.steps; ++i) {
         double next = 0.0;
-        for (int j = 0; j <= 2048; ++j) {
-            const double x = top * j / 2048.0, p = std::fabs(x * (k.a + x * x * (k.b + x * x * k.c)));
+        for (int j = 0; j <= 512; ++j) {
+            const double x = top * j / 512.0, p = std::fabs(x * (k.a + x * x * (k.b + x * x * k.c)));
             if (!(p <= next)) next = p;
         }
         top = next * 1.01;
@@ -377,8 +709,8 @@ bool scales_of(const Call& k, int longest, Scales& s) {
     }
     const double lam = all * all * 1.05;
     double q = 0.0, r = 0.0;
-    for (int j = 0; j <= 2048; ++j) {
-        const double x = lam * j / 2048.0, v = std::fabs(k.a + x * (k.b + x * k.c));
+    for (int j = 0; j <= 512; ++j) {
+        const double x = lam * j / 512.0, v = std::fabs(k.a + x * (k.b + x * k.c));
         if (v > q) q = v;
         if (v * x > r) r = v * x;
     }
@@ -391,170 +723,248 @@ bool scales_of(const Call& k, int longest, Scales& s) {
     return true;
 }
 
-// The steps of one matrix in segments; segment lengths fall on step k with starts(k) / ends(k).
-struct Segments {
-    int first, rest;                  // length of the first one, of the others (the last may be shorter)
-    bool starts(int k) const { return k == 0 || (k >= first && (k - first) % rest == 0); }
-    bool ends(int k, int steps) const { return k == steps - 1 || starts(k + 1); }
+// The steps of a plan in segments of the Gram form: plan 0 (16-bit results) five at once, (fp32) one by one; plan 1
+// two, then three.  More than five steps of an fp32 result go one by one: near one the usual polynomial spreads
+// neighbouring values (its slope is -1.4 at 0.75), so that every further step amplifies what a segment rounded.
+int plan_of(int out_type, int steps, const Shape& s) {
+    return out_type == FC3D_F32 && s.n >= 2 * s.m && s.m > 64 && steps <= 5;
+}
+bool starts(int out_type, int plan, int step) {
+    if (out_type != FC3D_F32) return step % 5 == 0;
+    return plan == 0 || step == 0 || step == 2;
+}
+
+constexpr int kMaxOps = 5 * 64;
+struct PlanOps {
+    int count;
+    Op op[kMaxOps][2];
 };
-// More than five steps of an fp32 result go one by one: near one the usual polynomial spreads neighbouring values
-// (its slope is -1.4 at 0.75), so that every further step amplifies what the segments before it rounded.
-Segments segments_of(int out_type, int steps, const Shape& s) {
-    if (out_type != FC3D_F32) return {5, 5};
-    if (s.n < 2 * s.m || steps > 5) return {1, 1};
-    return {2, 3};
-}
-
-template <int N>
-int64_t workgroups(Jobs<N>& t, int kind) {        // numbers the entries' workgroups, returns their sum
-    int64_t sum = 0;
-    for (int i = 0; i < t.count; ++i) {
-        Job& e = t.e[i];
-        const int64_t tm = padded(e.m) / kTile, tn = padded(e.n) / kTile;
-        e.first = (int)sum;
-        sum += kind == APPLY ? tm * tn : tm * (tm + 1) / 2;
+// Every launch's products of one plan
+void ops_of(const Call& k, int plan, const Scales& s, bool exact, PlanOps& to) {
+    to.count = 0;
+    uint8_t xt = BUF_XT0, p = BUF_P0;
+    const auto put = [&](Op first, Op second) {
+        to.op[to.count][0] = first;
+        to.op[to.count++][1] = second;
+    };
+    const Op none = {};
+    bool first_segment = true;
+    for (int step = 0; step < k.steps; ++step) {
+        const bool begin = starts(k.out_type, plan, step), end = step + 1 == k.steps || starts(k.out_type, plan, step + 1);
+        const uint8_t rho = exact && first_segment;
+        if (begin) put(Op{GRAM, BUF_X, BUF_X, BUF_A, s.a / (s.x * s.x), rho, 0}, none);
+        const uint8_t q = begin ? BUF_P0 : BUF_Q;              // the first of a segment is its running product too
+        if (begin) p = BUF_P0;
+        put(Op{POLY, BUF_A, BUF_A, q, (float)k.c * s.q / (s.a * s.a), 0, 0}, none);
+        Op running = none;
+        if (!begin) {
+            const uint8_t np = p == BUF_P0 ? BUF_P1 : BUF_P0;
+            running = Op{MUL, p, q, np, 1.0f / s.q, 0, 0};
+            p = np;
+        }
+        if (!end) {
+            put(Op{MUL, BUF_A, q, BUF_R, s.r / (s.a * s.q), 0, 0}, running);
+            put(Op{MUL, BUF_R, q, BUF_A, s.a / (s.r * s.q), 0, 0}, none);
+        } else {
+            if (running.kind != NONE) put(running, none);
+            const uint8_t last = step + 1 == k.steps, nxt = xt == BUF_XT0 ? BUF_XT1 : BUF_XT0;
+            put(Op{APPLY, p, xt, nxt, (last ? 1.0f : s.x) / (s.q * s.x), rho, last}, none);
+            xt = nxt;
+            first_segment = false;
+        }
     }
-    return sum;
 }
 
-int run_group(const Call& k, int from, int count, const Shape* shapes, const Scales& sc) {
-    Jobs<kMaxItems> all = {};
-    Ios io = {};
-    all.count = count;
-    int64_t parts = 0, halves = 0, norm_groups = 0, prep_groups = 0;
-    bool exact = k.g_type != FC3D_F32 && !k.mom;
+// What a group of matrices is worked on with, from its sizes alone: the workspace's size and its layout follow from it.
+struct Layout {
+    int64_t parts, halves, sum_tiles;
+    int gram;                         // the Gram products' kernel
+    int order[kMaxItems];             // the group's matrices as they are worked on: deep ones first, they take longest
+    Shape shape[kMaxItems];           // in that order, like split
+    int split[kMaxItems];
+    int64_t head() const { return (parts * 8 + kMaxItems * (4 + (int64_t)sizeof(Matrix)) + 255) / 256 * 256; }
+    int64_t sums_at() const { return head() + (halves * 2 + 255) / 256 * 256; }
+    int64_t bytes() const;
+};
+
+// The kernels a launch can take.  `beside`: workgroups that a compute unit holds.  A round of workgroups on all units
+// takes `fixed` microseconds (starting, finding the tile, the first operands, the result's way out) and slice[] for every
+// 64 of the depth, by the operands' planes (2 x 2, 2 x 1, 1 x 1); fitted to launches of 100 to 4000 tiles at depths of
+// 512 to 8192.  Two small workgroups per unit hide each other's waits best; 96 x 96 tiles fill one round where the small
+// ones need a second (2048 rows: 253 tiles, 41 us, against 50 us for 528); 128 x 128 tiles read least, for launches of many
+// rounds (2048 x 8192, P X: 165 us against 210) and matrices of 1024 rows (35 us against 42).
+struct Kernel {
+    int tile, waves, beside;
+    double fixed, slice[3];
+};
+constexpr Kernel kKernels[] = {
+    {64, 4, 2, 7.0, {0.75, 0.60, 0.42}}, {96, 4, 1, 8.0, {1.03, 0.95, 0.52}}, {128, 8, 1, 6.5, {1.75, 1.10, 0.75}}};
+constexpr int kKernelCount = sizeof(kKernels) / sizeof(kKernels[0]);
+constexpr int kUnits = 256;           // compute units
+
+// The kernel with the least expected time.  The last round, when not full, costs less: nothing shares its units.
+int kernel_for(const int64_t (&groups)[kKernelCount], int64_t slices, int planes) {
+    int best = 0;
+    double least = 1e300;
+    for (int i = 0; i < kKernelCount; ++i) {
+        const Kernel& c = kKernels[i];
+        const int64_t slots = (int64_t)kUnits * c.beside, rest = groups[i] % slots;
+        const double round = c.fixed + c.slice[planes] * (double)slices;
+        const double t = round * ((double)(groups[i] / slots) + (rest ? 0.6 + 0.4 * (double)rest / (double)slots : 0.0));
+        if (t < least) {
+            least = t;
+            best = i;
+        }
+    }
+    return best;
+}
+
+int64_t Layout::bytes() const {
+    return sums_at() + sum_tiles * kKernels[gram].tile * kKernels[gram].tile * 4;
+}
+
+int layout_of(const Call& k, int from, int count, Layout& l) {
     for (int i = 0; i < count; ++i) {
-        const int at = from + i;
-        const Shape& s = shapes[i];
-        all.e[i] = Job{halves, (int)s.m, (int)s.n, 0, 0, 0, 0, 0, i};
-        io.e[i] = Io{k.g[at], k.mom ? k.mom[at] : nullptr, k.out[at], k.lr ? k.lr[at] : 0.0f, k.rows[at] > k.cols[at], (int)parts};
+        Shape s;
+        if (!shape_of(k.rows[from + i], k.cols[from + i], s)) return FC3D_ERANGE;
+        if (s.m == 0) return FC3D_EINVAL;
+        int at = i;                                           // insertion: equal ones keep their order
+        for (; at > 0 && l.shape[at - 1].n < s.n; --at) {
+            l.shape[at] = l.shape[at - 1];
+            l.order[at] = l.order[at - 1];
+        }
+        l.shape[at] = s;
+        l.order[at] = i;
+    }
+    int64_t prep = 0, depth = 0;
+    int64_t groups[kKernelCount] = {};
+    l.parts = l.halves = 0;
+    for (int i = 0; i < count; ++i) {
+        Shape& s = l.shape[i];
+        s.mp = (s.m + kSlice - 1) / kSlice * kSlice;
+        s.np = (s.n + kSlice - 1) / kSlice * kSlice;
+        l.parts += s.parts();
+        l.halves += s.halves();
+        prep += s.mp / 64 * (s.np / 64);
+        for (int c = 0; c < kKernelCount; ++c) groups[c] += tiles_of(MUL, (int)s.mp, 0, 1, kKernels[c].tile);
+        if (s.np / kSlice > depth) depth = s.np / kSlice;
+    }
+    if (prep >= (1 << 23) || l.parts >= (1 << 23)) return FC3D_ERANGE;      // workgroups of one launch
+    // The Gram products: the kernel is picked for them once, since the sums of shared depth are laid out for its tile.
+    // Where there are few tiles, the depth is shared out, eight slices at least to each workgroup, one round of them.
+    l.gram = kernel_for(groups, depth, k.g_type != FC3D_F32 && !k.mom ? 2 : 0);
+    const int tile = kKernels[l.gram].tile;
+    int64_t tiles = groups[l.gram], slices = 0;
+    for (int i = 0; i < count; ++i) slices += tiles_of(MUL, (int)l.shape[i].mp, 0, 1, tile) * (l.shape[i].np / kSlice);
+    int64_t each = (slices + kUnits - 1) / kUnits;
+    if (each < 8) each = 8;
+    for (;; ++each) {
+        int64_t all = 0;
+        l.sum_tiles = 0;
+        for (int i = 0; i < count; ++i) {
+            const int64_t deep = l.shape[i].np / kSlice, t = tiles_of(MUL, (int)l.shape[i].mp, 0, 1, tile);
+            int64_t split = (deep + each - 1) / each;
+            const int64_t per = (deep + split - 1) / split;
+            split = (deep + per - 1) / per;                   // no share without a slice
+            if (tiles > kUnits) split = 1;
+            l.split[i] = (int)split;
+            all += t * split;
+            if (split > 1) l.sum_tiles += t * split;
+        }
+        if (all <= kUnits || l.sum_tiles == 0) break;         // one round, or nothing left to share
+    }
+    return FC3D_OK;
+}
+
+int64_t groups_of(const Launch& a, const Table& t, int tile) {
+    int64_t n = 0;
+    for (int i = 0; i < t.count; ++i)
+        for (int j = 0; j < 2; ++j) n += tiles_of(a.op[t.e[i].plan][j].kind, t.e[i].mp, t.e[i].np, t.e[i].split, tile);
+    return n;
+}
+
+template <int TILE, int WAVES>
+int product(const Call& k, const Launch& a, int64_t groups, int p1, int p2) {
+    const dim3 grid((unsigned)groups), block(WAVES * 64);
+    if (p1 == 1) FC3D_LAUNCH("ns_product", (ns_product_kernel<TILE, WAVES, 1, 1>), grid, block, 0, k.s, a);
+    else if (p2 == 1) FC3D_LAUNCH("ns_product", (ns_product_kernel<TILE, WAVES, 2, 1>), grid, block, 0, k.s, a);
+    else FC3D_LAUNCH("ns_product", (ns_product_kernel<TILE, WAVES, 2, 2>), grid, block, 0, k.s, a);
+    return FC3D_OK;
+}
+
+int run_group(const Call& k, int from, const Layout& l, const Scales& sc, int count) {
+    Table t = {};
+    t.count = count;
+    const bool exact = k.g_type != FC3D_F32 && !k.mom;
+    int64_t parts = 0, halves = 0, prep = 0, sums = 0;
+    bool used[kPlans] = {};
+    for (int i = 0; i < count; ++i) {
+        const Shape& s = l.shape[i];
+        const int at = from + l.order[i], plan = plan_of(k.out_type, k.steps, s);
+        t.e[i] = Matrix{k.g[at], k.mom ? k.mom[at] : nullptr, k.out[at], halves, (int)s.m, (int)s.n, (int)s.mp, (int)s.np,
+                        k.lr ? k.lr[at] : 0.0f, (int)parts, l.split[i], (int)sums, k.rows[at] > k.cols[at], plan};
+        used[plan] = true;
         parts += s.parts();
         halves += s.halves();
+        prep += s.mp / 64 * (s.np / 64);
+        if (l.split[i] > 1) sums += (int64_t)tiles_of(MUL, (int)s.mp, 0, 1, kKernels[l.gram].tile) * l.split[i];
     }
-    double* sums = reinterpret_cast<double*>(k.ws);
-    float* rho = reinterpret_cast<float*>(k.ws + parts * 8);
-    _Float16* planes = reinterpret_cast<_Float16*>(k.ws + head_bytes(parts));
+    double* squares = reinterpret_cast<double*>(k.ws);
+    Matrix* table = reinterpret_cast<Matrix*>(k.ws + parts * 8);
+    float* rho = reinterpret_cast<float*>(table + kMaxItems);
+    _Float16* planes = reinterpret_cast<_Float16*>(k.ws + l.head());
+    FC3D_LAUNCH("ns_norm", ns_norm_kernel, dim3((unsigned)parts), dim3(256), 0, k.s, t, k.g_type, k.blend, squares, table);
+    FC3D_LAUNCH("ns_prepare", ns_prepare_kernel, dim3((unsigned)prep), dim3(256), 0, k.s, table, count, k.g_type, k.blend,
+                squares, k.eps, sc.x, (int)exact, planes, rho);
 
-    Jobs<kMaxItems> t = all;
-    for (int i = 0; i < count; ++i) {
-        t.e[i].first = (int)norm_groups;
-        norm_groups += shapes[i].parts();
+    static thread_local PlanOps ops[kPlans];
+    int launches = 0;
+    for (int p = 0; p < kPlans; ++p) {
+        ops[p].count = 0;
+        if (used[p]) ops_of(k, p, sc, exact, ops[p]);
+        if (ops[p].count > launches) launches = ops[p].count;
     }
-    FC3D_LAUNCH("ns_norm", ns_norm_kernel, dim3((unsigned)norm_groups), dim3(256), 0, k.s, t, io, k.g_type, k.blend, sums);
-    for (int i = 0; i < count; ++i) {
-        t.e[i].first = (int)prep_groups;
-        prep_groups += shapes[i].mp / kTile * (shapes[i].np / kTile);
-    }
-    FC3D_LAUNCH("ns_prepare", ns_prepare_kernel, dim3((unsigned)prep_groups), dim3(256), 0, k.s, t, io, k.g_type, k.blend, sums,
-                k.eps, sc.x, (int)exact, planes, rho);
-
-    uint8_t xt[kMaxItems], p[kMaxItems];
-    for (int i = 0; i < count; ++i) xt[i] = BUF_XT0;
-    Product arg = {};
-    arg.planes = planes;
-    arg.rho = rho;
-    arg.out_type = k.out_type;
-    arg.step = k.lr != nullptr;
-    arg.decay = k.decay;
-    for (int step = 0; step < k.steps; ++step) {
-        Segments seg[kMaxItems];
-        uint8_t q[kMaxItems];
-        Jobs<kMaxItems> one = {};
-        // A = X X^T where a segment starts
-        for (int i = 0; i < count; ++i) {
-            seg[i] = segments_of(k.out_type, k.steps, shapes[i]);
-            if (!seg[i].starts(step)) continue;
-            Job& e = one.e[one.count++] = all.e[i];
-            e.src1 = e.src2 = BUF_X;
-            e.dst = BUF_A;
-        }
-        arg.use_rho = exact && step == 0;
-        if (one.count) {
-            const int64_t n = workgroups(one, GRAM);
-            arg.alpha[0] = sc.a / (sc.x * sc.x);
-            if (arg.use_rho)
-                FC3D_LAUNCH("ns_gram", (ns_product_kernel<GRAM, 1, 1, kMaxItems, NoIos>), dim3((unsigned)n), dim3(256), 0, k.s,
-                            one, NoIos{}, arg);
-            else
-                FC3D_LAUNCH("ns_gram", (ns_product_kernel<GRAM, 2, 2, kMaxItems, NoIos>), dim3((unsigned)n), dim3(256), 0, k.s,
-                            one, NoIos{}, arg);
-        }
-        // Q = a I + b A + c A A; the first of a segment is its running product too
-        one.count = 0;
-        for (int i = 0; i < count; ++i) {
-            Job& e = one.e[one.count++] = all.e[i];
-            e.src1 = e.src2 = BUF_A;
-            q[i] = e.dst = seg[i].starts(step) ? BUF_P0 : BUF_Q;
-            if (seg[i].starts(step)) p[i] = BUF_P0;
-        }
-        const int64_t n = workgroups(one, POLY);
-        arg.alpha[0] = (float)k.c * sc.q / (sc.a * sc.a);
-        arg.a = (float)k.a * sc.q;
-        arg.b = (float)k.b * sc.q / sc.a;
-        FC3D_LAUNCH("ns_poly", (ns_product_kernel<POLY, 2, 2, kMaxItems, NoIos>), dim3((unsigned)n), dim3(256), 0, k.s, one,
-                    NoIos{}, arg);
-        // R = A Q where the segment goes on, P := P Q where it did not start here
-        Jobs<kMaxJobs> two = {};
-        for (int i = 0; i < count; ++i) {
-            if (!seg[i].ends(step, k.steps)) {
-                Job& e = two.e[two.count++] = all.e[i];
-                e.src1 = BUF_A;
-                e.src2 = q[i];
-                e.dst = BUF_R;
-                e.op = 0;
+    Launch a = {};
+    a.a = (float)k.a * sc.q;
+    a.b = (float)k.b * sc.q / sc.a;
+    a.out_type = k.out_type;
+    a.step = k.lr != nullptr;
+    a.decay = k.decay;
+    a.matrices = count;
+    a.table = table;
+    a.planes = planes;
+    a.rho = rho;
+    a.sums = reinterpret_cast<float*>(k.ws + l.sums_at());
+    for (int i = 0; i < launches; ++i) {
+        bool gram = false, rho_gram = false, rho_apply = false;
+        for (int p = 0; p < kPlans; ++p)
+            for (int j = 0; j < 2; ++j) {
+                a.op[p][j] = i < ops[p].count ? ops[p].op[i][j] : Op{};
+                gram = gram || a.op[p][j].kind == GRAM;
+                rho_gram = rho_gram || (a.op[p][j].kind == GRAM && a.op[p][j].use_rho);
+                rho_apply = rho_apply || (a.op[p][j].kind == APPLY && a.op[p][j].use_rho);
             }
-            if (!seg[i].starts(step)) {
-                Job& e = two.e[two.count++] = all.e[i];
-                e.src1 = p[i];
-                e.src2 = q[i];
-                e.dst = p[i] = p[i] == BUF_P0 ? BUF_P1 : BUF_P0;
-                e.op = 1;
-            }
+        // an input taken as it is has one plane (its plan is the only one: 16-bit results)
+        const int p1 = rho_gram ? 1 : 2, p2 = rho_gram || rho_apply ? 1 : 2;
+        int64_t groups[kKernelCount], depth = 0;
+        for (int c = 0; c < kKernelCount; ++c) groups[c] = groups_of(a, t, kKernels[c].tile);
+        for (int j = 0; j < count; ++j) {
+            const Op& o = a.op[t.e[j].plan][0];
+            const int64_t d = o.kind == NONE ? 0 : o.kind == GRAM ? t.e[j].np / kSlice / t.e[j].split : t.e[j].mp / kSlice;
+            if (d > depth) depth = d;
         }
-        if (two.count) {
-            const int64_t groups = workgroups(two, MUL);
-            arg.alpha[0] = sc.r / (sc.a * sc.q);
-            arg.alpha[1] = 1.0f / sc.q;
-            FC3D_LAUNCH("ns_mul", (ns_product_kernel<MUL, 2, 2, kMaxJobs, NoIos>), dim3((unsigned)groups), dim3(256), 0, k.s, two,
-                        NoIos{}, arg);
-        }
-        // A := R Q
-        one.count = 0;
-        for (int i = 0; i < count; ++i) {
-            if (seg[i].ends(step, k.steps)) continue;
-            Job& e = one.e[one.count++] = all.e[i];
-            e.src1 = BUF_R;
-            e.src2 = q[i];
-            e.dst = BUF_A;
-        }
-        if (one.count) {
-            const int64_t groups = workgroups(one, MUL);
-            arg.alpha[0] = sc.a / (sc.r * sc.q);
-            FC3D_LAUNCH("ns_mul", (ns_product_kernel<MUL, 2, 2, kMaxItems, NoIos>), dim3((unsigned)groups), dim3(256), 0, k.s, one,
-                        NoIos{}, arg);
-        }
-        // X := P X where a segment ends, to the tensors behind the last one
-        one.count = 0;
-        Ios to = {};
-        for (int i = 0; i < count; ++i) {
-            if (!seg[i].ends(step, k.steps)) continue;
-            to.e[one.count] = io.e[i];
-            Job& e = one.e[one.count++] = all.e[i];
-            e.src1 = p[i];
-            e.src2 = xt[i];
-            e.dst = xt[i] = xt[i] == BUF_XT0 ? BUF_XT1 : BUF_XT0;
-        }
-        if (one.count) {
-            const int64_t groups = workgroups(one, APPLY);
-            arg.last = step == k.steps - 1;
-            arg.use_rho = exact && step < 5;          // the first segment of 16-bit results
-            arg.alpha[0] = (arg.last ? 1.0f : sc.x) / (sc.q * sc.x);
-            if (arg.use_rho)
-                FC3D_LAUNCH("ns_apply", (ns_product_kernel<APPLY, 2, 1, kMaxItems, Ios>), dim3((unsigned)groups), dim3(256), 0, k.s,
-                            one, to, arg);
-            else
-                FC3D_LAUNCH("ns_apply", (ns_product_kernel<APPLY, 2, 2, kMaxItems, Ios>), dim3((unsigned)groups), dim3(256), 0, k.s,
-                            one, to, arg);
+        const int c = gram ? l.gram : kernel_for(groups, depth, p2 == 2 ? 0 : 1);
+        const int rc = c == 0 ? product<64, 4>(k, a, groups[c], p1, p2) : c == 1 ? product<96, 4>(k, a, groups[c], p1, p2)
+                                                                       : product<128, 8>(k, a, groups[c], p1, p2);
+        if (rc != FC3D_OK) return rc;
+        int64_t sum_groups = 0;
+        for (int j = 0; j < count; ++j)
+            if (a.op[t.e[j].plan][0].kind == GRAM && t.e[j].split > 1) sum_groups += tiles_of(MUL, t.e[j].mp, 0, 1, kKernels[c].tile);
+        if (sum_groups) {
+            const dim3 grid((unsigned)sum_groups);
+            if (kKernels[c].tile == 64) FC3D_LAUNCH("ns_gram_sum", ns_gram_sum_kernel<64>, grid, dim3(256), 0, k.s, a);
+            else if (kKernels[c].tile == 96) FC3D_LAUNCH("ns_gram_sum", ns_gram_sum_kernel<96>, grid, dim3(256), 0, k.s, a);
+            else FC3D_LAUNCH("ns_gram_sum", ns_gram_sum_kernel<128>, grid, dim3(256), 0, k.s, a);
         }
     }
     return FC3D_OK;
@@ -566,7 +976,6 @@ bool off_align(const void* p, int type) { return (reinterpret_cast<uintptr_t>(p)
 // Matrices in groups of kMaxItems, one group after the other in the same workspace.  `run`: false only sizes it.
 int walk(const Call& k, bool run, size_t& bytes) {
     bytes = 0;
-    Shape shapes[kMaxItems];
     Scales sc = {};
     if (run) {
         const int longest = k.out_type == FC3D_F32 ? 3 : 5;
@@ -574,19 +983,11 @@ int walk(const Call& k, bool run, size_t& bytes) {
     }
     for (int from = 0; from < k.count; from += kMaxItems) {
         const int count = k.count - from < kMaxItems ? k.count - from : kMaxItems;
-        int64_t parts = 0, halves = 0, tiles = 0;
-        for (int i = 0; i < count; ++i) {
-            if (!shape_of(k.rows[from + i], k.cols[from + i], shapes[i])) return FC3D_ERANGE;
-            if (shapes[i].m == 0) return FC3D_EINVAL;
-            parts += shapes[i].parts();
-            halves += shapes[i].halves();
-            tiles += shapes[i].mp / kTile * (shapes[i].np / kTile);
-        }
-        if (tiles >= (1 << 23) || parts >= (1 << 23)) return FC3D_ERANGE;      // workgroups of one launch
-        const size_t need = (size_t)(head_bytes(parts) + halves * 2);
-        if (need > bytes) bytes = need;
+        Layout l = {};
+        if (const int rc = layout_of(k, from, count, l)) return rc;
+        if ((size_t)l.bytes() > bytes) bytes = (size_t)l.bytes();
         if (run)
-            if (const int rc = run_group(k, from, count, shapes, sc)) return rc;
+            if (const int rc = run_group(k, from, l, sc, count)) return rc;
     }
     return FC3D_OK;
 }

@@ -467,7 +467,7 @@ int fc3d_layer_norm_bwd(void *stream, const void *dy, const void *x, int x_type,
  * operand a pair of fp16 values and fp32 sums: the accuracy of fp32 products.  HOST arrays:
  * g, out (device pointers to dense row-major [rows][cols] tensors of `type`; out[i] may be
  * g[i]), rows, cols; they may be freed after the call.  A matrix must have a row and a column.
- * FC3D_ERANGE: sizes beyond 2^24, or coefficients that let singular values grow (beyond 16).
+ * FC3D_ERANGE: sizes beyond 2^23, or coefficients that let singular values grow (beyond 16).
  * workspace: fc3d_orthogonalize_workspace() bytes, 256-byte aligned, need not be initialised;
  * calls that may run at the same time need one each.                                          */
 size_t fc3d_orthogonalize_workspace(int count, const int64_t *rows, const int64_t *cols);
