@@ -1219,22 +1219,45 @@ def _norm_out(x, dim, last):
     return torch.empty_permuted(x.shape, perm, dtype=x.dtype, device=x.device)
 
 
+_get_device = torch._C._cuda_getDevice
+
+
 def _norm_forward(x, weight, bias, eps, dim, relu, want_stats):
-    last = _norm_last(x, dim)
-    xd, outer, C, inner, step = _norm_layout(x, dim, last)
-    y = _norm_out(x, dim, last)
-    stats = torch.empty((2, outer * inner), dtype=torch.float32, device=x.device) if want_stats else None
+    """(y, x as the kernel read it, statistics or None, what the backward pass needs to know of the layout)."""
+    if x.is_contiguous():
+        shape = x.shape
+        C = shape[dim]
+        inner = 1
+        for n in shape[dim + 1:]:
+            inner *= n
+        outer = x.numel() // (C * inner) if inner else 0
+        last, xd, step = dim == len(shape) - 1, x, C * inner
+        y = torch.empty_like(x)
+    else:
+        last = _norm_last(x, dim)
+        xd, outer, C, inner, step = _norm_layout(x, dim, last)
+        y = _norm_out(x, dim, last)
+    code = _TYPES[x.dtype]
     p = weight if weight is not None else bias
-    with _on_device(x.device):
-        status = _lib.fc3d_layer_norm_fwd(_stream(), xd.data_ptr(), _TYPES[x.dtype],
+    p_code = code if p is None or p.dtype == x.dtype else 0
+    n = outer * inner
+    stats = torch.empty(2 * n, dtype=torch.float32, device=x.device) if want_stats else None
+    at = stats.data_ptr() if want_stats else None
+    dev = x.get_device()
+    ctx = None if dev == _get_device() else _on_device(x.device)
+    if ctx is not None:
+        ctx.__enter__()
+    try:
+        status = _lib.fc3d_layer_norm_fwd(_raw_stream(dev) if _raw_stream is not None else _stream(), xd.data_ptr(), code,
                                           weight.data_ptr() if weight is not None else None,
-                                          bias.data_ptr() if bias is not None else None,
-                                          _TYPES[p.dtype] if p is not None else 0, outer, C, inner, step, eps, relu,
-                                          y.data_ptr(), stats.data_ptr() if want_stats else None,
-                                          stats.data_ptr() + 4 * outer * inner if want_stats else None)
-        if status:
-            _check(status, "fc3d_layer_norm_fwd")
-    return y, xd, stats, last
+                                          bias.data_ptr() if bias is not None else None, p_code, outer, C, inner, step, eps,
+                                          relu, y.data_ptr(), at, at + 4 * n if want_stats else None)
+    finally:
+        if ctx is not None:
+            ctx.__exit__(None, None, None)
+    if status:
+        _check(status, "fc3d_layer_norm_fwd")
+    return y, xd, stats, (dim, last, relu, outer, C, inner, step, code, p_code, dev)
 
 
 class LayerNormFn(torch.autograd.Function):
@@ -1242,38 +1265,43 @@ class LayerNormFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, weight, bias, eps, dim, relu):
-        y, xd, stats, last = _norm_forward(x, weight, bias, eps, dim, relu, True)
-        ctx.save_for_backward(xd, weight, bias if relu else None, stats)
-        ctx.meta = (dim, last, relu, xd is x, None if bias is None else bias.dtype)
+        y, xd, stats, meta = _norm_forward(x, weight, bias, eps, dim, relu, True)
+        ctx.save_for_backward(xd, weight, bias, stats)
+        ctx.meta = meta
         return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
         xd, weight, bias, stats = ctx.saved_tensors
-        dim, last, relu, as_given, bias_dtype = ctx.meta
+        dim, last, relu, outer, C, inner, x_step, code, p_code, dev = ctx.meta
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
-        dev = xd.device
-        g, outer, C, inner, g_step = _norm_layout(dy, dim, last)
-        # a copy that the forward made is dense in the order the kernels read
-        x_step = _norm_layout(xd, dim, last)[4] if as_given else C * inner
-        p_dtype = weight.dtype if weight is not None else bias_dtype
-        dx = _norm_out(xd if as_given else dy, dim, last) if need_x else None
-        dw = torch.empty(C, dtype=weight.dtype, device=dev) if need_w else None
-        db = torch.empty(C, dtype=bias_dtype, device=dev) if need_b else None
+        if dy.is_contiguous() and (not last or dim == dy.dim() - 1):
+            g, g_step = dy, C * inner
+        else:
+            g, _, _, _, g_step = _norm_layout(dy, dim, last)
+        dx = _norm_out(dy, dim, last) if need_x else None
+        dw = torch.empty_like(weight) if need_w else None
+        db = torch.empty_like(bias) if need_b else None
         ws = None
         if need_w or need_b:
-            ws = torch.empty(_lib.fc3d_layer_norm_bwd_workspace(_TYPES[xd.dtype], outer, C, inner) // 4,
-                             dtype=torch.float32, device=dev)
-        with _on_device(dev):
-            _check(_lib.fc3d_layer_norm_bwd(_stream(), g.data_ptr(), xd.data_ptr(), _TYPES[xd.dtype],
-                                            weight.data_ptr() if weight is not None else None,
-                                            bias.data_ptr() if bias is not None else None,
-                                            _TYPES[p_dtype] if p_dtype is not None else 0, stats.data_ptr(),
-                                            stats.data_ptr() + 4 * outer * inner, outer, C, inner, g_step, x_step,
-                                            relu, dx.data_ptr() if need_x else None, dw.data_ptr() if need_w else None,
-                                            db.data_ptr() if need_b else None, ws.data_ptr() if ws is not None else None),
-                   "fc3d_layer_norm_bwd")
+            ws = torch.empty(_lib.fc3d_layer_norm_bwd_workspace(code, outer, C, inner), dtype=torch.uint8, device=xd.device)
+        at = stats.data_ptr()
+        other = None if dev == _get_device() else _on_device(xd.device)
+        if other is not None:
+            other.__enter__()
+        try:
+            status = _lib.fc3d_layer_norm_bwd(_raw_stream(dev) if _raw_stream is not None else _stream(), g.data_ptr(),
+                                              xd.data_ptr(), code, weight.data_ptr() if weight is not None else None,
+                                              bias.data_ptr() if bias is not None else None, p_code, at,
+                                              at + 4 * outer * inner, outer, C, inner, g_step, x_step, relu,
+                                              dx.data_ptr() if need_x else None, dw.data_ptr() if need_w else None,
+                                              db.data_ptr() if need_b else None, ws.data_ptr() if ws is not None else None)
+        finally:
+            if other is not None:
+                other.__exit__(None, None, None)
+        if status:
+            _check(status, "fc3d_layer_norm_bwd")
         return dx, dw, db, None, None, None
 
 

@@ -228,6 +228,18 @@ def test_strides_and_alignment(dt):
         (dx,) = torch.autograd.grad(y, xs, dyv.cuda() if dyv is dy else dyv[:1, :1, :].cuda().expand(6, 5, 65))
         close(y, r["y"], r["ey"], dt, "rows of a wider tensor")
         close(dx, r["dx"], r["edx"], dt, "rows of a wider tensor")
+    # the normalised axis contiguous in the middle, the others not walked with one stride, all sizes alike
+    x, w, b, dy = inputs((4, 4, 4), 1, dt, F32, 7)
+    r = formula(x, w, b, dy, 1, 1e-5)
+    xs = torch.zeros(4, 6, 4, dtype=dt, device="cuda")
+    xs[:, :4] = x.cuda().transpose(1, 2)
+    xs = xs[:, :4].transpose(1, 2).detach().requires_grad_()
+    y = ops.layer_norm(xs, w.cuda(), b.cuda(), dim=1)
+    (dx,) = torch.autograd.grad(y, xs, dy.cuda())
+    close(y, r["y"], r["ey"], dt, "middle axis")
+    close(dx, r["dx"], r["edx"], dt, "middle axis")
+    x = inputs((6, 5, 65), -1, dt, F32, 6)[0]
+    w, b = inputs((6, 5, 65), -1, dt, F32, 6)[1:3]
     one = x[:1, :1].cuda().expand(6, 5, 65)
     r = formula(one.cpu(), w, b, None, -1, 1e-5)
     close(ops.layer_norm(one, w.cuda(), b.cuda()), r["y"], r["ey"], dt, "expanded input")
