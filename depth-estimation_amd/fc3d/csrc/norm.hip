@@ -16,25 +16,33 @@
 // small launch: no atomics, the same bits on every run.
 #include "fc3d_common.h"
 
+#include <type_traits>
+
 namespace fc3d {
 namespace {
 
 typedef __bf16 bf16;
 typedef _Float16 f16;
 
-constexpr int kVec = 4;              // values of one vector access: 16 bytes of fp32, 8 of a 16-bit type
+constexpr int kVec = 4;              // planes: values of one vector access (16 bytes of fp32, 8 of a 16-bit type)
 
 template <typename T, int V>
 struct Vec {
     T e[V];
 };
-template <typename T>
-struct Word {
-    typedef uint32_t type __attribute__((ext_vector_type(2), aligned(2)));
+template <int BYTES, int ALIGN>
+struct Word;
+template <>
+struct Word<16, 4> {
+    typedef uint32_t type __attribute__((ext_vector_type(4), aligned(4)));
 };
 template <>
-struct Word<float> {
-    typedef uint32_t type __attribute__((ext_vector_type(4), aligned(4)));
+struct Word<16, 2> {
+    typedef uint32_t type __attribute__((ext_vector_type(4), aligned(2)));
+};
+template <>
+struct Word<8, 2> {
+    typedef uint32_t type __attribute__((ext_vector_type(2), aligned(2)));
 };
 // Vector accesses at the element's own alignment: rows of odd length and planes of odd size start anywhere, and
 // global loads and stores take any address on this chip.
@@ -44,7 +52,7 @@ __device__ __forceinline__ Vec<T, V> ldv(const T* p) {
     if constexpr (V == 1) {
         r.e[0] = *p;
     } else {
-        typedef typename Word<T>::type word;
+        typedef typename Word<V * sizeof(T), sizeof(T)>::type word;
         const word w = *reinterpret_cast<const word*>(p);
         __builtin_memcpy(&r, &w, sizeof(r));
     }
@@ -55,9 +63,10 @@ __device__ __forceinline__ void stv(T* p, const Vec<T, V>& v) {
     if constexpr (V == 1) {
         *p = v.e[0];
     } else {
-        typename Word<T>::type w;
+        typedef typename Word<V * sizeof(T), sizeof(T)>::type word;
+        word w;
         __builtin_memcpy(&w, &v, sizeof(v));
-        *reinterpret_cast<typename Word<T>::type*>(p) = w;
+        *reinterpret_cast<word*>(p) = w;
     }
 }
 // The first n of V values (n <= 0: none); the rest reads as zero.
@@ -100,75 +109,105 @@ __device__ __forceinline__ bool passes(float pre) { return !(pre <= 0.0f); }
 
 // Sum over the LPR lanes that share a row, the same bits in every lane.  Above one wavefront the wavefronts' sums
 // meet in LDS; `slot` alternates between two areas, so that one barrier per sum is enough.
-template <int LPR>
+template <int LPR, int BLOCK>
 __device__ __forceinline__ float group_sum(float v, float* red, int slot) {
 #pragma unroll
     for (int o = (LPR < 64 ? LPR : 64) / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
     if constexpr (LPR > 64) {
-        constexpr int nw = LPR / 64;
-        float* a = red + slot * nw;
+        float* a = red + slot * (BLOCK / 64);
         if ((threadIdx.x & 63) == 0) a[threadIdx.x >> 6] = v;
         __syncthreads();
+        a += threadIdx.x / LPR * (LPR / 64);
         v = a[0];
 #pragma unroll
-        for (int i = 1; i < nw; ++i) v += a[i];
+        for (int i = 1; i < LPR / 64; ++i) v += a[i];
     }
     return v;
 }
 
-constexpr int kRowElems = 16;        // values of a row that one lane holds
-
 // ---- rows -------------------------------------------------------------------------------------------------
-// LPR lanes per row, kRowElems values each; a workgroup takes rows blockIdx.x * (BLOCK / LPR) + k * gridDim.x * ...,
-// its lanes keep their columns' weights.
-template <typename T, int LPR, int BLOCK>
-__global__ __launch_bounds__(BLOCK) void ln_rows_fwd(const T* __restrict__ x, const void* __restrict__ w, const void* __restrict__ b, bool w_f32, long rows, int C, long x_stride,
-                                                     float eps, int relu, T* __restrict__ y, float* __restrict__ mean,
-                                                     float* __restrict__ rstd) {
-    constexpr int V = kVec, NV = kRowElems / V;
-    constexpr int RPB = BLOCK / LPR;
-    __shared__ float red[LPR > 64 ? 2 * (LPR / 64) : 1];
-    const int lane = threadIdx.x % LPR, sub = threadIdx.x / LPR;
-    const float fc = (float)C;
-    float wv[NV * V], bv[NV * V];
-#pragma unroll
-    for (int k = 0; k < NV; ++k) {
-        const int c0 = (lane + k * LPR) * V;
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-            wv[k * V + j] = c0 + j < C ? param<T>(w, w_f32, c0 + j, 1.0f) : 0.0f;
-            bv[k * V + j] = c0 + j < C ? param<T>(b, w_f32, c0 + j, 0.0f) : 0.0f;
-        }
-    }
-    // every lane of a workgroup runs the same number of rounds: the sums above one wavefront hold barriers
-    for (long r0 = (long)blockIdx.x * RPB; r0 < rows; r0 += (long)gridDim.x * RPB) {
-        const long r = r0 + sub;
-        const bool live = r < rows;
-        const T* xr = x + (live ? r : r0) * x_stride;
-        Vec<T, V> xv[NV];
+// LPR lanes per row, E values each (vectors of 16 bytes, lane after lane); a workgroup takes rows
+// blockIdx.x * (BLOCK / LPR) + k * gridDim.x * ..., its lanes keep their columns' weights.  The next row is loaded before
+// the sums of the current one are formed, which would leave the memory idle otherwise (not with 1024 lanes per row: they
+// have 128 registers each).
+template <typename T, int LPR, int E>
+struct Row {
+    static constexpr int V = 16 / sizeof(T), NV = E / V;
+    Vec<T, V> v[NV];
+
+    __device__ __forceinline__ void load(const T* row, int lane, int C) {
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
             const int c0 = (lane + k * LPR) * V;
-            xv[k] = ldv_n<T, V>(xr + (c0 < C ? c0 : 0), C - c0);
+            v[k] = ldv_n<T, V>(row + (c0 < C ? c0 : 0), C - c0);
         }
+    }
+};
+
+// The weights or biases of a lane's columns, in whole vectors
+template <typename T, int LPR, int E>
+__device__ __forceinline__ void row_params(const void* p, bool f32, int lane, int C, float absent, float (&to)[E]) {
+    constexpr int V = Row<T, LPR, E>::V, NV = E / V;
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+        const int c0 = (lane + k * LPR) * V, at = c0 < C ? c0 : 0;
+        if (!p) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) to[k * V + j] = absent;
+        } else if (f32) {
+#pragma unroll
+            for (int h = 0; h < V; h += 4) {
+                const Vec<float, 4> v = ldv_n<float, 4>(static_cast<const float*>(p) + at + (c0 + h < C ? h : 0), C - c0 - h);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) to[k * V + h + j] = v.e[j];
+            }
+        } else {
+            const Vec<T, V> v = ldv_n<T, V>(static_cast<const T*>(p) + at, C - c0);
+#pragma unroll
+            for (int j = 0; j < V; ++j) to[k * V + j] = (float)v.e[j];
+        }
+    }
+}
+
+template <typename T, int LPR, int BLOCK, int E>
+__global__ __launch_bounds__(BLOCK) void ln_rows_fwd(const T* __restrict__ x, const void* __restrict__ w,
+                                                     const void* __restrict__ b, bool w_f32, long rows, int C,
+                                                     long x_stride, float eps, int relu, T* __restrict__ y,
+                                                     float* __restrict__ mean, float* __restrict__ rstd) {
+    constexpr int V = Row<T, LPR, E>::V, NV = E / V, RPB = BLOCK / LPR;
+    __shared__ float red[LPR > 64 ? 2 * (BLOCK / 64) : 1];
+    const int lane = threadIdx.x % LPR, sub = threadIdx.x / LPR;
+    const float fc = (float)C;
+    const long stride = (long)gridDim.x * RPB;
+    long r = (long)blockIdx.x * RPB + sub;
+    constexpr bool AHEAD = LPR < 1024;
+    Row<T, LPR, E> xv, ahead;
+    if constexpr (AHEAD) xv.load(x + (r < rows ? r : 0) * x_stride, lane, C);
+    float wv[E], bv[E];
+    row_params<T, LPR, E>(w, w_f32, lane, C, 1.0f, wv);
+    row_params<T, LPR, E>(b, w_f32, lane, C, 0.0f, bv);
+    // every lane of a workgroup runs the same number of rounds: the sums above one wavefront hold barriers
+    for (long r0 = (long)blockIdx.x * RPB; r0 < rows; r0 += stride, r += stride) {
+        if constexpr (!AHEAD) xv.load(x + (r < rows ? r : 0) * x_stride, lane, C);
+        else if (r0 + stride < rows) ahead.load(x + (r + stride < rows ? r + stride : 0) * x_stride, lane, C);
         float s = 0.0f;
 #pragma unroll
         for (int k = 0; k < NV; ++k)
 #pragma unroll
-            for (int j = 0; j < V; ++j) s += (float)xv[k].e[j];
-        const float mu = group_sum<LPR>(s, red, 0) / fc;
+            for (int j = 0; j < V; ++j) s += (float)xv.v[k].e[j];
+        const float mu = group_sum<LPR, BLOCK>(s, red, 0) / fc;
         s = 0.0f;
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
             const int n = C - (lane + k * LPR) * V;
 #pragma unroll
             for (int j = 0; j < V; ++j) {
-                const float d = j < n ? (float)xv[k].e[j] - mu : 0.0f;
+                const float d = j < n ? (float)xv.v[k].e[j] - mu : 0.0f;
                 s = fmaf(d, d, s);
             }
         }
-        const float rs = 1.0f / sqrtf(group_sum<LPR>(s, red, 1) / fc + eps);
-        if (live) {
+        const float rs = 1.0f / sqrtf(group_sum<LPR, BLOCK>(s, red, 1) / fc + eps);
+        if (r < rows) {
             T* yr = y + r * C;
 #pragma unroll
             for (int k = 0; k < NV; ++k) {
@@ -177,7 +216,7 @@ __global__ __launch_bounds__(BLOCK) void ln_rows_fwd(const T* __restrict__ x, co
                     Vec<T, V> o;
 #pragma unroll
                     for (int j = 0; j < V; ++j) {
-                        float v = fmaf(((float)xv[k].e[j] - mu) * rs, wv[k * V + j], bv[k * V + j]);
+                        float v = fmaf(((float)xv.v[k].e[j] - mu) * rs, wv[k * V + j], bv[k * V + j]);
                         if (relu) v = passes(v) ? v : 0.0f;
                         o.e[j] = (T)v;
                     }
@@ -189,62 +228,63 @@ __global__ __launch_bounds__(BLOCK) void ln_rows_fwd(const T* __restrict__ x, co
                 rstd[r] = rs;
             }
         }
+        if constexpr (AHEAD) xv = ahead;
     }
 }
 
 // partial: [gridDim.x][2][C] sums of g h and of g over the workgroup's rows, or NULL when no parameter asks for them
-template <typename T, int LPR, int BLOCK>
+template <typename T, int LPR, int BLOCK, int E>
 __global__ __launch_bounds__(BLOCK) void ln_rows_bwd(const T* __restrict__ dy, const T* __restrict__ x,
                                                      const void* __restrict__ w, const void* __restrict__ b, bool w_f32,
                                                      const float* __restrict__ mean, const float* __restrict__ rstd,
                                                      long rows, int C, long dy_stride, long x_stride, int relu,
                                                      T* __restrict__ dx, float* __restrict__ partial) {
-    constexpr int V = kVec, NV = kRowElems / V, E = kRowElems;
-    constexpr int RPB = BLOCK / LPR;
-    __shared__ float red[LPR > 64 ? 4 * (LPR / 64) : 1];
+    constexpr int V = Row<T, LPR, E>::V, NV = E / V, RPB = BLOCK / LPR;
+    __shared__ float red[LPR > 64 ? 4 * (BLOCK / 64) : 1];
     __shared__ float cols[RPB > 1 ? BLOCK * E : 1];
     const int lane = threadIdx.x % LPR, sub = threadIdx.x / LPR;
     const float fc = (float)C;
-    float wv[E], bv[E], aw[E], ab[E];
+    const long stride = (long)gridDim.x * RPB;
+    long r = (long)blockIdx.x * RPB + sub;
+    constexpr bool AHEAD = LPR < 1024;
+    Row<T, LPR, E> xv, gv, next_x, next_g;
+    float mu = 0.0f, rs = 0.0f;
+    const auto load = [&](long r, Row<T, LPR, E>& xr, Row<T, LPR, E>& gr, float& m, float& s) {
+        r = r < rows ? r : 0;
+        xr.load(x + r * x_stride, lane, C);
+        gr.load(dy + r * dy_stride, lane, C);
+        m = mean[r];
+        s = rstd[r];
+    };
+    if constexpr (AHEAD) load(r, xv, gv, mu, rs);
+    float wv[E], aw[E], ab[E];
+    row_params<T, LPR, E>(w, w_f32, lane, C, 1.0f, wv);
 #pragma unroll
-    for (int k = 0; k < NV; ++k) {
-        const int c0 = (lane + k * LPR) * V;
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-            wv[k * V + j] = c0 + j < C ? param<T>(w, w_f32, c0 + j, 1.0f) : 0.0f;
-            bv[k * V + j] = c0 + j < C ? param<T>(b, w_f32, c0 + j, 0.0f) : 0.0f;
-            aw[k * V + j] = 0.0f;
-            ab[k * V + j] = 0.0f;
-        }
+    for (int i = 0; i < E; ++i) {
+        aw[i] = 0.0f;
+        ab[i] = 0.0f;
     }
     int turn = 0;
-    for (long r0 = (long)blockIdx.x * RPB; r0 < rows; r0 += (long)gridDim.x * RPB, turn ^= 1) {
-        const long r = r0 + sub;
+    for (long r0 = (long)blockIdx.x * RPB; r0 < rows; r0 += stride, r += stride, turn ^= 1) {
         const bool live = r < rows;
-        const T* xr = x + (live ? r : r0) * x_stride;
-        const T* gr = dy + (live ? r : r0) * dy_stride;
-        Vec<T, V> xv[NV], gv[NV];
-#pragma unroll
-        for (int k = 0; k < NV; ++k) {
-            const int c0 = (lane + k * LPR) * V;
-            xv[k] = ldv_n<T, V>(xr + (c0 < C ? c0 : 0), C - c0);
-            gv[k] = ldv_n<T, V>(gr + (c0 < C ? c0 : 0), live ? C - c0 : 0);
-        }
-        const float mu = mean[live ? r : r0], rs = rstd[live ? r : r0];
+        float next_mu = 0.0f, next_rs = 0.0f;
+        if constexpr (!AHEAD) load(r, xv, gv, mu, rs);
+        else if (r0 + stride < rows) load(r + stride, next_x, next_g, next_mu, next_rs);
         float s1 = 0.0f, s2 = 0.0f;
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
-            const int n = C - (lane + k * LPR) * V;
+            const int n = live ? C - (lane + k * LPR) * V : 0;
 #pragma unroll
             for (int j = 0; j < V; ++j) {
                 const int i = k * V + j;
-                const float h = ((float)xv[k].e[j] - mu) * rs;
-                float g = (float)gv[k].e[j];
-                if (relu) {
-                    g = passes(fmaf(h, wv[i], bv[i])) ? g : 0.0f;
-                    gv[k].e[j] = (T)g;
+                const float h = ((float)xv.v[k].e[j] - mu) * rs;
+                float g = (float)gv.v[k].e[j];
+                if (relu) {                                   // (the biases are read again: they would cost a register each)
+                    const int c = (lane + k * LPR) * V + j;
+                    g = passes(fmaf(h, wv[i], c < C ? param<T>(b, w_f32, c, 0.0f) : 0.0f)) ? g : 0.0f;
+                    gv.v[k].e[j] = (T)g;
                 }
-                if (j < n && live) {
+                if (j < n) {
                     const float gw = g * wv[i];
                     s1 += gw;
                     s2 = fmaf(gw, h, s2);
@@ -253,8 +293,8 @@ __global__ __launch_bounds__(BLOCK) void ln_rows_bwd(const T* __restrict__ dy, c
                 }
             }
         }
-        const float m1 = group_sum<LPR>(s1, red, 2 * turn) / fc;
-        const float m2 = group_sum<LPR>(s2, red, 2 * turn + 1) / fc;
+        const float m1 = group_sum<LPR, BLOCK>(s1, red, 2 * turn) / fc;
+        const float m2 = group_sum<LPR, BLOCK>(s2, red, 2 * turn + 1) / fc;
         if (live && dx) {
             T* dr = dx + r * C;
 #pragma unroll
@@ -264,12 +304,18 @@ __global__ __launch_bounds__(BLOCK) void ln_rows_bwd(const T* __restrict__ dy, c
                     Vec<T, V> o;
 #pragma unroll
                     for (int j = 0; j < V; ++j) {
-                        const float h = ((float)xv[k].e[j] - mu) * rs;
-                        o.e[j] = (T)(rs * (fmaf((float)gv[k].e[j], wv[k * V + j], -m1) - h * m2));
+                        const float h = ((float)xv.v[k].e[j] - mu) * rs;
+                        o.e[j] = (T)(rs * (fmaf((float)gv.v[k].e[j], wv[k * V + j], -m1) - h * m2));
                     }
                     stv_n<T, V>(dr + c0, o, C - c0);
                 }
             }
+        }
+        if constexpr (AHEAD) {
+            xv = next_x;
+            gv = next_g;
+            mu = next_mu;
+            rs = next_rs;
         }
     }
     if (!partial) return;
@@ -420,12 +466,11 @@ __global__ __launch_bounds__(CL* PL) void ln_planes_bwd(const T* __restrict__ dy
     __shared__ float wave_part[PL > 64 ? CL * (PL / 64) * E : 1];
     const int pl = threadIdx.x % PL, cg = threadIdx.x / PL;
     const float fc = (float)C;
-    float wv[E], bv[E], aw[E], ab[E];
+    float wv[E], aw[E], ab[E];
 #pragma unroll
     for (int k = 0; k < E; ++k) {
         const int c = cg + k * CL;
         wv[k] = c < C ? param<T>(w, w_f32, c, 1.0f) : 0.0f;
-        bv[k] = c < C ? param<T>(b, w_f32, c, 0.0f) : 0.0f;
         aw[k] = 0.0f;
         ab[k] = 0.0f;
     }
@@ -456,12 +501,13 @@ __global__ __launch_bounds__(CL* PL) void ln_planes_bwd(const T* __restrict__ dy
 #pragma unroll
         for (int k = 0; k < E; ++k) {
             const bool on = cg + k * CL < C;
+            const float bias = relu && on ? param<T>(b, w_f32, cg + k * CL, 0.0f) : 0.0f;
 #pragma unroll
             for (int v = 0; v < V; ++v) {
                 const float h = ((float)xv[k].e[v] - mu[v]) * rs[v];
                 float g = (float)gv[k].e[v];
                 if (relu) {
-                    g = passes(fmaf(h, wv[k], bv[k])) ? g : 0.0f;
+                    g = passes(fmaf(h, wv[k], bias)) ? g : 0.0f;
                     gv[k].e[v] = (T)g;
                 }
                 if (on && v < n) {
@@ -675,8 +721,10 @@ __global__ __launch_bounds__(1024) void ln_params_sum(const float* __restrict__ 
     const int col = threadIdx.x & 31, part = threadIdx.x >> 5;
     const long at = (long)blockIdx.x * 32 + col;                  // over [2][C]
     float s = 0.0f;
-    if (at < 2 * C)
+    if (at < 2 * C) {
+#pragma unroll 8
         for (int i = part; i < n; i += 32) s += partial[(long)i * 2 * C + at];
+    }
     red[part][col] = s;
     __syncthreads();
     if (part == 0 && at < 2 * C) {
@@ -692,12 +740,12 @@ __global__ __launch_bounds__(1024) void ln_params_sum(const float* __restrict__ 
 }
 
 // ---- which kernel, how many workgroups ----------------------------------------------------------------------
-constexpr int kRowsMax = kRowElems * 1024;        // rows: the widest that 1024 lanes hold
+constexpr int kRowsMax = 16 * 1024;               // rows: the widest that 1024 lanes of 16 values hold
 constexpr int kPlanesMax = 1024;                  // planes: 128 channel groups of 8
 
-// Workgroups of a launch that loops over its positions: four per compute unit.  A backward launch leaves one row
-// of partial sums per workgroup, which the second launch reads: no more of them than that pays for.
-constexpr long kGroups = 1024;
+// Workgroups of a launch that loops over its positions.  A backward launch leaves one row of partial sums per
+// workgroup, which the second launch reads: no more of them than the compute units hold at a time.
+constexpr long kRowsFwd = 1280, kRowsBwd = 768, kPlanesFwd = 1024, kPlanesBwd = 512, kLong = 4096;
 
 struct Plan {
     bool rows, wide;      // wide: vectors along the positions (planes)
@@ -714,7 +762,7 @@ Plan plan_of(int64_t outer, int64_t C, int64_t inner) {
     p.rows = inner == 1;
     if (p.rows) {
         p.fits = C <= kRowsMax;
-        p.lpr = C <= 8 * kRowElems ? 8 : C <= 32 * kRowElems ? 32 : C <= 64 * kRowElems ? 64 : C <= 256 * kRowElems ? 256 : 1024;
+        p.lpr = C <= 128 ? 8 : C <= 512 ? 32 : C <= 1024 ? 64 : C <= 2048 ? 128 : C <= 4096 ? 256 : 1024;
         const int rpb = p.lpr < 256 ? 256 / p.lpr : 1;
         p.units = p.fits ? (outer + rpb - 1) / rpb : outer;
     } else {
@@ -723,20 +771,20 @@ Plan plan_of(int64_t outer, int64_t C, int64_t inner) {
         // would idle a quarter of the lanes
         const int64_t nv = (inner + kVec - 1) / kVec;
         p.wide = inner * 4 >= nv * kVec * 3;
-        p.cl = C <= 8 ? 1 : C <= 32 ? 4 : C <= 128 ? 16 : C <= 512 ? 64 : 128;
-        p.pl = p.cl <= 16 ? 256 / p.cl : p.cl == 64 ? 8 : 4;
+        p.cl = C <= 8 ? 1 : C <= 32 ? 4 : C <= 64 ? 8 : C <= 128 ? 16 : C <= 256 ? 32 : C <= 512 ? 64 : 128;
+        p.pl = p.cl <= 32 ? 256 / p.cl : p.cl == 64 ? 8 : 4;
         const int64_t nq = p.wide ? outer * nv : outer * inner;
         p.units = p.fits ? (nq + p.pl - 1) / p.pl : (outer * inner + kLongPos - 1) / kLongPos;
     }
     return p;
 }
 
-unsigned groups_of(const Plan& p) {
-    const long most = p.fits ? kGroups : 4096;
+unsigned groups_of(const Plan& p, bool fwd) {
+    const long most = !p.fits ? kLong : p.rows ? (fwd ? kRowsFwd : kRowsBwd) : fwd ? kPlanesFwd : kPlanesBwd;
     return (unsigned)(p.units < most ? p.units : most);
 }
 constexpr int kLongShares = 64;
-int64_t partials_of(const Plan& p) { return p.fits ? (int64_t)groups_of(p) : kLongShares; }
+int64_t partials_of(const Plan& p) { return p.fits ? (int64_t)groups_of(p, false) : kLongShares; }
 
 int check_sizes(int x_type, int w_type, int64_t outer, int64_t C, int64_t inner) {
     if (x_type < FC3D_F32 || x_type > FC3D_F16) return FC3D_EINVAL;
@@ -770,15 +818,15 @@ struct BwdArgs {
     float* partial;       // NULL: no parameter asks for a gradient
 };
 
-template <typename T, int LPR, int BLOCK>
+template <typename T, int LPR, int BLOCK, int E>
 int rows_launch(const FwdArgs& a, unsigned groups) {
-    FC3D_LAUNCH("layer_norm_fwd", (ln_rows_fwd<T, LPR, BLOCK>), dim3(groups), dim3(BLOCK), 0, a.s, (const T*)a.x, a.w, a.b,
+    FC3D_LAUNCH("layer_norm_fwd", (ln_rows_fwd<T, LPR, BLOCK, E>), dim3(groups), dim3(BLOCK), 0, a.s, (const T*)a.x, a.w, a.b,
                 a.w_f32, (long)a.outer, (int)a.C, (long)a.x_stride, a.eps, a.relu, (T*)a.y, a.mean, a.rstd);
     return FC3D_OK;
 }
-template <typename T, int LPR, int BLOCK>
+template <typename T, int LPR, int BLOCK, int E>
 int rows_launch(const BwdArgs& a, unsigned groups) {
-    FC3D_LAUNCH("layer_norm_bwd", (ln_rows_bwd<T, LPR, BLOCK>), dim3(groups), dim3(BLOCK), 0, a.s, (const T*)a.dy,
+    FC3D_LAUNCH("layer_norm_bwd", (ln_rows_bwd<T, LPR, BLOCK, E>), dim3(groups), dim3(BLOCK), 0, a.s, (const T*)a.dy,
                 (const T*)a.x, a.w, a.b, a.w_f32, a.mean, a.rstd, (long)a.outer, (int)a.C, (long)a.dy_stride,
                 (long)a.x_stride, a.relu, (T*)a.dx, a.partial);
     return FC3D_OK;
@@ -803,7 +851,9 @@ int planes_of(const A& a, const Plan& p, unsigned groups) {
     switch (p.cl) {
         case 1: return planes_launch<T, V, 1, 256>(a, groups);
         case 4: return planes_launch<T, V, 4, 64>(a, groups);
+        case 8: return planes_launch<T, V, 8, 32>(a, groups);
         case 16: return planes_launch<T, V, 16, 16>(a, groups);
+        case 32: return planes_launch<T, V, 32, 8>(a, groups);
         case 64: return planes_launch<T, V, 64, 8>(a, groups);
         default: return planes_launch<T, V, 128, 4>(a, groups);
     }
@@ -811,20 +861,21 @@ int planes_of(const A& a, const Plan& p, unsigned groups) {
 // The register kernel of a plan, forward or backward by the arguments' type
 template <typename T, typename A>
 int registers_of(const A& a, const Plan& p) {
-    const unsigned groups = groups_of(p);
+    const unsigned groups = groups_of(p, std::is_same<A, FwdArgs>::value);
     if (!p.rows) return p.wide ? planes_of<T, kVec>(a, p, groups) : planes_of<T, 1>(a, p, groups);
     switch (p.lpr) {
-        case 8: return rows_launch<T, 8, 256>(a, groups);
-        case 32: return rows_launch<T, 32, 256>(a, groups);
-        case 64: return rows_launch<T, 64, 256>(a, groups);
-        case 256: return rows_launch<T, 256, 256>(a, groups);
-        default: return rows_launch<T, 1024, 1024>(a, groups);
+        case 8: return rows_launch<T, 8, 256, 16>(a, groups);
+        case 32: return rows_launch<T, 32, 256, 16>(a, groups);
+        case 64: return rows_launch<T, 64, 256, 16>(a, groups);
+        case 128: return rows_launch<T, 128, 256, 16>(a, groups);
+        case 256: return rows_launch<T, 256, 256, 16>(a, groups);
+        default: return rows_launch<T, 1024, 1024, 16>(a, groups);
     }
 }
 
 template <typename T, bool PLANES>
 int long_of(const FwdArgs& a, const Plan& p) {
-    FC3D_LAUNCH("layer_norm_fwd", (ln_long_fwd<T, PLANES>), dim3(groups_of(p)), dim3(kLongBlock), 0, a.s, (const T*)a.x, a.w,
+    FC3D_LAUNCH("layer_norm_fwd", (ln_long_fwd<T, PLANES>), dim3(groups_of(p, true)), dim3(kLongBlock), 0, a.s, (const T*)a.x, a.w,
                 a.b, a.w_f32, (long)(a.outer * a.inner), (long)a.C, (long)a.inner, (long)a.x_stride, a.eps, a.relu, (T*)a.y,
                 a.mean, a.rstd);
     return FC3D_OK;
@@ -834,7 +885,7 @@ int long_of(const BwdArgs& a, const Plan& p) {
     const T *dy = (const T*)a.dy, *x = (const T*)a.x;
     const long positions = (long)(a.outer * a.inner);
     if (a.dx)
-        FC3D_LAUNCH("layer_norm_bwd", (ln_long_bwd<T, PLANES>), dim3(groups_of(p)), dim3(kLongBlock), 0, a.s, dy, x, a.w, a.b,
+        FC3D_LAUNCH("layer_norm_bwd", (ln_long_bwd<T, PLANES>), dim3(groups_of(p, false)), dim3(kLongBlock), 0, a.s, dy, x, a.w, a.b,
                     a.w_f32, a.mean, a.rstd, positions, (long)a.C, (long)a.inner, (long)a.dy_stride, (long)a.x_stride,
                     a.relu, (T*)a.dx);
     if (a.partial)

@@ -126,7 +126,8 @@ def test_refusals():
     assert bwd(dx=None) == 0
     assert lib.fc3d_layer_norm_bwd_workspace(0, 0, 8, 1) == 0 and lib.fc3d_layer_norm_bwd_workspace(0, 5, 0, 1) == 0
     assert lib.fc3d_layer_norm_bwd_workspace(0, 5, 4096, 1) == 5 * 2 * 4096 * 4         # a row per workgroup
-    assert lib.fc3d_layer_norm_bwd_workspace(0, 1 << 20, 64, 1) == 1024 * 2 * 64 * 4
+    n = lib.fc3d_layer_norm_bwd_workspace(0, 1 << 20, 64, 1)                            # bounded, however many rows
+    assert n % (2 * 64 * 4) == 0 and 256 <= n // (2 * 64 * 4) <= 2048
 
 
 def test_strides_of_merged_axes():
