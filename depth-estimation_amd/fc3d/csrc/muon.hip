@@ -18,9 +18,9 @@
 // directions whose share of A is below its rounding, amplified a^(2L)-fold: five steps at once cost 1e-4 of the
 // result in bad cases (measured in emulation, low rank plus noise), which is below the rounding of a 16-bit result;
 // for fp32 results the segments are of two and three steps, or of one for matrices that are nearly square
-// (n < 2 m, where the smallest singular values sit near zero) and for those of one tile (where the squares saved are
-// cheap), as accurate as step by step.  Against 64 bits: 512 x 4608 1.2e-6 of the result (fp32 matrix products
-// 4.2e-6), 256 x 256 6e-7 (1.8e-6), 64 x 288 1.4e-6 (1.4e-6).
+// (n < 2 m, where the smallest singular values sit near zero) and for those of up to 64 rows (where the squares saved
+// are cheap), as accurate as step by step.  Against 64 bits: 512 x 4608 1.2e-6 of the result (fp32 matrix products
+// 4.2e-6), 256 x 256 6e-7 (1.8e-6); 64 x 288 2.5e-8 (1.5e-6), worked on in 64 bits.
 #include "fc3d_common.h"
 
 #include <cmath>
@@ -71,36 +71,34 @@ struct Table {
     Matrix e[kMaxItems];
 };
 
-__device__ __forceinline__ float ld_any(const void* p, int type, size_t i) {
-    if (type == FC3D_F32) return static_cast<const float*>(p)[i];
-    if (type == FC3D_BF16) return (float)static_cast<const __bf16*>(p)[i];
-    return (float)static_cast<const _Float16*>(p)[i];
+// Element types are template arguments or dispatched outside the loops: a branch around every load would make each
+// wait for the one before.
+template <typename T>
+__device__ __forceinline__ float ld(const void* p, size_t i) {
+    return (float)static_cast<const T*>(p)[i];
+}
+template <typename F>
+__device__ __forceinline__ void with_type(int type, F&& f) {
+    if (type == FC3D_F32) f(float{});
+    else if (type == FC3D_BF16) f(__bf16{});
+    else f(_Float16{});
 }
 // four values, at the element's own alignment
 typedef float float4a __attribute__((ext_vector_type(4), aligned(4)));
 typedef uint32_t word2a __attribute__((ext_vector_type(2), aligned(2)));
-__device__ __forceinline__ void ld4_any(const void* p, int type, size_t i, float (&v)[4]) {
-    if (type == FC3D_F32) {
+template <typename T>
+__device__ __forceinline__ void ld4(const void* p, size_t i, float (&v)[4]) {
+    if constexpr (sizeof(T) == 4) {
         const float4a w = *reinterpret_cast<const float4a*>(static_cast<const float*>(p) + i);
 #pragma unroll
         for (int j = 0; j < 4; ++j) v[j] = w[j];
-        return;
-    }
-    const word2a w = *reinterpret_cast<const word2a*>(static_cast<const uint16_t*>(p) + i);
-    if (type == FC3D_BF16) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = __uint_as_float(j & 1 ? w[j >> 1] & 0xffff0000u : w[j >> 1] << 16);
     } else {
-        _Float16 h[4];
+        const word2a w = *reinterpret_cast<const word2a*>(static_cast<const T*>(p) + i);
+        T h[4];
         __builtin_memcpy(h, &w, 8);
 #pragma unroll
         for (int j = 0; j < 4; ++j) v[j] = (float)h[j];
     }
-}
-__device__ __forceinline__ void st_any(void* p, int type, size_t i, float v) {
-    if (type == FC3D_F32) static_cast<float*>(p)[i] = v;
-    else if (type == FC3D_BF16) static_cast<__bf16*>(p)[i] = (__bf16)v;
-    else static_cast<_Float16*>(p)[i] = (_Float16)v;
 }
 
 // Which matrix this workgroup works on: lane l counts the workgroups of matrix l, a scan over the wavefront numbers
@@ -131,7 +129,8 @@ __device__ __forceinline__ int parts_of(const Matrix& e) { return (int)(((size_t
 // Sums of squares of the update per workgroup (64 bits: any fp32 input stays in range), and the momentum's update.
 // The first workgroup leaves the table in device memory for the launches that follow: kernel arguments may lie in host
 // memory, where a search through them costs microseconds.
-__global__ __launch_bounds__(256) void ns_norm_kernel(Table t, int type, Blend k, double* __restrict__ parts,
+template <typename T>
+__global__ __launch_bounds__(256) void ns_norm_kernel(Table t, Blend k, double* __restrict__ parts,
                                                       Matrix* __restrict__ table) {
     __shared__ double red[4];
     const int lane = threadIdx.x & 63;
@@ -148,7 +147,7 @@ __global__ __launch_bounds__(256) void ns_norm_kernel(Table t, int type, Blend k
     const size_t hi = lo + kChunk < count ? lo + kChunk : count;
     double s = 0.0;
     const auto one = [&](size_t j) {
-        float u = ld_any(e.g, type, j);
+        float u = ld<T>(e.g, j);
         if (e.mom) {
             const float mn = fmaf(k.beta, e.mom[j], k.rest * u);
             e.mom[j] = mn;
@@ -160,10 +159,10 @@ __global__ __launch_bounds__(256) void ns_norm_kernel(Table t, int type, Blend k
 #pragma unroll 4
     for (size_t j = lo + 4 * threadIdx.x; j < whole; j += 1024) {
         float u[4];
-        ld4_any(e.g, type, j, u);
+        ld4<T>(e.g, j, u);
         if (e.mom) {
             float m[4];
-            ld4_any(e.mom, FC3D_F32, j, m);
+            ld4<float>(e.mom, j, m);
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
                 m[q] = fmaf(k.beta, m[q], k.rest * u[q]);
@@ -198,7 +197,8 @@ __device__ __forceinline__ void split8(_Float16* p, size_t plane, const float (&
 // X and its transpose, scaled by sx / (norm + eps), zero beyond the matrix, one 64 x 64 tile per workgroup.
 // `exact` (16-bit input taken as it is): one plane that holds the input times a power of two, without rounding; the
 // remaining factor in [1, 2) goes to rho and into the products that read X.
-__global__ __launch_bounds__(256) void ns_prepare_kernel(const Matrix* __restrict__ t, int matrices, int type, Blend k,
+template <typename T>
+__global__ __launch_bounds__(256) void ns_prepare_kernel(const Matrix* __restrict__ t, int matrices, Blend k,
                                                          const double* __restrict__ parts, double eps, float sx, int exact,
                                                          _Float16* __restrict__ planes, float* __restrict__ rho) {
     __shared__ float tile[64][65];
@@ -207,8 +207,32 @@ __global__ __launch_bounds__(256) void ns_prepare_kernel(const Matrix* __restric
     int block = blockIdx.x;
     const int w = find_matrix(lane < matrices ? (t[lane].mp / 64) * (t[lane].np / 64) : 0, block);
     const Matrix& e = t[w];
+    const int tn = e.np / 64;
+    const int i0 = block / tn * 64, j0 = block % tn * 64;
+    const int ty = threadIdx.x >> 6;
+    float v[16];
+    {
+        size_t at[16];
+        bool in[16];
+#pragma unroll
+        for (int q = 0; q < 16; ++q) {
+            const int fast = lane, slow = q * 4 + ty;        // fast: along the tensor's rows
+            const int i = i0 + (e.tall ? fast : slow), j = j0 + (e.tall ? slow : fast);
+            in[q] = i < e.m && j < e.n;
+            at[q] = !in[q] ? 0 : e.tall ? (size_t)j * e.m + i : (size_t)i * e.n + j;
+        }
+#pragma unroll
+        for (int q = 0; q < 16; ++q) v[q] = ld<T>(e.g, at[q]);
+        if (e.mom)
+#pragma unroll
+            for (int q = 0; q < 16; ++q) v[q] = blend(k, v[q], e.mom[at[q]]);
+#pragma unroll
+        for (int q = 0; q < 16; ++q)
+            if (!in[q]) v[q] = 0.0f;
+    }
     const int count = parts_of(e);
     double s = 0.0;
+#pragma unroll 4
     for (int q = threadIdx.x; q < count; q += 256) s += parts[e.part0 + q];
 #pragma unroll
     for (int q = 32; q > 0; q >>= 1) s += __shfl_xor(s, q, 64);
@@ -225,22 +249,12 @@ __global__ __launch_bounds__(256) void ns_prepare_kernel(const Matrix* __restric
             rest = (float)factor;
         }
     }
-    const int tn = e.np / 64;
-    const int i0 = block / tn * 64, j0 = block % tn * 64;
     if (block == 0 && threadIdx.x == 0) rho[w] = rest;
-    const int ty = threadIdx.x >> 6;
 #pragma unroll
     for (int q = 0; q < 16; ++q) {
-        const int fast = lane, slow = q * 4 + ty;            // fast: along the tensor's rows
-        const int r = e.tall ? fast : slow, c = e.tall ? slow : fast;
-        float v = 0.0f;
-        if (i0 + r < e.m && j0 + c < e.n) {
-            const size_t at = e.tall ? (size_t)(j0 + c) * e.m + (i0 + r) : (size_t)(i0 + r) * e.n + (j0 + c);
-            v = ld_any(e.g, type, at);
-            if (e.mom) v = blend(k, v, e.mom[at]);
-            v = exact ? ldexpf(v, shift) : (float)((double)v * factor);
-        }
-        tile[r][c] = v;
+        const int fast = lane, slow = q * 4 + ty, r = e.tall ? fast : slow, c = e.tall ? slow : fast;
+        const bool in = i0 + r < e.m && j0 + c < e.n;
+        tile[r][c] = !in ? 0.0f : exact ? ldexpf(v[q], shift) : (float)((double)v[q] * factor);
     }
     __syncthreads();
     const size_t plane = plane_of(BUF_X, e.mp, e.np);
@@ -249,13 +263,13 @@ __global__ __launch_bounds__(256) void ns_prepare_kernel(const Matrix* __restric
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
         const int id = threadIdx.x + 256 * q, r = id >> 3, c = (id & 7) * 8;
-        float v[8];
+        float u[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = tile[r][c + j];
-        split8(x + (size_t)(i0 + r) * e.np + j0 + c, plane, v);
+        for (int j = 0; j < 8; ++j) u[j] = tile[r][c + j];
+        split8(x + (size_t)(i0 + r) * e.np + j0 + c, plane, u);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = tile[c + j][r];
-        split8(xt + (size_t)(j0 + r) * e.mp + i0 + c, plane, v);
+        for (int j = 0; j < 8; ++j) u[j] = tile[c + j][r];
+        split8(xt + (size_t)(j0 + r) * e.mp + i0 + c, plane, u);
     }
 }
 
@@ -423,8 +437,8 @@ __global__ __launch_bounds__(WAVES * 64, TILE == 64 && WAVES == 4 ? 2 : 1) void 
     const int bi = QUADS ? (quad >> 1) * 64 : 0, bj = QUADS ? (quad & 1) * 64 : 0;
     const int own = QUADS ? (wave & 1) * 2 : wave;            // this wavefront's first 16 values of a stage's depth, in 16s
     // The matrix units' sums lose up to a unit of the running sum's last place per instruction: that the wavefronts
-    // share the depth keeps the chains short (a depth of 4608: 108 instructions; one wavefront's 864 would double
-    // the error of the result).
+    // share the depth keeps the chains short (a depth of 4608: 216 instructions, fewer where workgroups share it
+    // too; one wavefront's 864 would double the error of the result).
     float16v acc[BLK][BLK] = {};
     struct Part {                                             // both operands at 16 values of the depth
         half8 f1[BLK][P1], f2[BLK][P2];
@@ -543,17 +557,21 @@ __global__ __launch_bounds__(WAVES * 64, TILE == 64 && WAVES == 4 ? 2 : 1) void 
     if (o.use_rho) alpha *= o.kind == GRAM ? a.rho[w] * a.rho[w] : a.rho[w];
     const int i0 = ti * TILE, j0 = tj * TILE;
     if (o.kind == APPLY && o.last) {
+        with_type(a.out_type, [&](auto zero) {
+            typedef decltype(zero) T;
+            T* to = static_cast<T*>(e.out);
 #pragma unroll 4
-        for (int id = tid; id < TILE * TILE; id += THREADS) {
-            const int fast = id % TILE, slow = id / TILE;     // fast: along the tensor's rows
-            const int r = e.tall ? fast : slow, c = e.tall ? slow : fast;
-            if (i0 + r < e.m && j0 + c < e.n) {
-                const size_t at = e.tall ? (size_t)(j0 + c) * e.m + (i0 + r) : (size_t)(i0 + r) * e.n + (j0 + c);
-                float v = sum_at(r * LD + c) * alpha;
-                if (a.step) v = fmaf(a.decay, ld_any(e.out, a.out_type, at), -e.lr * v);
-                st_any(e.out, a.out_type, at, v);
+            for (int id = tid; id < TILE * TILE; id += THREADS) {
+                const int fast = id % TILE, slow = id / TILE; // fast: along the tensor's rows
+                const int r = e.tall ? fast : slow, c = e.tall ? slow : fast;
+                if (i0 + r < e.m && j0 + c < e.n) {
+                    const size_t at = e.tall ? (size_t)(j0 + c) * e.m + (i0 + r) : (size_t)(i0 + r) * e.n + (j0 + c);
+                    float v = sum_at(r * LD + c) * alpha;
+                    if (a.step) v = fmaf(a.decay, (float)to[at], -e.lr * v);
+                    to[at] = (T)v;
+                }
             }
-        }
+        });
         return;
     }
     // To the buffers, eight values of a row at a time: the tile, and its mirror image (or, of X, the transpose).  A tile
@@ -659,6 +677,269 @@ __global__ __launch_bounds__(256) void ns_gram_sum_kernel(Launch a) {
     }
 }
 
+// ---- matrices of up to 64 rows, in three launches -----------------------------------------------------------
+// A list of small matrices is bound by launches, not by products.  There the Gram form runs in 64 bits, all steps in one
+// segment (its rounding is 1e-16), one workgroup per matrix with everything in LDS.  The norm is the trace of A; X is only
+// read as the tensor holds it, by the first launch and the last.  64 x 288: 7 + 49 + 8 us, 64 us per call, against 109 us
+// for the general path's 17 launches.  The chain of 17 products on one compute unit is the rest: 768 fp64 matrix
+// instructions of 64 cycles on the busiest SIMD, 20 us, and the operands' way through LDS, which they wait for at the start
+// of each; more units per matrix would pay a launch or a wait for each other after every product.
+typedef double double4v __attribute__((ext_vector_type(4)));
+
+constexpr int kSmall = 64;            // rows
+constexpr int kSmallLd = 68;          // doubles from row to row in LDS
+constexpr int kPairs = 10;            // 16 x 16 tiles on and above the diagonal of 64 x 64
+constexpr int kGramValues = kPairs * 256;
+
+// lane l of the fp64 instruction: operands row l % 16, depth l / 16; results column l % 16, rows 4 r + l / 16
+__device__ __forceinline__ void pair_of(int p, int& ti, int& tj) {         // column by column
+    tj = p < 1 ? 0 : p < 3 ? 1 : p < 6 ? 2 : 3;
+    ti = p - tj * (tj + 1) / 2;
+}
+
+// N values of the update, at rows i(q) and columns j(q) of X (0 beyond it); `store`: the momentum moves on, which each
+// value does once.
+template <typename T, int N, typename I, typename J>
+__device__ __forceinline__ void small_values(const Matrix& e, const Blend& k, bool store, I&& row, J&& col, double (&x)[N]) {
+    float g[N], m[N];
+    size_t at[N];
+    bool in[N];
+#pragma unroll
+    for (int q = 0; q < N; ++q) {
+        const int i = row(q), j = col(q);
+        in[q] = i < e.m && j < e.n;
+        at[q] = !in[q] ? 0 : e.tall ? (size_t)j * e.m + i : (size_t)i * e.n + j;
+    }
+#pragma unroll
+    for (int q = 0; q < N; ++q) g[q] = ld<T>(e.g, at[q]);
+    if (e.mom) {
+#pragma unroll
+        for (int q = 0; q < N; ++q) m[q] = e.mom[at[q]];
+#pragma unroll
+        for (int q = 0; q < N; ++q) {
+            if (store) {
+                m[q] = fmaf(k.beta, m[q], k.rest * g[q]);
+                if (in[q]) e.mom[at[q]] = m[q];
+            }
+            g[q] = blend(k, g[q], m[q]);
+        }
+    }
+#pragma unroll
+    for (int q = 0; q < N; ++q) x[q] = in[q] ? (double)g[q] : 0.0;
+}
+
+// Sums of the Gram matrix over a chunk of columns (Matrix::np of them) per workgroup, in the instruction's own order
+template <typename T>
+__global__ __launch_bounds__(256) void ns_small_gram_kernel(Table t, Blend k, Matrix* __restrict__ table,
+                                                            double* __restrict__ gram) {
+    __shared__ double red[3][kGramValues];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    if (blockIdx.x == 0) {
+        const int words = t.count * (int)(sizeof(Matrix) / 4);
+        const uint32_t* from = reinterpret_cast<const uint32_t*>(&t.e[0]);
+        for (int q = tid; q < words; q += 256) reinterpret_cast<uint32_t*>(table)[q] = from[q];
+    }
+    int block = blockIdx.x;
+    const int w = find_matrix(lane < t.count ? t.e[lane < t.count ? lane : 0].split : 0, block);
+    const Matrix& e = t.e[w];
+    const int tiles = (e.m + 15) / 16;
+    const int lo = block * e.np, hi = lo + e.np < e.n ? lo + e.np : e.n;
+    double4v acc[kPairs] = {};
+    // sixteen columns at a time per wavefront: a lane holds four neighbouring ones of its row, the instruction takes
+    // them in any order as long as both operands keep it
+    for (int c = lo + wave * 16; c < hi; c += 64) {
+        double x[16];                                         // [tile][column]
+        small_values<T>(e, k, true, [&](int q) { return 16 * (q >> 2) + (lane & 15); },
+                        [&](int q) { return c + 4 * (lane >> 4) + (q & 3); }, x);
+#pragma unroll
+        for (int p = 0; p < kPairs; ++p) {
+            int ti, tj;
+            pair_of(p, ti, tj);
+            if (tj >= tiles) break;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) acc[p] = __builtin_amdgcn_mfma_f64_16x16x4f64(x[ti * 4 + q], x[tj * 4 + q], acc[p], 0, 0, 0);
+        }
+    }
+    if (wave > 0)
+#pragma unroll
+        for (int p = 0; p < kPairs; ++p)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) red[wave - 1][p * 256 + r * 64 + lane] = acc[p][r];
+    __syncthreads();
+    if (wave == 0) {
+        double* to = gram + ((size_t)e.sums0 + block) * kGramValues;
+#pragma unroll
+        for (int p = 0; p < kPairs; ++p)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int at = p * 256 + r * 64 + lane;
+                to[at] = ((acc[p][r] + red[0][at]) + red[1][at]) + red[2][at];
+            }
+    }
+}
+
+// One workgroup per matrix: A / (norm + eps)^2, the steps, and P / (norm + eps) to the front of the matrix's sums. A
+// product's tiles on and above the diagonal are dealt out to 16 wavefronts, four to a SIMD: one waits for its operands or
+// writes its tile while another's instructions run.
+struct SmallLds {
+    double A[kSmall * kSmallLd], Q[kSmall * kSmallLd], R[kSmall * kSmallLd], P[kSmall * kSmallLd], trace[16];
+};
+template <int tiles>
+__device__ __forceinline__ void small_chain(const Matrix& e, double* __restrict__ sums, int steps, double a, double b, double c,
+                                            double eps, SmallLds& lds) {
+    double *A = lds.A, *Q = lds.Q, *R = lds.R, *P = lds.P, *trace = lds.trace;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    constexpr int pairs = tiles * (tiles + 1) / 2;
+    const int row = lane >> 4, col = lane & 15;               // of a tile's result: row + 4 r, col
+    // a tile on the diagonal holds its pairs twice: the upper one counts
+    const auto put = [&](double* to, int ti, int tj, const double4v& v) {
+        double* over = to + (16 * ti + row) * kSmallLd + 16 * tj + col;
+        double* under = to + (16 * tj + col) * kSmallLd + 16 * ti + row;
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+            if (ti < tj || row + 4 * r <= col) {
+                over[4 * r * kSmallLd] = v[r];
+                under[4 * r] = v[r];
+            }
+    };
+    // S1 S2 at one tile; both symmetric and commuting
+    const auto product = [&](const double* S1, const double* S2, int ti, int tj) {
+        const double *p1 = S1 + (16 * ti + col) * kSmallLd + row, *p2 = S2 + (16 * tj + col) * kSmallLd + row;
+        double x[4 * tiles], y[4 * tiles];
+#pragma unroll
+        for (int q = 0; q < 4 * tiles; ++q) {
+            x[q] = p1[4 * q];
+            y[q] = p2[4 * q];
+        }
+        double4v acc[2] = {};
+#pragma unroll
+        for (int q = 0; q < 4 * tiles; ++q) acc[q & 1] = __builtin_amdgcn_mfma_f64_16x16x4f64(x[q], y[q], acc[q & 1], 0, 0, 0);
+        return acc[0] + acc[1];
+    };
+    int ti = 0, tj = 0;                                       // this wavefront's tile, and that of its second job below
+    if (wave < pairs) pair_of(wave, ti, tj);
+    double4v v = {};
+    double tr = 0.0;
+    if (wave < pairs) {
+        const double* from = sums + wave * 256 + lane;
+#pragma unroll 4
+        for (int s = 0; s < e.split; ++s)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) v[r] += from[(size_t)s * kGramValues + r * 64];
+        if (ti == tj)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) tr += row + 4 * r == col ? v[r] : 0.0;
+    }
+#pragma unroll
+    for (int q = 32; q > 0; q >>= 1) tr += __shfl_xor(tr, q, 64);
+    if (lane == 0) trace[wave] = tr;
+    __syncthreads();
+    tr = 0.0;
+#pragma unroll
+    for (int q = 0; q < pairs; ++q) tr += trace[q];
+    const double inv = 1.0 / (sqrt(tr) + eps);
+    if (wave < pairs) put(A, ti, tj, v * inv * inv);
+    __syncthreads();
+    for (int step = 0; step < steps; ++step) {
+        const bool first = step == 0, last = step + 1 == steps;
+        if (wave < pairs) {                                   // Q = a I + b A + c A A
+            double4v q = product(A, A, ti, tj);
+            const double* from = A + (16 * ti + row) * kSmallLd + 16 * tj + col;
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                q[r] = fma(b, from[4 * r * kSmallLd], c * q[r]) +
+                       (ti == tj && row + 4 * r == col && 16 * ti + col < e.m ? a : 0.0);
+            put(Q, ti, tj, q);
+            if (first) put(P, ti, tj, q);
+        }
+        __syncthreads();
+        // R = A Q, and P Q, which is held back until all have read P: the jobs behind R's fall to the wavefronts that have none
+        double4v next[2] = {};
+        if (!last && wave < pairs) put(R, ti, tj, product(A, Q, ti, tj));
+        if (!first)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int job = wave + 16 * h - (last ? 0 : pairs);
+                if (job < 0 || job >= pairs) continue;
+                int pi, pj;
+                pair_of(job, pi, pj);
+                next[h] = product(P, Q, pi, pj);
+            }
+        __syncthreads();
+        if (!first)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int job = wave + 16 * h - (last ? 0 : pairs);
+                if (job < 0 || job >= pairs) continue;
+                int pi, pj;
+                pair_of(job, pi, pj);
+                put(P, pi, pj, next[h]);
+            }
+        if (!last && wave < pairs) put(A, ti, tj, product(R, Q, ti, tj));
+        __syncthreads();
+    }
+    for (int q = tid; q < kSmall * kSmall; q += 1024) {
+        const int i = q / kSmall, j = q % kSmall;
+        sums[q] = i < 16 * tiles && j < 16 * tiles ? P[i * kSmallLd + j] * inv : 0.0;
+    }
+}
+
+__global__ __launch_bounds__(1024) void ns_small_chain_kernel(const Matrix* __restrict__ table, double* __restrict__ gram, int steps,
+                                                              double a, double b, double c, double eps) {
+    __shared__ SmallLds lds;
+    const Matrix e = table[blockIdx.x];
+    double* sums = gram + (size_t)e.sums0 * kGramValues;
+    switch ((e.m + 15) / 16) {
+        case 1: return small_chain<1>(e, sums, steps, a, b, c, eps, lds);
+        case 2: return small_chain<2>(e, sums, steps, a, b, c, eps, lds);
+        case 3: return small_chain<3>(e, sums, steps, a, b, c, eps, lds);
+        default: return small_chain<4>(e, sums, steps, a, b, c, eps, lds);
+    }
+}
+
+// result = P X, 64 columns per workgroup, 16 per wavefront
+template <typename T>
+__global__ __launch_bounds__(256) void ns_small_apply_kernel(const Matrix* __restrict__ table, int matrices, Blend k,
+                                                             const double* __restrict__ gram, int out_type, int step, float decay) {
+    __shared__ double P[kSmall * kSmallLd];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    int block = blockIdx.x;
+    const int w = find_matrix(lane < matrices ? (table[lane].n + 63) / 64 : 0, block);
+    const Matrix& e = table[w];
+    const int tiles = (e.m + 15) / 16, col = block * 64 + wave * 16 + (lane & 15);
+    double x[16];
+    small_values<T>(e, k, false, [&](int q) { return 4 * q + (lane >> 4); }, [&](int) { return col; }, x);
+    const double* from = gram + (size_t)e.sums0 * kGramValues;
+#pragma unroll
+    for (int q = 0; q < kSmall * kSmall / 256; ++q) P[(q * 256 + tid) / kSmall * kSmallLd + tid % kSmall] = from[q * 256 + tid];
+    __syncthreads();
+    double4v acc[4] = {};
+#pragma unroll
+    for (int ti = 0; ti < 4; ++ti) {
+        if (ti >= tiles) break;
+        const int r1 = (16 * ti + (lane & 15)) * kSmallLd + (lane >> 4);
+#pragma unroll
+        for (int q = 0; q < 16; ++q)
+            if (q < 4 * tiles) acc[ti] = __builtin_amdgcn_mfma_f64_16x16x4f64(P[r1 + 4 * q], x[q], acc[ti], 0, 0, 0);
+    }
+    with_type(out_type, [&](auto zero) {
+        typedef decltype(zero) U;
+        U* to = static_cast<U*>(e.out);
+#pragma unroll
+        for (int ti = 0; ti < 4; ++ti)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int i = 16 * ti + 4 * r + (lane >> 4);
+                if (i < e.m && col < e.n) {
+                    const size_t at = e.tall ? (size_t)col * e.m + i : (size_t)i * e.n + col;
+                    float v = (float)acc[ti][r];
+                    if (step) v = fmaf(decay, (float)to[at], -e.lr * v);
+                    to[at] = (U)v;
+                }
+            }
+    });
+}
+
 // ---- the sequence of launches ---------------------------------------------------------------------------------
 struct Call {
     hipStream_t s;
@@ -675,6 +956,8 @@ struct Call {
     char* ws;
 };
 
+bool is_exact(const Call& k) { return k.g_type != FC3D_F32 && !k.mom; }     // the operands of the first products: one plane
+
 struct Shape {
     int64_t m, n, mp, np;
     int64_t parts() const { return (m * n + kChunk - 1) / kChunk; }
@@ -690,12 +973,27 @@ bool shape_of(int64_t rows, int64_t cols, Shape& s) {
 
 float pow2_below(double bound) { return (float)std::exp2(14.0 - std::ceil(std::log2(bound))); }     // bound * it <= 2^14
 
+// How many steps the Gram form takes at once.  A segment of L amplifies what it rounded gain^(2L)-fold: 16-bit results
+// bear five of the usual steps (gain 3.4), fp32 ones three; steps that amplify more go two by two and one by one.  So do
+// more than five steps of an fp32 result: near one the usual polynomial spreads neighbouring values (its slope is -1.4 at
+// 0.75), and every further step amplifies what a segment rounded.
+constexpr double kGain = 4.0;
+int segment_of(const Call& k, double gain) {                  // the longest one: the running products' scale follows from it
+    const int most = gain > kGain ? (k.out_type == FC3D_F32 ? 1 : 2) : k.out_type != FC3D_F32 ? 5 : k.steps <= 5 ? 3 : 1;
+    return k.steps < most ? k.steps : most;
+}
+// Whether small matrices take all steps at once in 64 bits: what is rounded (1e-16) stays under 1e-5 when amplified, which
+// ten of the usual steps do.
+bool small_of(const Call& k, double gain) { return 2.0 * k.steps * std::log2(gain) <= 36.0; }
+
 struct Scales {
     float x, a, r, q;                 // X, A, R = A Q, and Q with the running product
+    double gain;                      // the most that a step multiplies a singular value by
+    int segment;                      // steps of one segment
 };
 // Bounds on the spectra: singular values start in [0, 1] and stay below the polynomial's maximum over what they can be.
 // false: the coefficients let them grow past what the fp16 pairs resolve.
-bool scales_of(const Call& k, int longest, Scales& s) {
+bool scales_of(const Call& k, Scales& s) {
     double top = 1.0, all = 1.0;
     for (int i = 0; i < k.steps; ++i) {
         double next = 0.0;
@@ -714,7 +1012,9 @@ bool scales_of(const Call& k, int longest, Scales& s) {
         if (v > q) q = v;
         if (v * x > r) r = v * x;
     }
-    const double p = std::pow(q > 1.0 ? q : 1.0, longest);
+    s.gain = q > 1.0 ? q : 1.0;
+    s.segment = segment_of(k, s.gain);
+    const double p = std::pow(s.gain, s.segment);
     if (!(p <= 65536.0)) return false;
     s.x = pow2_below(all * 1.05);
     s.a = pow2_below(lam);
@@ -723,15 +1023,13 @@ bool scales_of(const Call& k, int longest, Scales& s) {
     return true;
 }
 
-// The steps of a plan in segments of the Gram form: plan 0 (16-bit results) five at once, (fp32) one by one; plan 1
-// two, then three.  More than five steps of an fp32 result go one by one: near one the usual polynomial spreads
-// neighbouring values (its slope is -1.4 at 0.75), so that every further step amplifies what a segment rounded.
-int plan_of(int out_type, int steps, const Shape& s) {
-    return out_type == FC3D_F32 && s.n >= 2 * s.m && s.m > 64 && steps <= 5;
+// Plan 0 goes through segments of `segment` steps, plan 1 (fp32, large matrices) through one of two steps and one of
+// three.
+int plan_of(const Call& k, double gain, const Shape& s) {
+    return k.out_type == FC3D_F32 && gain <= kGain && s.n >= 2 * s.m && s.m > 64 && k.steps <= 5;
 }
-bool starts(int out_type, int plan, int step) {
-    if (out_type != FC3D_F32) return step % 5 == 0;
-    return plan == 0 || step == 0 || step == 2;
+bool starts(int segment, int plan, int step) {
+    return plan == 0 ? step % segment == 0 : step == 0 || step == 2;
 }
 
 constexpr int kMaxOps = 5 * 64;
@@ -749,8 +1047,9 @@ void ops_of(const Call& k, int plan, const Scales& s, bool exact, PlanOps& to) {
     };
     const Op none = {};
     bool first_segment = true;
+    const int segment = k.out_type == FC3D_F32 ? 1 : s.segment;     // plan 0 of an fp32 result: one by one
     for (int step = 0; step < k.steps; ++step) {
-        const bool begin = starts(k.out_type, plan, step), end = step + 1 == k.steps || starts(k.out_type, plan, step + 1);
+        const bool begin = starts(segment, plan, step), end = step + 1 == k.steps || starts(segment, plan, step + 1);
         const uint8_t rho = exact && first_segment;
         if (begin) put(Op{GRAM, BUF_X, BUF_X, BUF_A, s.a / (s.x * s.x), rho, 0}, none);
         const uint8_t q = begin ? BUF_P0 : BUF_Q;              // the first of a segment is its running product too
@@ -784,6 +1083,7 @@ struct Layout {
     int split[kMaxItems];
     int64_t head() const { return (parts * 8 + kMaxItems * (4 + (int64_t)sizeof(Matrix)) + 255) / 256 * 256; }
     int64_t sums_at() const { return head() + (halves * 2 + 255) / 256 * 256; }
+    bool small;                       // all of up to kSmall rows: sum_tiles is the number of partial Gram matrices
     int64_t bytes() const;
 };
 
@@ -801,6 +1101,7 @@ constexpr Kernel kKernels[] = {
     {64, 4, 2, 7.0, {0.75, 0.60, 0.42}}, {96, 4, 1, 8.0, {1.03, 0.95, 0.52}}, {128, 8, 1, 6.5, {1.75, 1.10, 0.75}}};
 constexpr int kKernelCount = sizeof(kKernels) / sizeof(kKernels[0]);
 constexpr int kUnits = 256;           // compute units
+constexpr int kChunks = 128;          // small matrices: workgroups that share the columns of one, at most
 
 // The kernel with the least expected time.  The last round, when not full, costs less: nothing shares its units.
 int kernel_for(const int64_t (&groups)[kKernelCount], int64_t slices, int planes) {
@@ -820,10 +1121,12 @@ int kernel_for(const int64_t (&groups)[kKernelCount], int64_t slices, int planes
 }
 
 int64_t Layout::bytes() const {
+    if (small) return head() + sum_tiles * kGramValues * 8;
     return sums_at() + sum_tiles * kKernels[gram].tile * kKernels[gram].tile * 4;
 }
 
-int layout_of(const Call& k, int from, int count, Layout& l) {
+// `planes`: of the Gram products' operands; `small`: in three launches, if the matrices allow it
+int layout_of(const Call& k, int from, int count, int planes, bool small, Layout& l) {
     for (int i = 0; i < count; ++i) {
         Shape s;
         if (!shape_of(k.rows[from + i], k.cols[from + i], s)) return FC3D_ERANGE;
@@ -838,7 +1141,21 @@ int layout_of(const Call& k, int from, int count, Layout& l) {
     }
     int64_t prep = 0, depth = 0;
     int64_t groups[kKernelCount] = {};
-    l.parts = l.halves = 0;
+    l.parts = l.halves = l.sum_tiles = 0;
+    l.small = small;
+    for (int i = 0; i < count; ++i) l.small = l.small && l.shape[i].m <= kSmall;
+    if (l.small) {
+        for (int i = 0; i < count; ++i) {
+            // columns of a chunk, at most kChunks chunks (two at least are laid out: the product P takes their place)
+            Shape& s = l.shape[i];
+            s.mp = kSmall;
+            s.np = ((s.n + kChunks - 1) / kChunks + 63) / 64 * 64;
+            l.split[i] = (int)((s.n + s.np - 1) / s.np);
+            l.sum_tiles += l.split[i] < 2 ? 2 : l.split[i];
+            prep += (s.n + 63) / 64;
+        }
+        return prep >= (1 << 23) ? FC3D_ERANGE : FC3D_OK;
+    }
     for (int i = 0; i < count; ++i) {
         Shape& s = l.shape[i];
         s.mp = (s.m + kSlice - 1) / kSlice * kSlice;
@@ -852,7 +1169,7 @@ int layout_of(const Call& k, int from, int count, Layout& l) {
     if (prep >= (1 << 23) || l.parts >= (1 << 23)) return FC3D_ERANGE;      // workgroups of one launch
     // The Gram products: the kernel is picked for them once, since the sums of shared depth are laid out for its tile.
     // Where there are few tiles, the depth is shared out, eight slices at least to each workgroup, one round of them.
-    l.gram = kernel_for(groups, depth, k.g_type != FC3D_F32 && !k.mom ? 2 : 0);
+    l.gram = kernel_for(groups, depth, planes);
     const int tile = kKernels[l.gram].tile;
     int64_t tiles = groups[l.gram], slices = 0;
     for (int i = 0; i < count; ++i) slices += tiles_of(MUL, (int)l.shape[i].mp, 0, 1, tile) * (l.shape[i].np / kSlice);
@@ -892,15 +1209,46 @@ int product(const Call& k, const Launch& a, int64_t groups, int p1, int p2) {
     return FC3D_OK;
 }
 
+template <typename F>
+int by_type(int type, F&& f) {
+    return type == FC3D_F32 ? f(float{}) : type == FC3D_BF16 ? f(__bf16{}) : f(_Float16{});
+}
+
+int run_small(const Call& k, int from, const Layout& l, int count) {
+    Table t = {};
+    t.count = count;
+    int64_t sums = 0, gram_groups = 0, apply_groups = 0;
+    for (int i = 0; i < count; ++i) {
+        const Shape& s = l.shape[i];
+        const int at = from + l.order[i];
+        t.e[i] = Matrix{k.g[at], k.mom ? k.mom[at] : nullptr, k.out[at], 0, (int)s.m, (int)s.n, (int)s.mp, (int)s.np,
+                        k.lr ? k.lr[at] : 0.0f, 0, l.split[i], (int)sums, k.rows[at] > k.cols[at], 0};
+        sums += l.split[i] < 2 ? 2 : l.split[i];
+        gram_groups += l.split[i];
+        apply_groups += (s.n + 63) / 64;
+    }
+    Matrix* table = reinterpret_cast<Matrix*>(k.ws);
+    double* gram = reinterpret_cast<double*>(k.ws + l.head());
+    return by_type(k.g_type, [&](auto zero) {
+        typedef decltype(zero) T;
+        FC3D_LAUNCH("ns_small_gram", ns_small_gram_kernel<T>, dim3((unsigned)gram_groups), dim3(256), 0, k.s, t, k.blend, table, gram);
+        FC3D_LAUNCH("ns_small_chain", ns_small_chain_kernel, dim3((unsigned)count), dim3(1024), 0, k.s, table, gram, k.steps, k.a,
+                    k.b, k.c, k.eps);
+        FC3D_LAUNCH("ns_small_apply", ns_small_apply_kernel<T>, dim3((unsigned)apply_groups), dim3(256), 0, k.s, table, count,
+                    k.blend, gram, k.out_type, (int)(k.lr != nullptr), k.decay);
+        return FC3D_OK;
+    });
+}
+
 int run_group(const Call& k, int from, const Layout& l, const Scales& sc, int count) {
     Table t = {};
     t.count = count;
-    const bool exact = k.g_type != FC3D_F32 && !k.mom;
+    const bool exact = is_exact(k);
     int64_t parts = 0, halves = 0, prep = 0, sums = 0;
     bool used[kPlans] = {};
     for (int i = 0; i < count; ++i) {
         const Shape& s = l.shape[i];
-        const int at = from + l.order[i], plan = plan_of(k.out_type, k.steps, s);
+        const int at = from + l.order[i], plan = plan_of(k, sc.gain, s);
         t.e[i] = Matrix{k.g[at], k.mom ? k.mom[at] : nullptr, k.out[at], halves, (int)s.m, (int)s.n, (int)s.mp, (int)s.np,
                         k.lr ? k.lr[at] : 0.0f, (int)parts, l.split[i], (int)sums, k.rows[at] > k.cols[at], plan};
         used[plan] = true;
@@ -913,9 +1261,14 @@ int run_group(const Call& k, int from, const Layout& l, const Scales& sc, int co
     Matrix* table = reinterpret_cast<Matrix*>(k.ws + parts * 8);
     float* rho = reinterpret_cast<float*>(table + kMaxItems);
     _Float16* planes = reinterpret_cast<_Float16*>(k.ws + l.head());
-    FC3D_LAUNCH("ns_norm", ns_norm_kernel, dim3((unsigned)parts), dim3(256), 0, k.s, t, k.g_type, k.blend, squares, table);
-    FC3D_LAUNCH("ns_prepare", ns_prepare_kernel, dim3((unsigned)prep), dim3(256), 0, k.s, table, count, k.g_type, k.blend,
-                squares, k.eps, sc.x, (int)exact, planes, rho);
+    const auto first = [&](auto zero) {
+        typedef decltype(zero) T;
+        FC3D_LAUNCH("ns_norm", ns_norm_kernel<T>, dim3((unsigned)parts), dim3(256), 0, k.s, t, k.blend, squares, table);
+        FC3D_LAUNCH("ns_prepare", ns_prepare_kernel<T>, dim3((unsigned)prep), dim3(256), 0, k.s, table, count, k.blend, squares,
+                    k.eps, sc.x, (int)exact, planes, rho);
+        return FC3D_OK;
+    };
+    if (const int rc = by_type(k.g_type, first)) return rc;
 
     static thread_local PlanOps ops[kPlans];
     int launches = 0;
@@ -973,23 +1326,36 @@ int run_group(const Call& k, int from, const Layout& l, const Scales& sc, int co
 bool known_type(int t) { return t >= FC3D_F32 && t <= FC3D_F16; }
 bool off_align(const void* p, int type) { return (reinterpret_cast<uintptr_t>(p) & (type == FC3D_F32 ? 3u : 1u)) != 0; }
 
-// Matrices in groups of kMaxItems, one group after the other in the same workspace.  `run`: false only sizes it.
-int walk(const Call& k, bool run, size_t& bytes) {
-    bytes = 0;
-    Scales sc = {};
-    if (run) {
-        const int longest = k.out_type == FC3D_F32 ? 3 : 5;
-        if (!scales_of(k, k.steps < longest ? k.steps : longest, sc)) return FC3D_ERANGE;
-    }
+// Matrices in groups of kMaxItems, one group after the other in the same workspace
+template <typename F>
+int in_groups(const Call& k, F&& f) {
     for (int from = 0; from < k.count; from += kMaxItems) {
         const int count = k.count - from < kMaxItems ? k.count - from : kMaxItems;
-        Layout l = {};
-        if (const int rc = layout_of(k, from, count, l)) return rc;
-        if ((size_t)l.bytes() > bytes) bytes = (size_t)l.bytes();
-        if (run)
-            if (const int rc = run_group(k, from, l, sc, count)) return rc;
+        if (const int rc = f(from, count)) return rc;
     }
     return FC3D_OK;
+}
+// The workspace is sized for every layout that a call with these sizes may take
+int size_of(const Call& k, size_t& bytes) {
+    bytes = 0;
+    return in_groups(k, [&](int from, int count) {
+        for (int way = 0; way < 3; ++way) {
+            Layout l = {};
+            if (const int rc = layout_of(k, from, count, way == 1 ? 2 : 0, way == 2, l)) return rc;
+            if ((size_t)l.bytes() > bytes) bytes = (size_t)l.bytes();
+        }
+        return (int)FC3D_OK;
+    });
+}
+
+int run(const Call& k) {
+    Scales sc = {};
+    if (!scales_of(k, sc)) return FC3D_ERANGE;
+    return in_groups(k, [&](int from, int count) {
+        Layout l = {};
+        if (const int rc = layout_of(k, from, count, is_exact(k) ? 2 : 0, small_of(k, sc.gain), l)) return rc;
+        return l.small ? run_small(k, from, l, count) : run_group(k, from, l, sc, count);
+    });
 }
 
 int check_call(const Call& k) {
@@ -1004,10 +1370,12 @@ int check_call(const Call& k) {
     }
     // sizes and coefficients are checked before the first launch, the latter alike for all types: a caller that works
     // on several lists is refused before the first one or not at all
+    Call most = k;
+    most.out_type = FC3D_BF16;
     Scales sc;
-    if (!scales_of(k, k.steps < 5 ? k.steps : 5, sc)) return FC3D_ERANGE;
+    if (!scales_of(most, sc)) return FC3D_ERANGE;
     size_t bytes;
-    return walk(k, false, bytes);
+    return size_of(k, bytes);
 }
 
 }  // namespace
@@ -1022,7 +1390,7 @@ extern "C" size_t fc3d_orthogonalize_workspace(int count, const int64_t* rows, c
     k.rows = rows;
     k.cols = cols;
     size_t bytes = 0;
-    return walk(k, false, bytes) == FC3D_OK ? bytes : 0;
+    return size_of(k, bytes) == FC3D_OK ? bytes : 0;
 }
 
 extern "C" int fc3d_orthogonalize(void* stream, int count, const void* const* g, void* const* out, const int64_t* rows,
@@ -1043,8 +1411,7 @@ extern "C" int fc3d_orthogonalize(void* stream, int count, const void* const* g,
     k.eps = eps;
     k.ws = (char*)workspace;
     if (const int rc = check_call(k)) return rc;
-    size_t bytes;
-    return walk(k, true, bytes);
+    return run(k);
 }
 
 extern "C" int fc3d_muon_step(void* stream, int count, void* const* params, const void* const* grads, float* const* momenta,
@@ -1073,6 +1440,5 @@ extern "C" int fc3d_muon_step(void* stream, int count, void* const* params, cons
     k.decay = (float)decay;
     k.ws = (char*)workspace;
     if (const int rc = check_call(k)) return rc;
-    size_t bytes;
-    return walk(k, true, bytes);
+    return run(k);
 }

@@ -169,6 +169,70 @@ def test_other_step_counts_and_coefficients(dt, steps):
 
 
 @gpu
+@pytest.mark.parametrize("steps", [5, 10, 11, 16])
+def test_rank_deficient_matrices_and_many_steps(steps):
+    """Directions that the input lacks: what a step rounds there is amplified as a singular value would be."""
+    from fc3d import ops
+    for m, n in ((40, 200), (64, 90), (96, 300)):
+        g = torch.Generator().manual_seed(steps * m)
+        x = torch.randn(m, 6, generator=g) @ torch.randn(6, n, generator=g)
+        near(ops.orthogonalize(x.cuda(), steps=steps), x, f"rank 6 of {m}, {steps} steps", steps)
+        x[m // 2:] = 0.0
+        near(ops.orthogonalize(x.cuda(), steps=steps), x, f"empty rows of {m}, {steps} steps", steps)
+
+
+@gpu
+@pytest.mark.parametrize("steps", [2, 3, 5])
+def test_steep_coefficients(steps):
+    """0.9 T_5(x), the Chebyshev polynomial: it multiplies small values by 4.5 and stays below one on [0, 1]."""
+    from fc3d import ops
+    coeffs = (4.5, -18.0, 14.4)
+    a, b, c = coeffs
+    lam = torch.linspace(0.0, 1.0, 20001, dtype=torch.float64, requires_grad=True)
+    q0 = a + b * lam + c * lam * lam
+    l1 = lam * q0 * q0
+    (q0 * (a + b * l1 + c * l1 * l1)).sum().backward()
+    slope = float((lam.detach().sqrt() * lam.grad.abs()).max())          # of two steps' factor, as for five above
+    for m, n in ((40, 200), (96, 300), (130, 150)):
+        g = update((m, n), "gauss", 300 + m)
+        near(ops.orthogonalize(g.cuda(), steps=steps, coefficients=coeffs), g, f"{m} x {n}, {steps} steps", steps, coeffs)
+        if steps == 2:
+            h = g.bfloat16()
+            ref = ns(h, torch.float64, steps, coeffs)
+            tol = bound(h.float(), ref, steps, coeffs) + torch.finfo(BF16).eps / 2 + \
+                slope * 2 * 2.0 ** -23 / math.sqrt(m) * math.sqrt(m) / float(ref.norm())
+            off = float((ops.orthogonalize(h.cuda(), steps=steps, coefficients=coeffs).cpu().double() - ref).norm() / ref.norm())
+            assert off <= tol, (m, n, off, tol)
+
+
+@gpu
+@pytest.mark.parametrize("dt", [F32, BF16, F16], ids=lambda t: str(t).replace("torch.", ""))
+def test_workspace_holds_every_type_and_step_count(dt):
+    """The workspace is sized by the matrices alone, what a call lays out in it depends on its types and steps too."""
+    import ctypes
+    from fc3d import _native
+    lib = _native.load()
+    I64, VP = ctypes.c_int64, ctypes.c_void_p
+    code = {F32: 0, BF16: 1, F16: 2}[dt]
+    for shapes in ([(64, 4000)], [(20, 30), (64, 64)], [(130, 9000)], [(300, 5000), (96, 200)], [(520, 4608), (64, 288), (32, 9)]):
+        gs = [update(s, "gauss", 40 + i, dt).cuda() for i, s in enumerate(shapes)]
+        k = len(shapes)
+        r, c = (I64 * k)(*[s[0] for s in shapes]), (I64 * k)(*[s[1] for s in shapes])
+        n = lib.fc3d_orthogonalize_workspace(k, r, c)
+        ws = torch.full((n + 512,), 77, dtype=torch.uint8, device="cuda")
+        base = ws.data_ptr() + 256
+        assert base % 256 == 0
+        at = (VP * k)(*[g.data_ptr() for g in gs])
+        for steps in (1, 5, 12):
+            out = [torch.empty_like(g) for g in gs]
+            to = (VP * k)(*[o.data_ptr() for o in out])
+            assert lib.fc3d_orthogonalize(torch.cuda.current_stream().cuda_stream, k, at, to, r, c, code, steps, *COEFFS, 1e-7, base) == 0
+            torch.cuda.synchronize()
+            assert bool((ws[:256] == 77).all()) and bool((ws[256 + n:] == 77).all()), (shapes, steps)
+            assert all(bool(torch.isfinite(o).all()) for o in out)
+
+
+@gpu
 def test_scales_zeros_and_special_values():
     from fc3d import ops
     g = update((40, 100), "gauss", 5)
