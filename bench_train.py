@@ -38,6 +38,10 @@ def main():
                          "batch semantics); rank_mean: per-rank losses, averaged gradients")
     ap.add_argument("--buckets", type=int, default=3, help="ranges the 69 MB gradient buffer is all-reduced in")
     ap.add_argument("--no-overlap", action="store_true", help="start the all-reduce after backward instead of from hooks")
+    ap.add_argument("--norm", choices=("batch", "layer"), default="batch",
+                    help="of the U-Nets: batch as in the reference, layer over the channels of every pixel")
+    ap.add_argument("--optimizer", choices=("adam", "muon"), default="adam",
+                    help="muon: orthogonalised momentum for the hidden convolutions, Adam for the rest")
     ap.add_argument("--n1-value", type=float, default=None,
                     help="steps/s of a previous --gpus 1 run: the line then carries scaling_efficiency_vs_n1")
     args = ap.parse_args()
@@ -59,7 +63,7 @@ def main():
     z_p, z_c, pose = d(sc["z_p"]), d(sc["z_c"]), d(sc["pose_p2c"])
     torch.manual_seed(1234)          # identical initial weights on every rank
     step = capture.TrainStep(dev, intrinsics=(W / 2, H / 2), loss=args.loss, n_buckets=args.buckets,
-                             overlap=not args.no_overlap)
+                             overlap=not args.no_overlap, norm=args.norm, optimizer=args.optimizer)
     # The first steps can sit in the convolution library's kernel search for minutes without a
     # word; a heartbeat on stderr tells a watching harness that the run is alive.
     import threading
@@ -100,7 +104,8 @@ def main():
         torch.cuda.synchronize()
         sim_ms = 1e3 * (time.perf_counter() - t1) / args.steps
     if rank == 0:
-        print(json.dumps({"metric": "training steps/sec (capture simulation + 2 U-Nets + reproj loss + Adam), data parallel",
+        print(json.dumps({"metric": "training steps/sec (capture simulation + 2 U-Nets + reproj loss + "
+                                    f"{args.optimizer.capitalize()}), data parallel",
                           "value": args.steps / el, "unit": "steps/s", "samples_per_s": world * args.batch * args.steps / el,
                           "n_gpus": world, "steps": args.steps, "warmup": args.warmup, "ms_per_step": 1e3 * el / args.steps,
                           "world_size": torch.distributed.get_world_size() if world > 1 else 1,
@@ -110,6 +115,7 @@ def main():
                           "config": {"workload": f"{args.batch}x{H}x{W} per GPU, global batch {world * args.batch}",
                                      "grad_allreduce_bytes": step.bucket.nbytes, "grad_ranges": len(step.bucket.ranges),
                                      "overlap": step.bucket.overlap, "loss_mode": args.loss,
+                                     "norm": args.norm, "optimizer": args.optimizer,
                                      "conv_find_mode": os.environ["MIOPEN_FIND_MODE"]},
                           "capture_simulation_ms": sim_ms, "capture_share": sim_ms / (1e3 * el / args.steps),
                           "loss": float(loss)}), flush=True)

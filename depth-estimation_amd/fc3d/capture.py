@@ -285,22 +285,34 @@ class TrainStep:
     are averaged (the usual data-parallel approximation); "global" -- the masked sums and mask
     counts are added over ranks before the losses are formed (utils_pytorch.py:161-163, :177), so
     the step equals a single-process step on the concatenated batch up to BatchNorm statistics,
-    which stay per rank."""
+    which stay per rank.
+
+    norm: "batch" as in the reference, "layer" for networks without batch statistics (fc3d.nets).
+    optimizer: "adam" as in the reference; "muon" moves the hidden convolutions by orthogonalised
+    momentum (fc3d.optim.Muon, at muon_lr) and leaves biases, norms, first layers and heads to Adam."""
 
     def __init__(self, device, n_layers=21, is_conv_psf=True, crop=None, lr=1e-4, weight_reproj=1.0, intrinsics=None,
-                 loss="rank_mean", n_buckets=3, overlap=True):
+                 loss="rank_mean", n_buckets=3, overlap=True, norm="batch", optimizer="adam", muon_lr=0.02):
         from . import dist as fdist
-        from . import nets
+        from . import nets, optim
         if loss not in ("rank_mean", "global"):
             raise ValueError(f"unknown loss mode {loss!r}")
-        self.model_xy = nets.UNet_xy().to(device)
-        self.model_z = nets.UNet_z().to(device)
+        if optimizer not in ("adam", "muon"):
+            raise ValueError(f"unknown optimizer {optimizer!r}")
+        self.model_xy = nets.UNet_xy(norm).to(device)
+        self.model_z = nets.UNet_z(norm).to(device)
         self.intrinsics = intrinsics
         self.params = list(self.model_xy.parameters()) + list(self.model_z.parameters())
         # every rank starts from rank 0's weights and BatchNorm statistics, whatever its own seed was
         fdist.broadcast_module_state([self.model_xy, self.model_z])
         self.bucket = fdist.FlatGradBucket(self.params, n_buckets=n_buckets, overlap=overlap)
-        self.opt = torch.optim.Adam(self.params, lr=lr)
+        self.muon = None
+        if optimizer == "muon":
+            matrices, others = optim.split_parameters([self.model_xy, self.model_z], leave=nets.UNet.EDGES)
+            self.muon = optim.Muon(matrices, lr=muon_lr)
+            self.opt = torch.optim.Adam(others, lr=lr)
+        else:
+            self.opt = torch.optim.Adam(self.params, lr=lr)
         self.n_layers, self.is_conv_psf, self.crop, self.w = n_layers, is_conv_psf, crop, weight_reproj
         self.loss_mode = loss
         self.keep_capture = False          # True: the simulated capture of the last step stays in self.last_capture
@@ -330,4 +342,6 @@ class TrainStep:
         self.bucket.average(async_op=True)
         self.bucket.wait()
         self.opt.step()
+        if self.muon is not None:
+            self.muon.step()
         return loss.detach()

@@ -1477,7 +1477,7 @@ def muon_step(params, grads, momenta, lr: float = 0.02, momentum: float = 0.95, 
     decay = 1.0 - lr * weight_decay
     if not (np.isfinite(lr) and np.isfinite(decay)):
         raise ValueError(f"lr and weight_decay must be finite (got {lr}, {weight_decay})")
-    written = set()
+    spans = []
     groups: dict = {}
     for p, g, m in zip(params, grads, momenta):
         code, g_code = _need_gpu_float(p, "weights"), _need_gpu_float(g, "gradients")
@@ -1495,12 +1495,19 @@ def muon_step(params, grads, momenta, lr: float = 0.02, momentum: float = 0.95, 
             continue
         if m.stride() != p.stride() and not (m.is_contiguous() and p.is_contiguous()):
             raise ValueError(f"a momentum of strides {m.stride()} beside a weight of strides {p.stride()}")
-        if p.data_ptr() in written or m.data_ptr() in written:
-            raise ValueError("a weight or momentum is in the list twice")
-        written.update((p.data_ptr(), m.data_ptr()))
         if g.stride() != p.stride() and not (g.is_contiguous() and p.is_contiguous()):
             g = torch.empty_like(p, dtype=g.dtype).copy_(g)
+        # dense, all three: what they take in memory
+        spans += [(t.data_ptr(), t.data_ptr() + t.numel() * t.element_size(), written)
+                  for t, written in ((p, True), (m, True), (g, False))]
         groups.setdefault((code, g_code), []).append((p, g, m, order, lr * factor))
+    last = last_written = 0                          # ends of what lies below, of all and of what is written
+    for start, end, written in sorted(spans):
+        if start < (last if written else last_written):
+            raise ValueError("weights and momenta must not share memory, with each other or with a gradient (is one in the list twice?)")
+        last = max(last, end)
+        if written:
+            last_written = max(last_written, end)
     # nothing is written before every list has its workspace
     spaces = [_ns_workspace([it[3][0] for it in items], [it[3][1] for it in items], params[0].device)
               for items in groups.values()]

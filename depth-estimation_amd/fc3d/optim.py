@@ -9,6 +9,21 @@ import torch
 from . import ops
 
 
+def split_parameters(modules, leave=()):
+    """(matrices, others): the modules' weights of two axes or more, which Muon takes, and all other parameters, among
+    them everything below a submodule that `leave` names (the first layer, the head).  Each parameter once, in order."""
+    modules = [modules] if isinstance(modules, torch.nn.Module) else list(modules)
+    matrices, others, seen = [], [], set()
+    for module in modules:
+        for name, p in module.named_parameters():
+            if id(p) in seen:
+                continue
+            seen.add(id(p))
+            kept = any(name == n or name.startswith(n + ".") for n in leave)
+            (others if kept or p.dim() < 2 else matrices).append(p)
+    return matrices, others
+
+
 class Muon(torch.optim.Optimizer):
     """lr, momentum, nesterov, weight_decay, steps, coefficients, eps, scale: as for fc3d.ops.muon_step, per group.
     The momentum is float32 whatever the weights' type."""

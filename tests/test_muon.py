@@ -362,6 +362,22 @@ def test_step_checks():
 
 
 @gpu
+def test_step_refuses_shared_memory():
+    """Whatever is written may lie over nothing else; gradients may share among themselves."""
+    from fc3d import ops
+    flat = torch.arange(200, dtype=torch.float32, device="cuda") / 200
+    at = lambda i, n=24: flat[i:i + n].view(4, n // 4)  # noqa: E731
+    before = flat.clone()
+    for p, g, m in (([at(0)], [at(0)], [at(48)]), ([at(0)], [at(48)], [at(48)]), ([at(0)], [at(20)], [at(48)]), ([at(0)], [at(48)], [at(8)]),
+                    ([at(0), at(12)], [at(48), at(72)], [at(96), at(120)]), ([at(0), at(24)], [at(48), at(48)], [at(72), at(92)])):
+        with pytest.raises(ValueError, match="share memory"):
+            ops.muon_step(p, g, m)
+    assert torch.equal(flat, before)
+    ops.muon_step([at(0), at(24)], [at(48), at(48)], [at(72), at(96)])         # neighbours, and one gradient for two
+    assert bool((flat[:48] != before[:48]).any()) and torch.equal(flat[48:72], before[48:72]) and torch.equal(flat[120:], before[120:])
+
+
+@gpu
 def test_step_of_weights_in_other_memory_orders():
     from fc3d import ops
     w, g, m = (update((24, 16, 3, 3), "gauss", 40 + i) for i in range(3))
