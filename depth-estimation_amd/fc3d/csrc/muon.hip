@@ -29,6 +29,9 @@ namespace fc3d {
 namespace {
 
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+
+typedef float float4v __attribute__((ext_vector_type(4)));
+typedef uint32_t uint4v __attribute__((ext_vector_type(4)));
 typedef float float16v __attribute__((ext_vector_type(16)));
 
 constexpr int kSlice = 64;            // depth of one staged slice of a product, and the unit that sizes are padded to
@@ -273,6 +276,11 @@ __global__ __launch_bounds__(256) void ns_prepare_kernel(const Matrix* __restric
     }
 }
 
+__device__ __forceinline__ uint32_t pair_word(float v) {
+    const _Float16 hi = (_Float16)v, lo = (_Float16)(v - (float)hi);
+    return (uint32_t)__builtin_bit_cast(uint16_t, hi) | (uint32_t)__builtin_bit_cast(uint16_t, lo) << 16;
+}
+
 // ---- products -----------------------------------------------------------------------------------------------
 // D[i][j] = sum_k S1[i][k] S2[j][k]: both operands run along the depth in memory (a symmetric matrix is its own
 // transpose, and X is kept in both orders), so one kernel serves every product:
@@ -335,30 +343,39 @@ __device__ __forceinline__ void upper_tile(int block, int t, int& ti, int& tj) {
     }
 }
 
+template <int T>
+struct Turn {
+    static constexpr int value = T;
+};
+
 // A workgroup computes a TILE x TILE tile.  A wavefront holds BLK x BLK of the 32 x 32 matrix instruction's sums, so that
 // an operand read from LDS feeds 3 BLK of them: TILE 64 and 96: every wavefront the whole tile, its part of the depth;
 // TILE 128: two wavefronts per quadrant.  Their sums meet at the end.  Stages are fetched ahead into registers (what
 // another compute unit has just written comes from behind the L2: most of a microsecond) and go through two LDS
 // buffers, one barrier per stage.  P1, P2: planes of the operands that count (1: the lo plane is zero).
+// 2048 rows and depth, one symmetric product, 37 us: about 5 us pass outside the workgroups, 1.6 until the first stage,
+// 25.7 in the stages, 4.5 for the result.  The stages alone take 15.7 us with nothing but the matrix instructions,
+// 16.6 with their reads from LDS, and the way from memory into LDS 20.6 us (400 MB, 19 TB/s out of the L2s): that path
+// bounds it, and the two overlap for the larger part.
 template <int TILE, int WAVES, int P1, int P2>
 __global__ __launch_bounds__(WAVES * 64, TILE == 64 && WAVES == 4 ? 2 : 1) void ns_product_kernel(Launch a) {
     constexpr bool QUADS = TILE == 128;
     constexpr int THREADS = WAVES * 64, BLK = QUADS ? 2 : TILE / 32;
     constexpr int NP = P1 + P2;
     constexpr int DEPTH = kSlice, ROW = DEPTH / 8;           // of a stage, in values and in 16-byte pieces
-    constexpr int AHEAD = QUADS ? 1 : 2;                     // stages in flight in registers
+    constexpr int AHEAD = QUADS ? (NP == 4 ? 1 : 2) : NP == 2 ? 3 : 2;      // stages in flight in registers
     static_assert(QUADS || WAVES * 16 == DEPTH, "every wavefront has 16 values of a stage's depth");
     constexpr int PIECES = TILE * ROW / THREADS;             // pieces of a stage per lane and plane
     constexpr int ROWS = THREADS / ROW;                      // rows that the workgroup's lanes cover at once
-    constexpr int SHARES = QUADS ? 2 : WAVES, LD = TILE + 1;
+    constexpr int SHARES = QUADS ? 2 : WAVES, LD = TILE + 8, LD2 = TILE + 4;
     constexpr int STAGE = NP * TILE * ROW;                   // pieces of one stage
-    constexpr int SUMS = SHARES * TILE * LD;                 // floats of the workgroup's result
-    constexpr int BYTES = 2 * STAGE * 16 > SUMS * 4 ? 2 * STAGE * 16 : SUMS * 4;
+    constexpr int SWAP = TILE * TILE * 4 * (SHARES - 1), RESULT = TILE * (LD + LD2) * 4;    // bytes
+    constexpr int MOST = SWAP > RESULT ? SWAP : RESULT, BYTES = 2 * STAGE * 16 > MOST ? 2 * STAGE * 16 : MOST;
     __shared__ __attribute__((aligned(16))) char shared[BYTES];
     half8* lds = reinterpret_cast<half8*>(shared);
     float* out = reinterpret_cast<float*>(shared);
 
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     int block = (int)block_x();
     // every lane reads one matrix of the table: what the workgroup needs of its own comes from that lane's registers
     Matrix e = a.table[lane < a.matrices ? lane : 0];
@@ -480,7 +497,7 @@ __global__ __launch_bounds__(WAVES * 64, TILE == 64 && WAVES == 4 ? 2 : 1) void 
         // LDS and memory instructions one by one between the matrix instructions: issued in a row they would fill the LDS
         // queue, and the matrix units would wait for it
         if (whole && P1 == 2 && P2 == 2) {
-            constexpr int READS = 4 * BLK, MOVES = NP * PIECES, EACH = QUADS || BLK == 3 ? 1 : 2;
+            constexpr int READS = 4 * BLK, LOADS = NP * PIECES, EACH = QUADS || BLK == 3 ? 1 : 2;
 #pragma unroll
             for (int half = 0; half < (QUADS ? 2 : 1); ++half) {
 #pragma unroll
@@ -489,7 +506,7 @@ __global__ __launch_bounds__(WAVES * 64, TILE == 64 && WAVES == 4 ? 2 : 1) void 
                     __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);        // matrix
                 }
 #pragma unroll
-                for (int q = 0; q < MOVES / EACH / (QUADS ? 2 : 1); ++q) {
+                for (int q = 0; q < LOADS / EACH / (QUADS ? 2 : 1); ++q) {
                     __builtin_amdgcn_sched_group_barrier(0x200, EACH, 0);     // LDS write
                     __builtin_amdgcn_sched_group_barrier(0x020, EACH, 0);     // load
                     __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
@@ -498,75 +515,152 @@ __global__ __launch_bounds__(WAVES * 64, TILE == 64 && WAVES == 4 ? 2 : 1) void 
         }
         __builtin_amdgcn_sched_barrier(0);
     };
-    Part fa, fb;                                              // even and odd stages; quadrants: the two halves of one
-    Part& odd = QUADS ? fa : fb;
-    Part& other = QUADS ? fb : fa;
-    fetch(0, next[0]);
-    if constexpr (AHEAD == 2) fetch(stages > 1 ? 1 : 0, next[1]);
-    stage(0, next[0]);
-    if (stages > AHEAD) fetch(AHEAD, next[0]);
-    half8 (&second)[NP * PIECES] = next[AHEAD - 1];
-    step(0, second, fa, fb, true, false);
-    int s = 1;
-    for (; s + 2 + AHEAD < stages; s += 2) {
-        step(s, next[0], odd, other, false, true);
-        step(s + 1, second, fa, fb, false, true);
-    }
-    for (; s < stages; ++s) {                                  // the last ones, by turns through copies
-        step(s, next[0], odd, other, false, false);
-        if constexpr (AHEAD == 2) {
+    // Even and odd stages' operands, or, in quadrants, those of a stage's two halves.  Registers, LDS buffers and operands
+    // come round every GROUP stages; the last ones, which fetch no more, are written out behind the loop.
+    Part part[2];
+    constexpr int GROUP = AHEAD == 3 ? 6 : 2;
+    const auto turn = [&](int s, auto t, bool first, bool whole) {       // stage s, the t-th of a group behind the first stage
+        constexpr int T = decltype(t)::value;
+        step(s, next[(T + 1) % AHEAD], part[QUADS ? 0 : T & 1], part[QUADS ? 1 : (T + 1) & 1], first, whole);
+    };
 #pragma unroll
-            for (int q = 0; q < NP * PIECES; ++q) {
-                const half8 t = next[0][q];
-                next[0][q] = next[1][q];
-                next[1][q] = t;
+    for (int q = 0; q < AHEAD; ++q) fetch(q < stages ? q : stages - 1, next[q]);
+    stage(0, next[0]);
+    fetch(AHEAD < stages ? AHEAD : stages - 1, next[0]);
+    int s = 1;
+    if (s + GROUP + AHEAD < stages) {                         // the loop is entered with all loads in flight, on no other path
+        turn(0, Turn<0>{}, true, true);
+        for (; s + GROUP + AHEAD < stages; s += GROUP) {
+            turn(s, Turn<1>{}, false, true);
+            turn(s + 1, Turn<2>{}, false, true);
+            if constexpr (GROUP == 6) {
+                turn(s + 2, Turn<3>{}, false, true);
+                turn(s + 3, Turn<4>{}, false, true);
+                turn(s + 4, Turn<5>{}, false, true);
+                turn(s + 5, Turn<6>{}, false, true);
             }
         }
-        if constexpr (!QUADS) {
-            const Part t = fa;
-            fa = fb;
-            fb = t;
+    } else {
+        turn(0, Turn<0>{}, true, false);
+    }
+    const int rest = stages - s;                              // at most GROUP + AHEAD
+    const auto tail = [&](auto t) {
+        constexpr int T = decltype(t)::value;
+        if (T <= GROUP + AHEAD && T <= rest) turn(s + T - 1, t, false, false);
+    };
+    tail(Turn<1>{});
+    tail(Turn<2>{});
+    tail(Turn<3>{});
+    tail(Turn<4>{});
+    if constexpr (GROUP == 6) {
+        tail(Turn<5>{});
+        tail(Turn<6>{});
+        tail(Turn<7>{});
+        tail(Turn<8>{});
+        tail(Turn<9>{});
+    }
+    // A lane holds column (lane & 31) of a 32 x 32 block, rows 8 (r / 4) + 4 (lane / 32) + r % 4
+    constexpr int OWN = 4 / SHARES;                           // of a block's quads of rows
+    const int half = QUADS ? wave & 1 : wave;
+    const int i0 = ti * TILE, j0 = tj * TILE;
+    const auto row_of = [&](int q, int k) { return bi + q / BLK * 32 + 8 * (half * OWN + k) + 4 * (lane >> 5); };
+    const auto col_of = [&](int q) { return bj + q % BLK * 32 + (lane & 31); };
+    constexpr int G = TILE / 8, MOVES = (TILE * G + THREADS - 1) / THREADS;       // a tile in pieces of eight values
+    half8 hi[MOVES], lo[MOVES];                               // POLY: A at the tile, on its way while the last products run
+    if (o.kind == POLY) {
+        int lda;
+        size_t pa;
+        const _Float16* A = buffer(e, a.planes, o.src1, lda, pa);
+#pragma unroll
+        for (int q = 0; q < MOVES; ++q) {
+            const int id = tid + THREADS * q, r = id / G, c = id % G * 8;
+            const size_t at = r < rows1 && c < rows2 ? (size_t)(i0 + r) * lda + j0 + c : 0;
+            hi[q] = *reinterpret_cast<const half8*>(A + at);
+            lo[q] = *reinterpret_cast<const half8*>(A + pa + at);
         }
     }
-    multiply(QUADS ? fb : other);
+    if (QUADS || (rest & 1)) multiply(part[1]);
+    else multiply(part[0]);
 
-    // ---- the result through LDS, so that it leaves in whole rows of either order.  Lane: column (lane & 31) of a
-    // 32 x 32 block, rows 8 (r / 4) + 4 (lane / 32) + r % 4
+    // ---- the result.  The wavefronts that share a block's depth exchange their sums as they hold them, 16 bytes at a
+    // time, and each is left with the whole sum of its rows.
+    float alpha = o.alpha;
+    if (o.use_rho) alpha *= o.kind == GRAM ? a.rho[w] * a.rho[w] : a.rho[w];
+    float4v sum[BLK * BLK][OWN];
+    float4v* swap = reinterpret_cast<float4v*>(shared);
+    const auto slot = [&](int to, int from, int q, int k) {   // of the share `from` (without the receiver's own) for wavefront `to`
+        return ((to * (SHARES - 1) + from) * (BLK * BLK * OWN) + q * OWN + k) * 64 + lane;
+    };
     __syncthreads();
+#pragma unroll
+    for (int d = 0; d < SHARES; ++d)
+#pragma unroll
+        for (int q = 0; q < BLK * BLK; ++q)
+#pragma unroll
+            for (int k = 0; k < OWN; ++k) {
+                const int r = 4 * (d * OWN + k);
+                const float16v& c = acc[q / BLK][q % BLK];
+                const float4v v = {c[r], c[r + 1], c[r + 2], c[r + 3]};
+                if (d == half) sum[q][k] = v;
+                else swap[slot(QUADS ? (wave & ~1) + d : d, half < d ? half : half - 1, q, k)] = v;
+            }
+    __syncthreads();
+#pragma unroll
+    for (int f = 0; f < SHARES - 1; ++f)
+#pragma unroll
+        for (int q = 0; q < BLK * BLK; ++q)
+#pragma unroll
+            for (int k = 0; k < OWN; ++k) sum[q][k] += swap[slot(wave, f, q, k)];
+    if (o.kind == GRAM && e.split > 1) {
+        float* to = a.sums + ((size_t)e.sums0 + (size_t)block * e.split + share) * TILE * TILE;
+#pragma unroll
+        for (int q = 0; q < BLK * BLK; ++q)
+#pragma unroll
+            for (int k = 0; k < OWN; ++k)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) to[(row_of(q, k) + r) * TILE + col_of(q)] = sum[q][k][r];
+        return;
+    }
 #pragma unroll
     for (int q = 0; q < BLK * BLK; ++q)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            const int i = bi + q / BLK * 32 + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3), j = bj + q % BLK * 32 + (lane & 31);
-            out[(QUADS ? wave & 1 : wave) * TILE * LD + i * LD + j] = acc[q / BLK][q % BLK][r];
-        }
-    __syncthreads();
-    const auto sum_at = [&](int at) {                         // the wavefronts' shares of one value
-        float v = out[at];
-#pragma unroll
-        for (int h = 1; h < SHARES; ++h) v += out[h * TILE * LD + at];
-        return v;
-    };
-    if (o.kind == GRAM && e.split > 1) {
-        float* to = a.sums + ((size_t)e.sums0 + (size_t)block * e.split + share) * TILE * TILE;
-#pragma unroll 4
-        for (int id = tid; id < TILE * TILE; id += THREADS) to[id] = sum_at(id / TILE * LD + id % TILE);
-        return;
-    }
-    float alpha = o.alpha;
-    if (o.use_rho) alpha *= o.kind == GRAM ? a.rho[w] * a.rho[w] : a.rho[w];
-    const int i0 = ti * TILE, j0 = tj * TILE;
+        for (int k = 0; k < OWN; ++k) sum[q][k] *= alpha;
     if (o.kind == APPLY && o.last) {
         with_type(a.out_type, [&](auto zero) {
             typedef decltype(zero) T;
             T* to = static_cast<T*>(e.out);
-#pragma unroll 4
+            if (!e.tall) {                                    // along the tensor's rows as the lanes hold them
+#pragma unroll
+                for (int q = 0; q < BLK * BLK; ++q)
+#pragma unroll
+                    for (int k = 0; k < OWN; ++k) {
+                        const int i = i0 + row_of(q, k), j = j0 + col_of(q);
+                        T* row = to + (size_t)i * e.n + j;
+                        float4v old = {};
+                        if (a.step)
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) old[r] = i + r < e.m && j < e.n ? (float)row[(size_t)r * e.n] : 0.0f;
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            float v = sum[q][k][r];
+                            if (a.step) v = fmaf(a.decay, old[r], -e.lr * v);
+                            if (i + r < e.m && j < e.n) row[(size_t)r * e.n] = (T)v;
+                        }
+                    }
+                return;
+            }
+            __syncthreads();
+#pragma unroll
+            for (int q = 0; q < BLK * BLK; ++q)
+#pragma unroll
+                for (int k = 0; k < OWN; ++k) *reinterpret_cast<float4v*>(out + col_of(q) * LD2 + row_of(q, k)) = sum[q][k];
+            __syncthreads();
+#pragma unroll 8
             for (int id = tid; id < TILE * TILE; id += THREADS) {
-                const int fast = id % TILE, slow = id / TILE; // fast: along the tensor's rows
-                const int r = e.tall ? fast : slow, c = e.tall ? slow : fast;
-                if (i0 + r < e.m && j0 + c < e.n) {
-                    const size_t at = e.tall ? (size_t)(j0 + c) * e.m + (i0 + r) : (size_t)(i0 + r) * e.n + (j0 + c);
-                    float v = sum_at(r * LD + c) * alpha;
+                const int i = id % TILE, j = id / TILE;
+                if (i0 + i < e.m && j0 + j < e.n) {
+                    const size_t at = (size_t)(j0 + j) * e.m + i0 + i;
+                    float v = out[j * LD2 + i];
                     if (a.step) v = fmaf(a.decay, (float)to[at], -e.lr * v);
                     to[at] = (T)v;
                 }
@@ -574,39 +668,93 @@ __global__ __launch_bounds__(WAVES * 64, TILE == 64 && WAVES == 4 ? 2 : 1) void 
         });
         return;
     }
-    // To the buffers, eight values of a row at a time: the tile, and its mirror image (or, of X, the transpose).  A tile
-    // on the diagonal holds every pair twice, its cross terms summed in two orders: the upper one counts for both.
+    // To the buffers: the tile, and its mirror image (or, of X, the transpose), from LDS in whole rows, eight values at a
+    // time.  A tile on the diagonal holds every pair twice, its cross terms summed in two orders: the upper one counts.
     const bool diagonal = o.kind != APPLY && ti == tj;
-    constexpr int G = TILE / 8;
+    uint32_t* pairs = reinterpret_cast<uint32_t*>(shared);    // hi and lo in one word
+    uint32_t* mirror = pairs + TILE * LD;
+    __syncthreads();
+    if (o.kind == POLY) {                                     // A through LDS, into the lanes that hold the sums
+        float* A = reinterpret_cast<float*>(shared);
+#pragma unroll
+        for (int q = 0; q < MOVES; ++q) {
+            const int id = tid + THREADS * q, r = id / G, c = id % G * 8;
+            if (r >= TILE) break;
+            float4v x, y;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                x[j] = (float)hi[q][j] + (float)lo[q][j];
+                y[j] = (float)hi[q][4 + j] + (float)lo[q][4 + j];
+            }
+            *reinterpret_cast<float4v*>(A + r * LD + c) = x;
+            *reinterpret_cast<float4v*>(A + r * LD + c + 4) = y;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int q = 0; q < BLK * BLK; ++q)
+#pragma unroll
+            for (int k = 0; k < OWN; ++k)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int i = row_of(q, k) + r, j = col_of(q);
+                    sum[q][k][r] = fmaf(a.b, A[i * LD + j], sum[q][k][r]);
+                    if (i0 + i == j0 + j && i0 + i < e.m) sum[q][k][r] += a.a;
+                }
+        __syncthreads();
+    }
+    const auto words_of = [&](int q, int k) {
+        return uint4v{pair_word(sum[q][k][0]), pair_word(sum[q][k][1]), pair_word(sum[q][k][2]), pair_word(sum[q][k][3])};
+    };
+    if (!diagonal) {
+#pragma unroll
+        for (int q = 0; q < BLK * BLK; ++q)
+#pragma unroll
+            for (int k = 0; k < OWN; ++k) {
+                const uint4v word = words_of(q, k);
+                *reinterpret_cast<uint4v*>(mirror + col_of(q) * LD2 + row_of(q, k)) = word;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) pairs[(row_of(q, k) + r) * LD + col_of(q)] = word[r];
+            }
+    } else {
+#pragma unroll
+        for (int q = 0; q < BLK * BLK; ++q)
+#pragma unroll
+            for (int k = 0; k < OWN; ++k) {
+                const uint4v word = words_of(q, k);
+                const int i = row_of(q, k), j = col_of(q);
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    if (i + r <= j) {
+                        pairs[(i + r) * LD + j] = word[r];
+                        pairs[j * LD + i + r] = word[r];
+                    }
+            }
+    }
+    __syncthreads();
     for (int side = 0; side < (diagonal ? 1 : 2); ++side) {
         int ld;
         size_t plane;
         _Float16* d = buffer(e, a.planes, o.kind == APPLY && side == 0 ? (int)BUF_X : o.dst, ld, plane);
-        const int to_i = side ? j0 : i0, to_j = side ? i0 : j0, rows = side ? rows2 : rows1, cols = side ? rows1 : rows2;
-#pragma unroll 2
-        for (int id = tid; id < TILE * G; id += THREADS) {
-            const int r = id / G, c = id % G * 8;
-            if (r >= rows || c >= cols) continue;
-            const size_t at = (size_t)(to_i + r) * ld + to_j + c;
-            float v[8];
-            half8 hi, lo;
-            if (o.kind == POLY) {                             // (A is its own mirror image)
-                int lda;
-                size_t pa;
-                const _Float16* A = buffer(e, a.planes, o.src1, lda, pa) + at;
-                hi = *reinterpret_cast<const half8*>(A);
-                lo = *reinterpret_cast<const half8*>(A + pa);
-            }
+        d += (size_t)(side ? j0 : i0) * ld + (side ? i0 : j0);
+        const uint32_t* from = side ? mirror : pairs;
+        const int rows = side ? rows2 : rows1, cols = side ? rows1 : rows2;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = sum_at(side || (diagonal && r > c + j) ? (c + j) * LD + r : r * LD + c + j) * alpha;
-            if (o.kind == POLY) {
+        for (int q = 0; q < MOVES; ++q) {
+            const int id = tid + THREADS * q, r = id / G, c = id % G * 8;
+            if (r >= TILE || r >= rows || c >= cols) continue;
+            const uint32_t* at = from + r * (side ? LD2 : LD) + c;
+            const uint4v x = *reinterpret_cast<const uint4v*>(at), y = *reinterpret_cast<const uint4v*>(at + 4);
+            uint4v h, l;
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    v[j] = fmaf(a.b, (float)hi[j] + (float)lo[j], v[j]);
-                    if (to_i + r == to_j + c + j && to_i + r < e.m) v[j] += a.a;
-                }
+            for (int j = 0; j < 2; ++j) {
+                h[j] = __builtin_amdgcn_perm(x[2 * j + 1], x[2 * j], 0x05040100u);
+                h[2 + j] = __builtin_amdgcn_perm(y[2 * j + 1], y[2 * j], 0x05040100u);
+                l[j] = __builtin_amdgcn_perm(x[2 * j + 1], x[2 * j], 0x07060302u);
+                l[2 + j] = __builtin_amdgcn_perm(y[2 * j + 1], y[2 * j], 0x07060302u);
             }
-            split8(d + at, plane, v);
+            _Float16* to = d + (size_t)r * ld + c;
+            *reinterpret_cast<uint4v*>(to) = h;
+            *reinterpret_cast<uint4v*>(to + plane) = l;
         }
     }
 }
