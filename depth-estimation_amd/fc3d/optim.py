@@ -26,7 +26,8 @@ def split_parameters(modules, leave=()):
 
 class Muon(torch.optim.Optimizer):
     """lr, momentum, nesterov, weight_decay, steps, coefficients, eps, scale: as for fc3d.ops.muon_step, per group.
-    The momentum is float32 whatever the weights' type."""
+    The momentum is float32 whatever the weights' type.  step() can be captured into a graph once every weight has been
+    stepped outside of one; the replays keep the rates they were captured with."""
 
     def __init__(self, params, lr: float = 0.02, momentum: float = 0.95, nesterov: bool = True, weight_decay: float = 0.0,
                  steps: int = 5, coefficients=ops.NS_COEFFICIENTS, eps: float = 1e-7, scale: str = "spectral"):
@@ -40,10 +41,13 @@ class Muon(torch.optim.Optimizer):
         ops.muon_scale((1, 1), scale)
         super().__init__(params, dict(lr=lr, momentum=momentum, nesterov=nesterov, weight_decay=weight_decay, steps=steps,
                                       coefficients=tuple(coefficients), eps=eps, scale=scale))
-        for group in self.param_groups:
-            for p in group["params"]:
-                if p.dim() < 2:
-                    raise ValueError(f"Muon is for weights of two axes or more, got one of shape {tuple(p.shape)}")
+
+    def add_param_group(self, param_group):
+        super().add_param_group(param_group)
+        for p in self.param_groups[-1]["params"]:
+            if p.dim() < 2:
+                self.param_groups.pop()
+                raise ValueError(f"Muon is for weights of two axes or more, got one of shape {tuple(p.shape)}")
 
     @torch.no_grad()
     def step(self, closure=None):
@@ -60,6 +64,9 @@ class Muon(torch.optim.Optimizer):
                     raise RuntimeError("Muon does not take sparse gradients")
                 state = self.state[p]
                 if "momentum_buffer" not in state:
+                    if p.is_cuda and torch.cuda.is_current_stream_capturing():
+                        raise RuntimeError("Muon: take one step before capturing one into a graph (a momentum made during the "
+                                           "capture would be cleared by every replay)")
                     state["momentum_buffer"] = torch.zeros_like(p, dtype=torch.float32)
                 lists = by_device.setdefault(p.device, ([], [], []))
                 for to, t in zip(lists, (p, p.grad, state["momentum_buffer"])):

@@ -11,7 +11,7 @@
  *
  * Conventions
  *  - every pointer is a DEVICE pointer unless the comment says "host";
- *  - all tensors are fp32 unless the name ends in _u8 / _i32 / _u64;
+ *  - all tensors are fp32 unless the name ends in _u8 / _i32 / _u64 or a type argument names another;
  *  - images are dense row-major [B][H][W][C]; where an input may be a strided
  *    view the element strides are passed explicitly;
  *  - `stream` is a hipStream_t passed as void* (NULL = the default stream);
@@ -466,8 +466,9 @@ int fc3d_layer_norm_bwd(void *stream, const void *dy, const void *x, int x_type,
  * (of the transpose where rows > cols), and out = X.  Evaluated in the Gram form with every
  * operand a pair of fp16 values and fp32 sums: the accuracy of fp32 products.  HOST arrays:
  * g, out (device pointers to dense row-major [rows][cols] tensors of `type`; out[i] may be
- * g[i]), rows, cols; they may be freed after the call.  A matrix must have a row and a column.
- * FC3D_ERANGE: sizes beyond 2^23, or coefficients that let singular values grow (beyond 16).
+ * g[i], nothing else may overlap), rows, cols; they may be freed after the call.  A matrix must
+ * have a row and a column.
+ * FC3D_ERANGE: sizes beyond 2^23, or coefficients that let singular values grow beyond 16.
  * workspace: fc3d_orthogonalize_workspace() bytes, 256-byte aligned, need not be initialised;
  * calls that may run at the same time need one each.                                          */
 size_t fc3d_orthogonalize_workspace(int count, const int64_t *rows, const int64_t *cols);
@@ -479,8 +480,8 @@ int fc3d_orthogonalize(void *stream, int count, const void *const *g, void *cons
  *   m <- momentum m + (1 - momentum) g;  u = (1 - momentum) g + momentum m if nesterov, else m;
  *   w <- decay w - lr[i] O(u),  O as in fc3d_orthogonalize.
  * HOST arrays as there; params in param_type, grads in grad_type, momenta fp32, all dense
- * row-major [rows][cols]; lr: one factor per matrix.  No matrix may appear twice.  The workspace
- * is that of fc3d_orthogonalize for the same sizes.                                           */
+ * row-major [rows][cols]; lr: one factor per matrix.  Neither params nor momenta may overlap each
+ * other or a gradient.  The workspace is that of fc3d_orthogonalize for the same sizes.        */
 int fc3d_muon_step(void *stream, int count, void *const *params, const void *const *grads, float *const *momenta,
                    const int64_t *rows, const int64_t *cols, const float *lr, int param_type, int grad_type,
                    double momentum, int nesterov, double decay, int steps, double a, double b, double c, double eps,

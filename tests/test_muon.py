@@ -182,6 +182,22 @@ def test_rank_deficient_matrices_and_many_steps(steps):
 
 
 @gpu
+@pytest.mark.parametrize("dt", [F32, BF16, F16], ids=lambda t: str(t).replace("torch.", ""))
+def test_many_steps_keep_the_singular_values_bounded(dt):
+    """The default polynomial maps [0, 1.21] into itself (1.203 at its maximum): whatever rounding leaves in directions that
+    the input lacks grows to that and no further.  Bound: 1.21 and a 16-bit result's rounding."""
+    from fc3d import ops
+    for m, n in ((40, 200), (96, 300), (70, 75)):
+        g = torch.Generator().manual_seed(m)
+        x = torch.randn(m, 5, generator=g) @ torch.randn(5, n, generator=g)
+        x[m // 2:] = 0.0
+        for steps in (16, 30, 64):
+            y = ops.orthogonalize(x.to(dt).cuda(), steps=steps).cpu().double()
+            top = float(torch.linalg.svdvals(y)[0])
+            assert 0.6 < top <= 1.21 * (1 + torch.finfo(dt).eps), (m, n, steps, top)
+
+
+@gpu
 @pytest.mark.parametrize("steps", [2, 3, 5])
 def test_steep_coefficients(steps):
     """0.9 T_5(x), the Chebyshev polynomial: it multiplies small values by 4.5 and stays below one on [0, 1]."""
@@ -392,6 +408,48 @@ def test_step_of_weights_in_other_memory_orders():
     ops.muon_step([a], [b], [c], scale="rms")
     ops.muon_step([ta.t()], [tb.t()], [tc.t()], scale="rms")           # the factor is the same both ways round
     assert torch.equal(a, ta) and torch.equal(c, tc)
+
+
+def test_groups_of_the_optimizer():
+    from fc3d import optim
+    opt = optim.Muon([torch.nn.Parameter(torch.zeros(4, 4))])
+    with pytest.raises(ValueError, match="two axes"):
+        opt.add_param_group({"params": [torch.nn.Parameter(torch.zeros(4))]})
+    assert len(opt.param_groups) == 1                                  # as it was
+    opt.add_param_group({"params": [torch.nn.Parameter(torch.zeros(4, 2))], "lr": 0.5})
+    assert [g["lr"] for g in opt.param_groups] == [0.02, 0.5]
+    assert opt.step() is None                                          # no gradients: nothing to do, on any device
+
+
+@gpu
+def test_optimizer_in_a_graph(monkeypatch):
+    from fc3d import optim
+    make = lambda: torch.nn.Parameter(update((40, 90), "gauss", 90).cuda())  # noqa: E731
+    p, q = make(), make()
+    opts = [optim.Muon([t]) for t in (p, q)]
+    p.grad, q.grad = torch.zeros_like(p), torch.zeros_like(q)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    with pytest.raises(RuntimeError, match="before capturing"):
+        opts[0].step()
+    monkeypatch.undo()
+    assert torch.equal(p, q)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        opts[0].step()                                                 # its momentum exists from here on
+    torch.cuda.current_stream().wait_stream(side)
+    opts[1].step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side, capture_error_mode="thread_local"):
+        opts[0].step()
+    for turn in range(4):
+        g = update((40, 90), "low", 91 + turn).cuda()
+        p.grad.copy_(g)
+        q.grad.copy_(g)
+        graph.replay()
+        opts[1].step()
+        torch.cuda.synchronize()
+        assert torch.equal(p, q) and torch.equal(opts[0].state[p]["momentum_buffer"], opts[1].state[q]["momentum_buffer"])
 
 
 @gpu
