@@ -107,39 +107,74 @@ __device__ __forceinline__ void put_param(void* p, int type, long i, float v) {
 // Whether max(pre, 0) hands pre on; a NaN passes, in both directions
 __device__ __forceinline__ bool passes(float pre) { return !(pre <= 0.0f); }
 
-// Sum over the LPR lanes that share a row, the same bits in every lane.  Above one wavefront the wavefronts' sums
-// meet in LDS; `slot` alternates between two areas, so that one barrier per sum is enough.
+// N sums over the LPR lanes that share a row, the same bits in every lane.  Above one wavefront the wavefronts' sums
+// meet in LDS; `slot` alternates between two areas, so that one barrier for all of them is enough.
+template <int LPR, int BLOCK, int N>
+__device__ __forceinline__ void group_sums(float (&v)[N], float* red, int slot) {
+#pragma unroll
+    for (int o = (LPR < 64 ? LPR : 64) / 2; o > 0; o >>= 1)
+#pragma unroll
+        for (int n = 0; n < N; ++n) v[n] += __shfl_xor(v[n], o, 64);
+    if constexpr (LPR > 64) {
+        float* a = red + slot * (BLOCK / 64) * N;
+        if ((threadIdx.x & 63) == 0)
+#pragma unroll
+            for (int n = 0; n < N; ++n) a[(threadIdx.x >> 6) * N + n] = v[n];
+        __syncthreads();
+        a += threadIdx.x / LPR * (LPR / 64) * N;
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            v[n] = a[n];
+#pragma unroll
+            for (int i = 1; i < LPR / 64; ++i) v[n] += a[i * N + n];
+        }
+    }
+}
 template <int LPR, int BLOCK>
 __device__ __forceinline__ float group_sum(float v, float* red, int slot) {
-#pragma unroll
-    for (int o = (LPR < 64 ? LPR : 64) / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
-    if constexpr (LPR > 64) {
-        float* a = red + slot * (BLOCK / 64);
-        if ((threadIdx.x & 63) == 0) a[threadIdx.x >> 6] = v;
-        __syncthreads();
-        a += threadIdx.x / LPR * (LPR / 64);
-        v = a[0];
-#pragma unroll
-        for (int i = 1; i < LPR / 64; ++i) v += a[i];
-    }
-    return v;
+    float one[1] = {v};
+    group_sums<LPR, BLOCK>(one, red, slot);
+    return one[0];
 }
 
 // ---- rows -------------------------------------------------------------------------------------------------
 // LPR lanes per row, E values each (vectors of 16 bytes, lane after lane); a workgroup takes rows
 // blockIdx.x * (BLOCK / LPR) + k * gridDim.x * ..., its lanes keep their columns' weights.  The next row is loaded before
-// the sums of the current one are formed, which would leave the memory idle otherwise (not with 1024 lanes per row: they
-// have 128 registers each).
+// the sums of the current one are formed, which would leave the memory idle otherwise (not with 1024 lanes per row, which
+// have 128 registers: 4096 x 8192 fp32 44 us, 54 with the next row ahead).
 template <typename T, int LPR, int E>
 struct Row {
     static constexpr int V = 16 / sizeof(T), NV = E / V;
     Vec<T, V> v[NV];
 
-    __device__ __forceinline__ void load(const T* row, int lane, int C) {
+    // even: the row is whole vectors.  A branch of lanes around a load makes its wait part of the branch, one load after the
+    // other; so the lanes behind the row's end read its first values and put them away (backward, bf16, 32768 x 1024 46 ->
+    // 39 us, 16384 x 2048 49 -> 44; fp32 81 -> 77).
+    __device__ __forceinline__ void load(const T* row, int lane, int C, bool even) {
+        if (even) {
+#pragma unroll
+            for (int k = 0; k < NV; ++k) {
+                const int c0 = (lane + k * LPR) * V;
+                v[k] = ldv<T, V>(row + (c0 < C ? c0 : 0));
+            }
+#pragma unroll
+            for (int k = 0; k < NV; ++k)
+                if ((lane + k * LPR) * V >= C) v[k] = Vec<T, V>{};
+        } else {
+#pragma unroll
+            for (int k = 0; k < NV; ++k) {
+                const int c0 = (lane + k * LPR) * V;
+                v[k] = ldv_n<T, V>(row + (c0 < C ? c0 : 0), C - c0);
+            }
+        }
+    }
+    __device__ __forceinline__ void store(T* row, int lane, int C, bool even) const {
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
             const int c0 = (lane + k * LPR) * V;
-            v[k] = ldv_n<T, V>(row + (c0 < C ? c0 : 0), C - c0);
+            if (c0 >= C) continue;
+            if (even) stv<T, V>(row + c0, v[k]);
+            else stv_n<T, V>(row + c0, v[k], C - c0);
         }
     }
 };
@@ -178,18 +213,19 @@ __global__ __launch_bounds__(BLOCK) void ln_rows_fwd(const T* __restrict__ x, co
     __shared__ float red[LPR > 64 ? 2 * (BLOCK / 64) : 1];
     const int lane = threadIdx.x % LPR, sub = threadIdx.x / LPR;
     const float fc = (float)C;
+    const bool even = C % V == 0;
     const long stride = (long)gridDim.x * RPB;
     long r = (long)blockIdx.x * RPB + sub;
     constexpr bool AHEAD = LPR < 1024;
     Row<T, LPR, E> xv, ahead;
-    if constexpr (AHEAD) xv.load(x + (r < rows ? r : 0) * x_stride, lane, C);
+    if constexpr (AHEAD) xv.load(x + (r < rows ? r : 0) * x_stride, lane, C, even);
     float wv[E], bv[E];
     row_params<T, LPR, E>(w, w_f32, lane, C, 1.0f, wv);
     row_params<T, LPR, E>(b, w_f32, lane, C, 0.0f, bv);
     // every lane of a workgroup runs the same number of rounds: the sums above one wavefront hold barriers
     for (long r0 = (long)blockIdx.x * RPB; r0 < rows; r0 += stride, r += stride) {
-        if constexpr (!AHEAD) xv.load(x + (r < rows ? r : 0) * x_stride, lane, C);
-        else if (r0 + stride < rows) ahead.load(x + (r + stride < rows ? r + stride : 0) * x_stride, lane, C);
+        if constexpr (!AHEAD) xv.load(x + (r < rows ? r : 0) * x_stride, lane, C, even);
+        else if (r0 + stride < rows) ahead.load(x + (r + stride < rows ? r + stride : 0) * x_stride, lane, C, even);
         float s = 0.0f;
 #pragma unroll
         for (int k = 0; k < NV; ++k)
@@ -208,21 +244,15 @@ __global__ __launch_bounds__(BLOCK) void ln_rows_fwd(const T* __restrict__ x, co
         }
         const float rs = 1.0f / sqrtf(group_sum<LPR, BLOCK>(s, red, 1) / fc + eps);
         if (r < rows) {
-            T* yr = y + r * C;
 #pragma unroll
-            for (int k = 0; k < NV; ++k) {
-                const int c0 = (lane + k * LPR) * V;
-                if (c0 < C) {
-                    Vec<T, V> o;
+            for (int k = 0; k < NV; ++k)
 #pragma unroll
-                    for (int j = 0; j < V; ++j) {
-                        float v = fmaf(((float)xv.v[k].e[j] - mu) * rs, wv[k * V + j], bv[k * V + j]);
-                        if (relu) v = passes(v) ? v : 0.0f;
-                        o.e[j] = (T)v;
-                    }
-                    stv_n<T, V>(yr + c0, o, C - c0);
+                for (int j = 0; j < V; ++j) {
+                    float v = fmaf(((float)xv.v[k].e[j] - mu) * rs, wv[k * V + j], bv[k * V + j]);
+                    if (relu) v = passes(v) ? v : 0.0f;
+                    xv.v[k].e[j] = (T)v;
                 }
-            }
+            xv.store(y + r * C, lane, C, even);
             if (mean && lane == 0) {
                 mean[r] = mu;
                 rstd[r] = rs;
@@ -244,6 +274,7 @@ __global__ __launch_bounds__(BLOCK) void ln_rows_bwd(const T* __restrict__ dy, c
     __shared__ float cols[RPB > 1 ? BLOCK * E : 1];
     const int lane = threadIdx.x % LPR, sub = threadIdx.x / LPR;
     const float fc = (float)C;
+    const bool even = C % V == 0;
     const long stride = (long)gridDim.x * RPB;
     long r = (long)blockIdx.x * RPB + sub;
     constexpr bool AHEAD = LPR < 1024;
@@ -251,8 +282,8 @@ __global__ __launch_bounds__(BLOCK) void ln_rows_bwd(const T* __restrict__ dy, c
     float mu = 0.0f, rs = 0.0f;
     const auto load = [&](long r, Row<T, LPR, E>& xr, Row<T, LPR, E>& gr, float& m, float& s) {
         r = r < rows ? r : 0;
-        xr.load(x + r * x_stride, lane, C);
-        gr.load(dy + r * dy_stride, lane, C);
+        xr.load(x + r * x_stride, lane, C, even);
+        gr.load(dy + r * dy_stride, lane, C, even);
         m = mean[r];
         s = rstd[r];
     };
@@ -293,23 +324,18 @@ __global__ __launch_bounds__(BLOCK) void ln_rows_bwd(const T* __restrict__ dy, c
                 }
             }
         }
-        const float m1 = group_sum<LPR, BLOCK>(s1, red, 2 * turn) / fc;
-        const float m2 = group_sum<LPR, BLOCK>(s2, red, 2 * turn + 1) / fc;
+        float both[2] = {s1, s2};
+        group_sums<LPR, BLOCK>(both, red, turn);
+        const float m1 = both[0] / fc, m2 = both[1] / fc;
         if (live && dx) {
-            T* dr = dx + r * C;
 #pragma unroll
-            for (int k = 0; k < NV; ++k) {
-                const int c0 = (lane + k * LPR) * V;
-                if (c0 < C) {
-                    Vec<T, V> o;
+            for (int k = 0; k < NV; ++k)
 #pragma unroll
-                    for (int j = 0; j < V; ++j) {
-                        const float h = ((float)xv.v[k].e[j] - mu) * rs;
-                        o.e[j] = (T)(rs * (fmaf((float)gv.v[k].e[j], wv[k * V + j], -m1) - h * m2));
-                    }
-                    stv_n<T, V>(dr + c0, o, C - c0);
+                for (int j = 0; j < V; ++j) {
+                    const float h = ((float)xv.v[k].e[j] - mu) * rs;
+                    xv.v[k].e[j] = (T)(rs * (fmaf((float)gv.v[k].e[j], wv[k * V + j], -m1) - h * m2));
                 }
-            }
+            xv.store(dx + r * C, lane, C, even);
         }
         if constexpr (AHEAD) {
             xv = next_x;
@@ -381,6 +407,53 @@ __device__ __forceinline__ void channel_sums(float (&s)[V], float* red) {
     }
 }
 
+// A lane's channels at n of V positions (n < V: the end of a plane).  A branch around a load of 16-bit values makes its wait
+// part of the branch, one load after the other: there one branch goes around all of them, and channels behind the last
+// read the first and are put away (32 x 64 x 65536 bf16: forward 152 -> 120 us, backward 271 -> 208).  fp32 values arrive in
+// the registers that hold them and are faster with a branch each (224 against 235 us), or, backward with 8 channels a lane,
+// with one branch around all and one per channel (322 against 332 and 353).
+template <typename T, int V, int CL, int E, bool BWD>
+__device__ __forceinline__ void plane_load(const T* p, int cg, int C, long inner, int n, Vec<T, V> (&to)[E]) {
+    if constexpr (sizeof(T) == 4 && !(BWD && E == 8)) {
+#pragma unroll
+        for (int k = 0; k < E; ++k) {
+            const int c = cg + k * CL;
+            to[k] = ldv_n<T, V>(p + (c < C ? c : 0) * inner, c < C ? n : 0);
+        }
+        return;
+    }
+    if (n >= V) {
+#pragma unroll
+        for (int k = 0; k < E; ++k) {
+            const int c = cg + k * CL;
+            to[k] = Vec<T, V>{};
+            if (sizeof(T) == 2 || c < C) to[k] = ldv<T, V>(p + (c < C ? c : 0) * inner);
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < E; ++k) {
+            const int c = cg + k * CL;
+            to[k] = ldv_n<T, V>(p + (c < C ? c : 0) * inner, c < C ? n : 0);
+        }
+    }
+    if (sizeof(T) == 2 && C < CL * E)
+#pragma unroll
+        for (int k = 0; k < E; ++k)
+            if (cg + k * CL >= C) to[k] = Vec<T, V>{};
+}
+template <typename T, int V, int CL, int E>
+__device__ __forceinline__ void plane_store(T* p, int cg, int C, long inner, int n, const Vec<T, V> (&v)[E]) {
+    if (sizeof(T) == 2 && n >= V) {
+#pragma unroll
+        for (int k = 0; k < E; ++k)
+            if (cg + k * CL < C) stv<T, V>(p + (cg + k * CL) * inner, v[k]);
+    } else {
+#pragma unroll
+        for (int k = 0; k < E; ++k)
+            if (cg + k * CL < C) stv_n<T, V>(p + (cg + k * CL) * inner, v[k], n);
+    }
+}
+
 template <typename T, int V, int CL, int PL, int E>
 __global__ __launch_bounds__(CL* PL) void ln_planes_fwd(const T* __restrict__ x, const void* __restrict__ w, const void* __restrict__ b, bool w_f32, unsigned nq, unsigned nvec, int C,
                                                         long inner, long x_stride, float eps, int relu, T* __restrict__ y,
@@ -403,11 +476,7 @@ __global__ __launch_bounds__(CL* PL) void ln_planes_fwd(const T* __restrict__ x,
         const int n = live ? (int)(inner - p < V ? inner - p : V) : 0;
         const T* xp = x + (long)img * x_stride + p;
         Vec<T, V> xv[E];
-#pragma unroll
-        for (int k = 0; k < E; ++k) {
-            const int c = cg + k * CL;
-            xv[k] = ldv_n<T, V>(xp + (c < C ? c : 0) * inner, c < C ? n : 0);
-        }
+        plane_load<T, V, CL, E, false>(xp, cg, C, inner, n, xv);
         float mu[V], rs[V];
 #pragma unroll
         for (int v = 0; v < V; ++v) {
@@ -429,21 +498,15 @@ __global__ __launch_bounds__(CL* PL) void ln_planes_fwd(const T* __restrict__ x,
         channel_sums<CL, PL, V>(rs, red);
 #pragma unroll
         for (int v = 0; v < V; ++v) rs[v] = 1.0f / sqrtf(rs[v] / fc + eps);
-        T* yp = y + (long)img * inner * C + p;
 #pragma unroll
-        for (int k = 0; k < E; ++k) {
-            const int c = cg + k * CL;
-            if (c < C) {
-                Vec<T, V> o;
+        for (int k = 0; k < E; ++k)
 #pragma unroll
-                for (int v = 0; v < V; ++v) {
-                    float a = fmaf(((float)xv[k].e[v] - mu[v]) * rs[v], wv[k], bv[k]);
-                    if (relu) a = passes(a) ? a : 0.0f;
-                    o.e[v] = (T)a;
-                }
-                stv_n<T, V>(yp + c * inner, o, n);
+            for (int v = 0; v < V; ++v) {
+                float a = fmaf(((float)xv[k].e[v] - mu[v]) * rs[v], wv[k], bv[k]);
+                if (relu) a = passes(a) ? a : 0.0f;
+                xv[k].e[v] = (T)a;
             }
-        }
+        plane_store<T, V, CL, E>(y + (long)img * inner * C + p, cg, C, inner, n, xv);
         if (mean && cg == 0) {
 #pragma unroll
             for (int v = 0; v < V; ++v)
@@ -462,7 +525,7 @@ __global__ __launch_bounds__(CL* PL) void ln_planes_bwd(const T* __restrict__ dy
                                                         unsigned nq, unsigned nvec, int C, long inner, long dy_stride,
                                                         long x_stride, int relu, T* __restrict__ dx,
                                                         float* __restrict__ partial) {
-    __shared__ float red[CL > 1 ? channel_groups<CL, PL>() * PL * V : 1];
+    __shared__ float red[CL > 1 ? channel_groups<CL, PL>() * PL * 2 * V : 1];
     __shared__ float wave_part[PL > 64 ? CL * (PL / 64) * E : 1];
     const int pl = threadIdx.x % PL, cg = threadIdx.x / PL;
     const float fc = (float)C;
@@ -483,20 +546,16 @@ __global__ __launch_bounds__(CL* PL) void ln_planes_bwd(const T* __restrict__ dy
         const T* xp = x + (long)img * x_stride + p;
         const T* gp = dy + (long)img * dy_stride + p;
         Vec<T, V> xv[E], gv[E];
-#pragma unroll
-        for (int k = 0; k < E; ++k) {
-            const int c = cg + k * CL;
-            xv[k] = ldv_n<T, V>(xp + (c < C ? c : 0) * inner, c < C ? n : 0);
-            gv[k] = ldv_n<T, V>(gp + (c < C ? c : 0) * inner, c < C ? n : 0);
-        }
-        float mu[V], rs[V], s1[V], s2[V];
+        plane_load<T, V, CL, E, true>(xp, cg, C, inner, n, xv);
+        plane_load<T, V, CL, E, true>(gp, cg, C, inner, n, gv);
+        float mu[V], rs[V], sums[2 * V];                      // of g w, then of g w h
 #pragma unroll
         for (int v = 0; v < V; ++v) {
             const long at = (long)img * inner + p + (v < n ? v : 0);
             mu[v] = mean[at];
             rs[v] = rstd[at];
-            s1[v] = 0.0f;
-            s2[v] = 0.0f;
+            sums[v] = 0.0f;
+            sums[V + v] = 0.0f;
         }
 #pragma unroll
         for (int k = 0; k < E; ++k) {
@@ -512,35 +571,25 @@ __global__ __launch_bounds__(CL* PL) void ln_planes_bwd(const T* __restrict__ dy
                 }
                 if (on && v < n) {
                     const float gw = g * wv[k];
-                    s1[v] += gw;
-                    s2[v] = fmaf(gw, h, s2[v]);
+                    sums[v] += gw;
+                    sums[V + v] = fmaf(gw, h, sums[V + v]);
                     aw[k] = fmaf(g, h, aw[k]);
                     ab[k] += g;
                 }
             }
         }
-        channel_sums<CL, PL, V>(s1, red);
-        channel_sums<CL, PL, V>(s2, red);
+        channel_sums<CL, PL, 2 * V>(sums, red);
         if (dx) {
-            T* dp = dx + (long)img * inner * C + p;
 #pragma unroll
-            for (int v = 0; v < V; ++v) {
-                s1[v] /= fc;
-                s2[v] /= fc;
-            }
+            for (int v = 0; v < 2 * V; ++v) sums[v] /= fc;
 #pragma unroll
-            for (int k = 0; k < E; ++k) {
-                const int c = cg + k * CL;
-                if (c < C) {
-                    Vec<T, V> o;
+            for (int k = 0; k < E; ++k)
 #pragma unroll
-                    for (int v = 0; v < V; ++v) {
-                        const float h = ((float)xv[k].e[v] - mu[v]) * rs[v];
-                        o.e[v] = (T)(rs[v] * (fmaf((float)gv[k].e[v], wv[k], -s1[v]) - h * s2[v]));
-                    }
-                    stv_n<T, V>(dp + c * inner, o, n);
+                for (int v = 0; v < V; ++v) {
+                    const float h = ((float)xv[k].e[v] - mu[v]) * rs[v];
+                    xv[k].e[v] = (T)(rs[v] * (fmaf((float)gv[k].e[v], wv[k], -sums[v]) - h * sums[V + v]));
                 }
-            }
+            plane_store<T, V, CL, E>(dx + (long)img * inner * C + p, cg, C, inner, n, xv);
         }
     }
     if (!partial) return;
@@ -745,46 +794,70 @@ constexpr int kPlanesMax = 1024;                  // planes: 128 channel groups 
 
 // Workgroups of a launch that loops over its positions.  A backward launch leaves one row of partial sums per
 // workgroup, which the second launch reads: no more of them than the compute units hold at a time.
-constexpr long kRowsFwd = 1280, kRowsBwd = 768, kPlanesFwd = 1024, kPlanesBwd = 512, kLong = 4096;
+constexpr long kRowsFwd = 1280, kRowsBwd = 512, kPlanesFwd = 1024, kPlanesBwd = 512, kLong = 4096;
 
 struct Plan {
     bool rows, wide;      // wide: vectors along the positions (planes)
     bool fits;            // the register kernels hold a position's channels
-    int lpr;              // rows: lanes per row
-    int cl, pl;           // planes: channel groups, positions (or vectors of positions) side by side
-    long units;           // workgroups that the positions fill once
+    int lanes;            // rows: lanes per row; planes: channel groups
+    int beside;           // rows, positions or vectors of positions of one workgroup
+    int each;             // values (rows) or channels (planes) of a lane
+    long units, most;     // workgroups that the positions fill once, and of a launch
 };
 
 int elem_size(int type) { return type == FC3D_F32 ? 4 : 2; }
 
-Plan plan_of(int64_t outer, int64_t C, int64_t inner) {
+// What a lane holds and how many lanes share a position.  Rows, forward: 16 values a lane.  Rows, backward: 8, so that four
+// or five wavefronts a SIMD hide each other's waits instead of three (16384 x 2048 bf16 54 -> 49 us, 8192 x 4096 87 -> 56);
+// beyond 8192 values a lane has to take 16.  Planes, forward: 8 channels.  Planes, backward, the fastest of 4 and 8
+// channels a lane and of 128 to 1024 lanes: 16-bit images of 64 channels 395 us with 8, 271 with 4 (537 MB of values; its
+// registers are conversions'); fp32 332 and 356; fp32 of 512 channels 47 with 8, 46 with 4 on twice the lanes.
+Plan plan_of(bool fwd, int type, int64_t outer, int64_t C, int64_t inner) {
     Plan p = {};
     p.rows = inner == 1;
+    const auto take = [&](int lanes, int beside, int each, long most) {
+        p.lanes = lanes;
+        p.beside = beside;
+        p.each = each;
+        p.most = most;
+    };
     if (p.rows) {
         p.fits = C <= kRowsMax;
-        p.lpr = C <= 128 ? 8 : C <= 512 ? 32 : C <= 1024 ? 64 : C <= 2048 ? 128 : C <= 4096 ? 256 : 1024;
-        const int rpb = p.lpr < 256 ? 256 / p.lpr : 1;
-        p.units = p.fits ? (outer + rpb - 1) / rpb : outer;
+        const int block = fwd ? 256 : 512;
+        if (C <= 64) take(8, block / 8, 8, 0);
+        else if (C > 4096) take(1024, 1, C <= 8192 ? 8 : 16, 0);
+        else {
+            int lanes = fwd ? 8 : 16;
+            while (lanes * (fwd ? 16 : 8) < C) lanes *= 2;
+            take(lanes, block / lanes, fwd ? 16 : 8, 0);
+        }
+        p.most = fwd ? kRowsFwd : kRowsBwd;
+        p.units = p.fits ? (outer + p.beside - 1) / p.beside : outer;
     } else {
         p.fits = C <= kPlanesMax;
         // a plane that is no multiple of the vector leaves part of its last vector empty: single values where that
         // would idle a quarter of the lanes
         const int64_t nv = (inner + kVec - 1) / kVec;
         p.wide = inner * 4 >= nv * kVec * 3;
-        p.cl = C <= 8 ? 1 : C <= 32 ? 4 : C <= 64 ? 8 : C <= 128 ? 16 : C <= 256 ? 32 : C <= 512 ? 64 : 128;
-        p.pl = p.cl <= 32 ? 256 / p.cl : p.cl == 64 ? 8 : 4;
+        if (fwd) {
+            const int cl = C <= 8 ? 1 : C <= 32 ? 4 : C <= 64 ? 8 : C <= 128 ? 16 : C <= 256 ? 32 : C <= 512 ? 64 : 128;
+            take(cl, cl <= 32 ? 256 / cl : cl == 64 ? 8 : 4, 8, kPlanesFwd);
+        } else if (C <= 32) take(C <= 8 ? 2 : 8, C <= 8 ? 128 : 32, 4, 2 * kPlanesBwd);
+        else if (C <= 64) type == FC3D_F32 ? take(8, 32, 8, kPlanesBwd) : take(16, 16, 4, 2 * kPlanesBwd);
+        else if (C <= 128) type == FC3D_F32 ? take(32, 16, 4, kPlanesBwd) : take(32, 8, 4, 2 * kPlanesBwd);
+        else if (C <= 256) take(64, 8, 4, kPlanesBwd);
+        else if (C <= 512) type == FC3D_F32 ? take(128, 8, 4, kPlanesBwd) : take(64, 8, 8, kPlanesBwd);
+        else take(128, 4, 8, kPlanesBwd);
         const int64_t nq = p.wide ? outer * nv : outer * inner;
-        p.units = p.fits ? (nq + p.pl - 1) / p.pl : (outer * inner + kLongPos - 1) / kLongPos;
+        p.units = p.fits ? (nq + p.beside - 1) / p.beside : (outer * inner + kLongPos - 1) / kLongPos;
     }
+    if (!p.fits) p.most = kLong;
     return p;
 }
 
-unsigned groups_of(const Plan& p, bool fwd) {
-    const long most = !p.fits ? kLong : p.rows ? (fwd ? kRowsFwd : kRowsBwd) : fwd ? kPlanesFwd : kPlanesBwd;
-    return (unsigned)(p.units < most ? p.units : most);
-}
+unsigned groups_of(const Plan& p) { return (unsigned)(p.units < p.most ? p.units : p.most); }
 constexpr int kLongShares = 64;
-int64_t partials_of(const Plan& p) { return p.fits ? (int64_t)groups_of(p, false) : kLongShares; }
+int64_t partials_of(const Plan& p) { return p.fits ? (int64_t)groups_of(p) : kLongShares; }      // of a backward plan
 
 int check_sizes(int x_type, int w_type, int64_t outer, int64_t C, int64_t inner) {
     if (x_type < FC3D_F32 || x_type > FC3D_F16) return FC3D_EINVAL;
@@ -831,51 +904,92 @@ int rows_launch(const BwdArgs& a, unsigned groups) {
                 (long)a.x_stride, a.relu, (T*)a.dx, a.partial);
     return FC3D_OK;
 }
-template <typename T, int V, int CL, int PL>
+template <typename T, int V, int CL, int PL, int E>
 int planes_launch(const FwdArgs& a, unsigned groups) {
     const unsigned nvec = (unsigned)((a.inner + V - 1) / V), nq = (unsigned)(a.outer * nvec);
-    FC3D_LAUNCH("layer_norm_fwd", (ln_planes_fwd<T, V, CL, PL, 8>), dim3(groups), dim3(CL * PL), 0, a.s, (const T*)a.x, a.w,
+    FC3D_LAUNCH("layer_norm_fwd", (ln_planes_fwd<T, V, CL, PL, E>), dim3(groups), dim3(CL * PL), 0, a.s, (const T*)a.x, a.w,
                 a.b, a.w_f32, nq, nvec, (int)a.C, (long)a.inner, (long)a.x_stride, a.eps, a.relu, (T*)a.y, a.mean, a.rstd);
     return FC3D_OK;
 }
-template <typename T, int V, int CL, int PL>
+template <typename T, int V, int CL, int PL, int E>
 int planes_launch(const BwdArgs& a, unsigned groups) {
     const unsigned nvec = (unsigned)((a.inner + V - 1) / V), nq = (unsigned)(a.outer * nvec);
-    FC3D_LAUNCH("layer_norm_bwd", (ln_planes_bwd<T, V, CL, PL, 8>), dim3(groups), dim3(CL * PL), 0, a.s, (const T*)a.dy,
+    FC3D_LAUNCH("layer_norm_bwd", (ln_planes_bwd<T, V, CL, PL, E>), dim3(groups), dim3(CL * PL), 0, a.s, (const T*)a.dy,
                 (const T*)a.x, a.w, a.b, a.w_f32, a.mean, a.rstd, nq, nvec, (int)a.C, (long)a.inner, (long)a.dy_stride,
                 (long)a.x_stride, a.relu, (T*)a.dx, a.partial);
     return FC3D_OK;
 }
-template <typename T, int V, typename A>
-int planes_of(const A& a, const Plan& p, unsigned groups) {
-    switch (p.cl) {
-        case 1: return planes_launch<T, V, 1, 256>(a, groups);
-        case 4: return planes_launch<T, V, 4, 64>(a, groups);
-        case 8: return planes_launch<T, V, 8, 32>(a, groups);
-        case 16: return planes_launch<T, V, 16, 16>(a, groups);
-        case 32: return planes_launch<T, V, 32, 8>(a, groups);
-        case 64: return planes_launch<T, V, 64, 8>(a, groups);
-        default: return planes_launch<T, V, 128, 4>(a, groups);
+template <typename T, int V>
+int planes_of(const FwdArgs& a, const Plan& p, unsigned groups) {
+    switch (p.lanes) {
+        case 1: return planes_launch<T, V, 1, 256, 8>(a, groups);
+        case 4: return planes_launch<T, V, 4, 64, 8>(a, groups);
+        case 8: return planes_launch<T, V, 8, 32, 8>(a, groups);
+        case 16: return planes_launch<T, V, 16, 16, 8>(a, groups);
+        case 32: return planes_launch<T, V, 32, 8, 8>(a, groups);
+        case 64: return planes_launch<T, V, 64, 8, 8>(a, groups);
+        default: return planes_launch<T, V, 128, 4, 8>(a, groups);
+    }
+}
+template <typename T, int V>
+int planes_of(const BwdArgs& a, const Plan& p, unsigned groups) {
+    constexpr bool F32 = sizeof(T) == 4;
+    switch (p.lanes) {
+        case 2: return planes_launch<T, V, 2, 128, 4>(a, groups);
+        case 8:
+            if constexpr (F32)
+                if (p.each == 8) return planes_launch<T, V, 8, 32, 8>(a, groups);
+            return planes_launch<T, V, 8, 32, 4>(a, groups);
+        case 16:
+            if constexpr (!F32) return planes_launch<T, V, 16, 16, 4>(a, groups);
+            return FC3D_EINVAL;                               // (no plan of fp32)
+        case 32: return planes_launch<T, V, 32, F32 ? 16 : 8, 4>(a, groups);
+        case 64:
+            if constexpr (!F32)
+                if (p.each == 8) return planes_launch<T, V, 64, 8, 8>(a, groups);
+            return planes_launch<T, V, 64, 8, 4>(a, groups);
+        default:
+            if constexpr (F32)
+                if (p.each == 4) return planes_launch<T, V, 128, 8, 4>(a, groups);
+            return planes_launch<T, V, 128, 4, 8>(a, groups);
+    }
+}
+template <typename T>
+int rows_of(const FwdArgs& a, const Plan& p, unsigned groups) {
+    switch (p.lanes) {
+        case 8: return p.each == 8 ? rows_launch<T, 8, 256, 8>(a, groups) : rows_launch<T, 8, 256, 16>(a, groups);
+        case 16: return rows_launch<T, 16, 256, 16>(a, groups);
+        case 32: return rows_launch<T, 32, 256, 16>(a, groups);
+        case 64: return rows_launch<T, 64, 256, 16>(a, groups);
+        case 128: return rows_launch<T, 128, 256, 16>(a, groups);
+        case 256: return rows_launch<T, 256, 256, 16>(a, groups);
+        default: return p.each == 8 ? rows_launch<T, 1024, 1024, 8>(a, groups) : rows_launch<T, 1024, 1024, 16>(a, groups);
+    }
+}
+template <typename T>
+int rows_of(const BwdArgs& a, const Plan& p, unsigned groups) {
+    switch (p.lanes) {
+        case 8: return rows_launch<T, 8, 512, 8>(a, groups);
+        case 16: return rows_launch<T, 16, 512, 8>(a, groups);
+        case 32: return rows_launch<T, 32, 512, 8>(a, groups);
+        case 64: return rows_launch<T, 64, 512, 8>(a, groups);
+        case 128: return rows_launch<T, 128, 512, 8>(a, groups);
+        case 256: return rows_launch<T, 256, 512, 8>(a, groups);
+        case 512: return rows_launch<T, 512, 512, 8>(a, groups);
+        default: return p.each == 8 ? rows_launch<T, 1024, 1024, 8>(a, groups) : rows_launch<T, 1024, 1024, 16>(a, groups);
     }
 }
 // The register kernel of a plan, forward or backward by the arguments' type
 template <typename T, typename A>
 int registers_of(const A& a, const Plan& p) {
-    const unsigned groups = groups_of(p, std::is_same<A, FwdArgs>::value);
-    if (!p.rows) return p.wide ? planes_of<T, kVec>(a, p, groups) : planes_of<T, 1>(a, p, groups);
-    switch (p.lpr) {
-        case 8: return rows_launch<T, 8, 256, 16>(a, groups);
-        case 32: return rows_launch<T, 32, 256, 16>(a, groups);
-        case 64: return rows_launch<T, 64, 256, 16>(a, groups);
-        case 128: return rows_launch<T, 128, 256, 16>(a, groups);
-        case 256: return rows_launch<T, 256, 256, 16>(a, groups);
-        default: return rows_launch<T, 1024, 1024, 16>(a, groups);
-    }
+    const unsigned groups = groups_of(p);
+    if (p.rows) return rows_of<T>(a, p, groups);
+    return p.wide ? planes_of<T, kVec>(a, p, groups) : planes_of<T, 1>(a, p, groups);
 }
 
 template <typename T, bool PLANES>
 int long_of(const FwdArgs& a, const Plan& p) {
-    FC3D_LAUNCH("layer_norm_fwd", (ln_long_fwd<T, PLANES>), dim3(groups_of(p, true)), dim3(kLongBlock), 0, a.s, (const T*)a.x, a.w,
+    FC3D_LAUNCH("layer_norm_fwd", (ln_long_fwd<T, PLANES>), dim3(groups_of(p)), dim3(kLongBlock), 0, a.s, (const T*)a.x, a.w,
                 a.b, a.w_f32, (long)(a.outer * a.inner), (long)a.C, (long)a.inner, (long)a.x_stride, a.eps, a.relu, (T*)a.y,
                 a.mean, a.rstd);
     return FC3D_OK;
@@ -885,7 +999,7 @@ int long_of(const BwdArgs& a, const Plan& p) {
     const T *dy = (const T*)a.dy, *x = (const T*)a.x;
     const long positions = (long)(a.outer * a.inner);
     if (a.dx)
-        FC3D_LAUNCH("layer_norm_bwd", (ln_long_bwd<T, PLANES>), dim3(groups_of(p, false)), dim3(kLongBlock), 0, a.s, dy, x, a.w, a.b,
+        FC3D_LAUNCH("layer_norm_bwd", (ln_long_bwd<T, PLANES>), dim3(groups_of(p)), dim3(kLongBlock), 0, a.s, dy, x, a.w, a.b,
                     a.w_f32, a.mean, a.rstd, positions, (long)a.C, (long)a.inner, (long)a.dy_stride, (long)a.x_stride,
                     a.relu, (T*)a.dx);
     if (a.partial)
@@ -931,12 +1045,12 @@ extern "C" int fc3d_layer_norm_fwd(void* stream, const void* x, int x_type, cons
         return FC3D_EALIGN;
     const FwdArgs a = {(hipStream_t)stream, x, weight, bias, w_type == FC3D_F32, outer, channels, inner, x_stride, eps, relu,
                        y, mean, rstd};
-    return type_of(a, plan_of(outer, channels, inner), x_type);
+    return type_of(a, plan_of(true, x_type, outer, channels, inner), x_type);
 }
 
 extern "C" size_t fc3d_layer_norm_bwd_workspace(int x_type, int64_t outer, int64_t channels, int64_t inner) {
     if (check_sizes(x_type, x_type, outer, channels, inner) != FC3D_OK || outer == 0) return 0;
-    return (size_t)partials_of(plan_of(outer, channels, inner)) * 2 * (size_t)channels * sizeof(float);
+    return (size_t)partials_of(plan_of(false, x_type, outer, channels, inner)) * 2 * (size_t)channels * sizeof(float);
 }
 
 extern "C" int fc3d_layer_norm_bwd(void* stream, const void* dy, const void* x, int x_type, const void* weight,
@@ -959,7 +1073,7 @@ extern "C" int fc3d_layer_norm_bwd(void* stream, const void* dy, const void* x, 
         return FC3D_EALIGN;
     const BwdArgs a = {(hipStream_t)stream, dy, x, weight, bias, w_type == FC3D_F32, mean, rstd, outer, channels, inner,
                        dy_stride, x_stride, relu, dx, dw || db ? (float*)workspace : nullptr};
-    const Plan p = plan_of(outer, channels, inner);
+    const Plan p = plan_of(false, x_type, outer, channels, inner);
     const int rc = type_of(a, p, x_type);
     if (rc != FC3D_OK || !a.partial) return rc;
     FC3D_LAUNCH("layer_norm_params_sum", ln_params_sum, dim3((unsigned)((2 * channels + 31) / 32)), dim3(1024), 0, a.s,
