@@ -92,6 +92,18 @@ __device__ __forceinline__ void stv_n(T* p, const Vec<T, V>& v, int n) {
         if (j < n) p[j] = v.e[j];
 }
 
+// The same 16 bytes, of which the compiler knows nothing: what it has computed from them before does not count
+template <typename T, int V>
+__device__ __forceinline__ Vec<T, V> unknown(const Vec<T, V>& v) {
+    typedef uint32_t word __attribute__((ext_vector_type(sizeof(v) / 4)));
+    word w;
+    __builtin_memcpy(&w, &v, sizeof(v));
+    asm volatile("" : "+v"(w));
+    Vec<T, V> r;
+    __builtin_memcpy(&r, &w, sizeof(v));
+    return r;
+}
+
 // A weight or bias: fp32 or the activations' 16-bit type (the same branch in every lane), `absent` without one
 template <typename T>
 __device__ __forceinline__ float param(const void* p, bool f32, long i, float absent) {
@@ -216,7 +228,7 @@ __global__ __launch_bounds__(BLOCK) void ln_rows_fwd(const T* __restrict__ x, co
     const bool even = C % V == 0;
     const long stride = (long)gridDim.x * RPB;
     long r = (long)blockIdx.x * RPB + sub;
-    constexpr bool AHEAD = LPR < 1024;
+    constexpr bool AHEAD = LPR < 1024 && LPR * E < 16384;
     Row<T, LPR, E> xv, ahead;
     if constexpr (AHEAD) xv.load(x + (r < rows ? r : 0) * x_stride, lane, C, even);
     float wv[E], bv[E];
@@ -277,7 +289,7 @@ __global__ __launch_bounds__(BLOCK) void ln_rows_bwd(const T* __restrict__ dy, c
     const bool even = C % V == 0;
     const long stride = (long)gridDim.x * RPB;
     long r = (long)blockIdx.x * RPB + sub;
-    constexpr bool AHEAD = LPR < 1024;
+    constexpr bool AHEAD = LPR < 1024 && LPR * E < 16384;
     Row<T, LPR, E> xv, gv, next_x, next_g;
     float mu = 0.0f, rs = 0.0f;
     const auto load = [&](long r, Row<T, LPR, E>& xr, Row<T, LPR, E>& gr, float& m, float& s) {
@@ -327,6 +339,13 @@ __global__ __launch_bounds__(BLOCK) void ln_rows_bwd(const T* __restrict__ dy, c
         float both[2] = {s1, s2};
         group_sums<LPR, BLOCK>(both, red, turn);
         const float m1 = both[0] / fc, m2 = both[1] / fc;
+        if constexpr (sizeof(T) == 2 && LPR * E >= 16384) {   // to be unpacked again below: kept as fp32 it would not fit
+#pragma unroll
+            for (int k = 0; k < NV; ++k) {
+                xv.v[k] = unknown(xv.v[k]);
+                gv.v[k] = unknown(gv.v[k]);
+            }
+        }
         if (live && dx) {
 #pragma unroll
             for (int k = 0; k < NV; ++k)
@@ -809,7 +828,8 @@ int elem_size(int type) { return type == FC3D_F32 ? 4 : 2; }
 
 // What a lane holds and how many lanes share a position.  Rows, forward: 16 values a lane.  Rows, backward: 8, so that four
 // or five wavefronts a SIMD hide each other's waits instead of three (16384 x 2048 bf16 54 -> 49 us, 8192 x 4096 87 -> 56);
-// beyond 8192 values a lane has to take 16.  Planes, forward: 8 channels.  Planes, backward, the fastest of 4 and 8
+// beyond 8192 values 512 lanes take 32, with twice the registers of 1024 lanes that take 16 (2048 x 16000 fp32 138 -> 116,
+// bf16 129 -> 100 us).  Planes, forward: 8 channels.  Planes, backward, the fastest of 4 and 8
 // channels a lane and of 128 to 1024 lanes: 16-bit images of 64 channels 395 us with 8, 271 with 4 (537 MB of values; its
 // registers are conversions'); fp32 332 and 356; fp32 of 512 channels 47 with 8, 46 with 4 on twice the lanes.
 Plan plan_of(bool fwd, int type, int64_t outer, int64_t C, int64_t inner) {
@@ -825,7 +845,8 @@ Plan plan_of(bool fwd, int type, int64_t outer, int64_t C, int64_t inner) {
         p.fits = C <= kRowsMax;
         const int block = fwd ? 256 : 512;
         if (C <= 64) take(8, block / 8, 8, 0);
-        else if (C > 4096) take(1024, 1, C <= 8192 ? 8 : 16, 0);
+        else if (C > 8192) take(fwd ? 1024 : 512, 1, fwd ? 16 : 32, 0);
+        else if (C > 4096) take(1024, 1, 8, 0);
         else {
             int lanes = fwd ? 8 : 16;
             while (lanes * (fwd ? 16 : 8) < C) lanes *= 2;
@@ -975,8 +996,8 @@ int rows_of(const BwdArgs& a, const Plan& p, unsigned groups) {
         case 64: return rows_launch<T, 64, 512, 8>(a, groups);
         case 128: return rows_launch<T, 128, 512, 8>(a, groups);
         case 256: return rows_launch<T, 256, 512, 8>(a, groups);
-        case 512: return rows_launch<T, 512, 512, 8>(a, groups);
-        default: return p.each == 8 ? rows_launch<T, 1024, 1024, 8>(a, groups) : rows_launch<T, 1024, 1024, 16>(a, groups);
+        case 512: return p.each == 8 ? rows_launch<T, 512, 512, 8>(a, groups) : rows_launch<T, 512, 512, 32>(a, groups);
+        default: return rows_launch<T, 1024, 1024, 8>(a, groups);
     }
 }
 // The register kernel of a plan, forward or backward by the arguments' type
