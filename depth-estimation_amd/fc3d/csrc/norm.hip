@@ -13,7 +13,7 @@
 // statistics are formed (mean first, then the squares of the differences: no cancellation), and written once.
 // Statistics, sums over positions and all arithmetic are 32 bits; a 16-bit result is rounded once, at its store.
 // Sums over positions are kept per workgroup, written as partial sums and added in a fixed order by a second,
-// small launch: no atomics, the same bits on every run.
+// small launch: no atomics, the same bits on every run.  A single workgroup's sums are the gradients.
 #include "fc3d_common.h"
 
 #include <type_traits>
@@ -274,13 +274,25 @@ __global__ __launch_bounds__(BLOCK) void ln_rows_fwd(const T* __restrict__ x, co
     }
 }
 
-// partial: [gridDim.x][2][C] sums of g h and of g over the workgroup's rows, or NULL when no parameter asks for them
+// Where a backward launch leaves its sums of g h and of g: [gridDim.x][2][C] partial sums, or, of a single workgroup, the
+// gradients themselves.
+struct Sums {
+    float* partial;
+    void *dw, *db;        // either may be NULL, both are when no parameter asks for a gradient
+    int type;
+    __host__ __device__ __forceinline__ bool wanted() const { return dw || db; }
+    __device__ __forceinline__ void put(int which, long C, long c, float v) const {
+        if (gridDim.x > 1) partial[((long)blockIdx.x * 2 + which) * C + c] = v;
+        else if (which ? db : dw) put_param(which ? db : dw, type, c, v);
+    }
+};
+
 template <typename T, int LPR, int BLOCK, int E>
 __global__ __launch_bounds__(BLOCK) void ln_rows_bwd(const T* __restrict__ dy, const T* __restrict__ x,
                                                      const void* __restrict__ w, const void* __restrict__ b, bool w_f32,
                                                      const float* __restrict__ mean, const float* __restrict__ rstd,
                                                      long rows, int C, long dy_stride, long x_stride, int relu,
-                                                     T* __restrict__ dx, float* __restrict__ partial) {
+                                                     T* __restrict__ dx, Sums sums) {
     constexpr int V = Row<T, LPR, E>::V, NV = E / V, RPB = BLOCK / LPR;
     __shared__ float red[LPR > 64 ? 4 * (BLOCK / 64) : 1];
     __shared__ float cols[RPB > 1 ? BLOCK * E : 1];
@@ -363,8 +375,7 @@ __global__ __launch_bounds__(BLOCK) void ln_rows_bwd(const T* __restrict__ dy, c
             rs = next_rs;
         }
     }
-    if (!partial) return;
-    float* pw = partial + (long)blockIdx.x * 2 * C;
+    if (!sums.wanted()) return;
 #pragma unroll
     for (int which = 0; which < 2; ++which) {
         float* a = which ? ab : aw;
@@ -378,7 +389,7 @@ __global__ __launch_bounds__(BLOCK) void ln_rows_bwd(const T* __restrict__ dy, c
 #pragma unroll 4
                 for (int q = 0; q < RPB; ++q) s += cols[q * E * LPR + t];
                 const int i = t / LPR, c = (t % LPR + (i / V) * LPR) * V + i % V;
-                if (c < C) pw[which * C + c] = s;
+                if (c < C) sums.put(which, C, c, s);
             }
         } else {
 #pragma unroll
@@ -386,7 +397,7 @@ __global__ __launch_bounds__(BLOCK) void ln_rows_bwd(const T* __restrict__ dy, c
                 const int c0 = (lane + k * LPR) * V;
 #pragma unroll
                 for (int j = 0; j < V; ++j)
-                    if (c0 + j < C) pw[which * C + c0 + j] = a[k * V + j];
+                    if (c0 + j < C) sums.put(which, C, c0 + j, a[k * V + j]);
             }
         }
     }
@@ -542,8 +553,7 @@ __global__ __launch_bounds__(CL* PL) void ln_planes_bwd(const T* __restrict__ dy
                                                         const void* __restrict__ w, const void* __restrict__ b, bool w_f32,
                                                         const float* __restrict__ mean, const float* __restrict__ rstd,
                                                         unsigned nq, unsigned nvec, int C, long inner, long dy_stride,
-                                                        long x_stride, int relu, T* __restrict__ dx,
-                                                        float* __restrict__ partial) {
+                                                        long x_stride, int relu, T* __restrict__ dx, Sums out) {
     __shared__ float red[CL > 1 ? channel_groups<CL, PL>() * PL * 2 * V : 1];
     __shared__ float wave_part[PL > 64 ? CL * (PL / 64) * E : 1];
     const int pl = threadIdx.x % PL, cg = threadIdx.x / PL;
@@ -611,8 +621,7 @@ __global__ __launch_bounds__(CL* PL) void ln_planes_bwd(const T* __restrict__ dy
             plane_store<T, V, CL, E>(dx + (long)img * inner * C + p, cg, C, inner, n, xv);
         }
     }
-    if (!partial) return;
-    float* pw = partial + (long)blockIdx.x * 2 * C;
+    if (!out.wanted()) return;
 #pragma unroll
     for (int which = 0; which < 2; ++which) {
         float* a = which ? ab : aw;
@@ -632,13 +641,13 @@ __global__ __launch_bounds__(CL* PL) void ln_planes_bwd(const T* __restrict__ dy
                 float s = 0.0f;
 #pragma unroll
                 for (int i = 0; i < NW; ++i) s += wave_part[(g * NW + i) * E + k];
-                if (c < C) pw[which * C + c] = s;
+                if (c < C) out.put(which, C, c, s);
             }
         } else {
             if (pl == 0)
 #pragma unroll
                 for (int k = 0; k < E; ++k)
-                    if (cg + k * CL < C) pw[which * C + cg + k * CL] = a[k];
+                    if (cg + k * CL < C) out.put(which, C, cg + k * CL, a[k]);
         }
     }
 }
@@ -879,6 +888,7 @@ Plan plan_of(bool fwd, int type, int64_t outer, int64_t C, int64_t inner) {
 unsigned groups_of(const Plan& p) { return (unsigned)(p.units < p.most ? p.units : p.most); }
 constexpr int kLongShares = 64;
 int64_t partials_of(const Plan& p) { return p.fits ? (int64_t)groups_of(p) : kLongShares; }      // of a backward plan
+bool direct(const Plan& p) { return p.fits && groups_of(p) == 1; }       // the sums are the gradients: no workspace
 
 int check_sizes(int x_type, int w_type, int64_t outer, int64_t C, int64_t inner) {
     if (x_type < FC3D_F32 || x_type > FC3D_F16) return FC3D_EINVAL;
@@ -909,7 +919,7 @@ struct BwdArgs {
     int64_t outer, C, inner, dy_stride, x_stride;
     int relu;
     void* dx;
-    float* partial;       // NULL: no parameter asks for a gradient
+    Sums sums;
 };
 
 template <typename T, int LPR, int BLOCK, int E>
@@ -922,7 +932,7 @@ template <typename T, int LPR, int BLOCK, int E>
 int rows_launch(const BwdArgs& a, unsigned groups) {
     FC3D_LAUNCH("layer_norm_bwd", (ln_rows_bwd<T, LPR, BLOCK, E>), dim3(groups), dim3(BLOCK), 0, a.s, (const T*)a.dy,
                 (const T*)a.x, a.w, a.b, a.w_f32, a.mean, a.rstd, (long)a.outer, (int)a.C, (long)a.dy_stride,
-                (long)a.x_stride, a.relu, (T*)a.dx, a.partial);
+                (long)a.x_stride, a.relu, (T*)a.dx, a.sums);
     return FC3D_OK;
 }
 template <typename T, int V, int CL, int PL, int E>
@@ -937,7 +947,7 @@ int planes_launch(const BwdArgs& a, unsigned groups) {
     const unsigned nvec = (unsigned)((a.inner + V - 1) / V), nq = (unsigned)(a.outer * nvec);
     FC3D_LAUNCH("layer_norm_bwd", (ln_planes_bwd<T, V, CL, PL, E>), dim3(groups), dim3(CL * PL), 0, a.s, (const T*)a.dy,
                 (const T*)a.x, a.w, a.b, a.w_f32, a.mean, a.rstd, nq, nvec, (int)a.C, (long)a.inner, (long)a.dy_stride,
-                (long)a.x_stride, a.relu, (T*)a.dx, a.partial);
+                (long)a.x_stride, a.relu, (T*)a.dx, a.sums);
     return FC3D_OK;
 }
 template <typename T, int V>
@@ -1023,11 +1033,11 @@ int long_of(const BwdArgs& a, const Plan& p) {
         FC3D_LAUNCH("layer_norm_bwd", (ln_long_bwd<T, PLANES>), dim3(groups_of(p)), dim3(kLongBlock), 0, a.s, dy, x, a.w, a.b,
                     a.w_f32, a.mean, a.rstd, positions, (long)a.C, (long)a.inner, (long)a.dy_stride, (long)a.x_stride,
                     a.relu, (T*)a.dx);
-    if (a.partial)
+    if (a.sums.wanted())
         FC3D_LAUNCH("layer_norm_params", (ln_long_params<T, PLANES>),
                     dim3((unsigned)(PLANES ? a.C : (a.C + 255) / 256), kLongShares), dim3(256), 0, a.s, dy, x, a.w, a.b,
                     a.w_f32, a.mean, a.rstd, positions, (long)a.C, (long)a.inner, (long)a.dy_stride, (long)a.x_stride,
-                    a.relu, a.partial);
+                    a.relu, a.sums.partial);
     return FC3D_OK;
 }
 
@@ -1071,7 +1081,8 @@ extern "C" int fc3d_layer_norm_fwd(void* stream, const void* x, int x_type, cons
 
 extern "C" size_t fc3d_layer_norm_bwd_workspace(int x_type, int64_t outer, int64_t channels, int64_t inner) {
     if (check_sizes(x_type, x_type, outer, channels, inner) != FC3D_OK || outer == 0) return 0;
-    return (size_t)partials_of(plan_of(false, x_type, outer, channels, inner)) * 2 * (size_t)channels * sizeof(float);
+    const Plan p = plan_of(false, x_type, outer, channels, inner);
+    return direct(p) ? 0 : (size_t)partials_of(p) * 2 * (size_t)channels * sizeof(float);
 }
 
 extern "C" int fc3d_layer_norm_bwd(void* stream, const void* dy, const void* x, int x_type, const void* weight,
@@ -1087,17 +1098,17 @@ extern "C" int fc3d_layer_norm_bwd(void* stream, const void* dy, const void* x, 
                     (hipStream_t)stream, (long)channels, w_type, dw, db);
         return FC3D_OK;
     }
+    const Plan p = plan_of(false, x_type, outer, channels, inner);
     if (!dy || !x || !mean || !rstd || dy_stride < 0 || x_stride < 0 || ((dw || db) && !workspace)) return FC3D_EINVAL;
     if (!aligned_to(dy, elem_size(x_type)) || !aligned_to(x, elem_size(x_type)) || !aligned_to(dx, elem_size(x_type)) ||
         !aligned_to(weight, elem_size(w_type)) || !aligned_to(bias, elem_size(w_type)) || !aligned_to(mean, 4) ||
         !aligned_to(rstd, 4) || !aligned_to(workspace, 4))
         return FC3D_EALIGN;
     const BwdArgs a = {(hipStream_t)stream, dy, x, weight, bias, w_type == FC3D_F32, mean, rstd, outer, channels, inner,
-                       dy_stride, x_stride, relu, dx, dw || db ? (float*)workspace : nullptr};
-    const Plan p = plan_of(false, x_type, outer, channels, inner);
+                       dy_stride, x_stride, relu, dx, Sums{(float*)workspace, dw, db, w_type}};
     const int rc = type_of(a, p, x_type);
-    if (rc != FC3D_OK || !a.partial) return rc;
+    if (rc != FC3D_OK || !a.sums.wanted() || direct(p)) return rc;
     FC3D_LAUNCH("layer_norm_params_sum", ln_params_sum, dim3((unsigned)((2 * channels + 31) / 32)), dim3(1024), 0, a.s,
-                a.partial, (int)partials_of(p), (long)channels, w_type, dw, db);
+                a.sums.partial, (int)partials_of(p), (long)channels, w_type, dw, db);
     return FC3D_OK;
 }

@@ -1271,8 +1271,12 @@ class LayerNormFn(torch.autograd.Function):
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
+        # the wrapper that refuses second derivatives costs 5 us: only where a graph of the backward pass is made
+        return _norm_backward_once(ctx, dy) if torch.is_grad_enabled() else LayerNormFn.gradients(ctx, dy)
+
+    @staticmethod
+    def gradients(ctx, dy):
         xd, weight, bias, stats = ctx.saved_tensors
         dim, last, relu, outer, C, inner, x_step, code, p_code, dev = ctx.meta
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
@@ -1283,10 +1287,12 @@ class LayerNormFn(torch.autograd.Function):
         dx = _norm_out(dy, dim, last) if need_x else None
         dw = torch.empty_like(weight) if need_w else None
         db = torch.empty_like(bias) if need_b else None
-        ws = None
+        at = ws_at = stats.data_ptr()                            # (some pointer, where no workspace is needed)
         if need_w or need_b:
-            ws = torch.empty(_lib.fc3d_layer_norm_bwd_workspace(code, outer, C, inner), dtype=torch.uint8, device=xd.device)
-        at = stats.data_ptr()
+            nbytes = _lib.fc3d_layer_norm_bwd_workspace(code, outer, C, inner)
+            if nbytes:
+                ws = torch.empty(nbytes, dtype=torch.uint8, device=xd.device)
+                ws_at = ws.data_ptr()
         other = None if dev == _get_device() else _on_device(xd.device)
         if other is not None:
             other.__enter__()
@@ -1296,13 +1302,16 @@ class LayerNormFn(torch.autograd.Function):
                                               bias.data_ptr() if bias is not None else None, p_code, at,
                                               at + 4 * outer * inner, outer, C, inner, g_step, x_step, relu,
                                               dx.data_ptr() if need_x else None, dw.data_ptr() if need_w else None,
-                                              db.data_ptr() if need_b else None, ws.data_ptr() if ws is not None else None)
+                                              db.data_ptr() if need_b else None, ws_at)
         finally:
             if other is not None:
                 other.__exit__(None, None, None)
         if status:
             _check(status, "fc3d_layer_norm_bwd")
         return dx, dw, db, None, None, None
+
+
+_norm_backward_once = torch.autograd.function.once_differentiable(LayerNormFn.gradients)
 
 
 def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None,

@@ -452,8 +452,8 @@ int fc3d_layer_norm_fwd(void *stream, const void *x, int x_type, const void *wei
 
 /* Its backward pass.  dy has the layout of x with its own stride over the outer index; dx (dense),
  * dw, db ([channels] in w_type) may each be NULL.  workspace: fc3d_layer_norm_bwd_workspace()
- * bytes, 4-byte aligned, need not be initialised (NULL allowed without dw and db): partial sums per
- * workgroup, added in a fixed order (bit-reproducible).  relu != 0: dy passes where the
+ * bytes, 4-byte aligned, need not be initialised (NULL allowed without dw and db; any pointer where
+ * the size is 0): partial sums per workgroup, added in a fixed order (bit-reproducible).  relu != 0: dy passes where the
  * forward's value before the activation is not <= 0, recomputed from x.                      */
 size_t fc3d_layer_norm_bwd_workspace(int x_type, int64_t outer, int64_t channels, int64_t inner);
 int fc3d_layer_norm_bwd(void *stream, const void *dy, const void *x, int x_type, const void *weight, const void *bias,

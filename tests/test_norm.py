@@ -426,3 +426,46 @@ def test_offsets_beyond_32_bits():
     planes.copy_(x.cuda())
     r = formula(x, None, None, None, 1, 1e-5)
     close(ops.layer_norm(planes, dim=1), r["y"], r["ey"], BF16, "planes")
+
+
+@gpu
+def test_second_derivatives_are_refused():
+    from fc3d import ops
+    x = torch.randn(6, 20, device="cuda", requires_grad=True)
+    w = torch.randn(20, device="cuda", requires_grad=True)
+    y = ops.layer_norm(x, w)
+    first, = torch.autograd.grad(y.square().sum(), x, create_graph=True)        # the first derivative itself is there
+    plain, = torch.autograd.grad(ops.layer_norm(x, w).square().sum(), x)
+    assert torch.equal(first, plain)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(first.sum(), x)
+
+
+@gpu
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16, torch.float16], ids=lambda t: str(t).replace("torch.", ""))
+def test_gradients_of_one_workgroup(dt):
+    """Few rows or positions: the sums are written as gradients at once, in the parameters' type, one or both."""
+    from fc3d import ops
+    for shape, dim in (((5, 24), -1), ((1, 5000), -1), ((2, 1800), -1), ((2, 24, 3, 5), 1), ((1, 300, 2, 3), 1)):
+        C = shape[dim]
+        g = torch.Generator().manual_seed(C)
+        x, dy = (torch.randn(shape, generator=g).to(dt) for _ in range(2))
+        for pt in {dt, torch.float32}:
+            w, b = (torch.randn(C, generator=g).to(pt) for _ in range(2))
+            xr, wr, br = (t.double().requires_grad_() for t in (x, w, b))
+            ref = torch.nn.functional.layer_norm(xr.movedim(dim, -1), (C,), wr, br, 1e-5).movedim(-1, dim)
+            ref.backward(dy.double())
+            for need_w, need_b in ((True, True), (True, False), (False, True)):
+                xd, wd, bd = x.cuda().requires_grad_(), w.cuda().requires_grad_(need_w), b.cuda().requires_grad_(need_b)
+                ops.layer_norm(xd, wd, bd, dim=dim).backward(dy.cuda())
+                # a handful of terms each: sums of n <= 30 products in fp32 with h itself off by the norm's few half steps of
+                # a value up to sqrt(C), n + 16 half steps of sum |dy h|; then the rounding to the parameters' type
+                for t, r, need in ((wd, wr, need_w), (bd, br, need_b)):
+                    if not need:
+                        assert t.grad is None
+                        continue
+                    assert t.grad.dtype == pt
+                    n = x.numel() // C
+                    terms = (dy.double().abs() * (1 + x.double().abs())).movedim(dim, -1).reshape(-1, C).sum(0) * 4
+                    tol = (n + 16) * 2.0 ** -24 * terms + torch.finfo(pt).eps / 2 * r.grad.abs() + 1e-7
+                    assert bool(((t.grad.cpu().double() - r.grad).abs() <= tol).all()), (shape, dt, pt)
