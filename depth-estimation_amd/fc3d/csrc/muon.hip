@@ -629,24 +629,31 @@ __global__ __launch_bounds__(WAVES * 64, TILE == 64 && WAVES == 4 ? 2 : 1) void 
         with_type(a.out_type, [&](auto zero) {
             typedef decltype(zero) T;
             T* to = static_cast<T*>(e.out);
+            // A step reads the weights: all of a lane's first, without a branch of their own (behind the matrix its last
+            // row and column), which would wait for each.
             if (!e.tall) {                                    // along the tensor's rows as the lanes hold them
+                T old[BLK * BLK][OWN][4];
+                if (a.step)
+#pragma unroll
+                    for (int q = 0; q < BLK * BLK; ++q)
+#pragma unroll
+                        for (int k = 0; k < OWN; ++k)
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) {
+                                const int i = i0 + row_of(q, k) + r, j = j0 + col_of(q);
+                                old[q][k][r] = to[(size_t)(i < e.m ? i : e.m - 1) * e.n + (j < e.n ? j : e.n - 1)];
+                            }
 #pragma unroll
                 for (int q = 0; q < BLK * BLK; ++q)
 #pragma unroll
-                    for (int k = 0; k < OWN; ++k) {
-                        const int i = i0 + row_of(q, k), j = j0 + col_of(q);
-                        T* row = to + (size_t)i * e.n + j;
-                        float4v old = {};
-                        if (a.step)
-#pragma unroll
-                            for (int r = 0; r < 4; ++r) old[r] = i + r < e.m && j < e.n ? (float)row[(size_t)r * e.n] : 0.0f;
+                    for (int k = 0; k < OWN; ++k)
 #pragma unroll
                         for (int r = 0; r < 4; ++r) {
+                            const int i = i0 + row_of(q, k) + r, j = j0 + col_of(q);
                             float v = sum[q][k][r];
-                            if (a.step) v = fmaf(a.decay, old[r], -e.lr * v);
-                            if (i + r < e.m && j < e.n) row[(size_t)r * e.n] = (T)v;
+                            if (a.step) v = fmaf(a.decay, (float)old[q][k][r], -e.lr * v);
+                            if (i < e.m && j < e.n) to[(size_t)i * e.n + j] = (T)v;
                         }
-                    }
                 return;
             }
             __syncthreads();
@@ -655,14 +662,21 @@ __global__ __launch_bounds__(WAVES * 64, TILE == 64 && WAVES == 4 ? 2 : 1) void 
 #pragma unroll
                 for (int k = 0; k < OWN; ++k) *reinterpret_cast<float4v*>(out + col_of(q) * LD2 + row_of(q, k)) = sum[q][k];
             __syncthreads();
-#pragma unroll 8
-            for (int id = tid; id < TILE * TILE; id += THREADS) {
-                const int i = id % TILE, j = id / TILE;
-                if (i0 + i < e.m && j0 + j < e.n) {
-                    const size_t at = (size_t)(j0 + j) * e.m + i0 + i;
-                    float v = out[j * LD2 + i];
-                    if (a.step) v = fmaf(a.decay, (float)to[at], -e.lr * v);
-                    to[at] = (T)v;
+            constexpr int CHUNK = BLK == 3 ? 9 : 8;            // values of a lane in flight
+            for (int from = tid; from < TILE * TILE; from += CHUNK * THREADS) {
+                T old[CHUNK];
+                if (a.step)
+#pragma unroll
+                    for (int c = 0; c < CHUNK; ++c) {
+                        const int id = from + c * THREADS, i = i0 + id % TILE, j = j0 + id / TILE;
+                        old[c] = to[(size_t)(j < e.n ? j : e.n - 1) * e.m + (i < e.m ? i : e.m - 1)];
+                    }
+#pragma unroll
+                for (int c = 0; c < CHUNK; ++c) {
+                    const int id = from + c * THREADS, i = i0 + id % TILE, j = j0 + id / TILE;
+                    float v = out[(id / TILE) * LD2 + id % TILE];
+                    if (a.step) v = fmaf(a.decay, (float)old[c], -e.lr * v);
+                    if (i < e.m && j < e.n) to[(size_t)j * e.m + i] = (T)v;
                 }
             }
         });
@@ -1239,14 +1253,15 @@ struct Layout {
 // takes `fixed` microseconds (starting, finding the tile, the first operands, the result's way out) and slice[] for every
 // 64 of the depth, by the operands' planes (2 x 2, 2 x 1, 1 x 1); fitted to launches of 100 to 4000 tiles at depths of
 // 512 to 8192.  Two small workgroups per unit hide each other's waits best; 96 x 96 tiles fill one round where the small
-// ones need a second (2048 rows: 253 tiles, 41 us, against 50 us for 528); 128 x 128 tiles read least, for launches of many
-// rounds (2048 x 8192, P X: 165 us against 210) and matrices of 1024 rows (35 us against 42).
+// ones need a second (2048 rows: 253 tiles, 37 us, against 46 us for 528); 128 x 128 tiles read least, for launches of many
+// rounds of deep products (2048 x 8192, P X: 145 us against 191) and symmetric products of 1024 rows (32 us against 38);
+// small ones hide a step's last product, which reads and writes the weights (1024 rows: 112 us against 129).
 struct Kernel {
     int tile, waves, beside;
     double fixed, slice[3];
 };
 constexpr Kernel kKernels[] = {
-    {64, 4, 2, 7.0, {0.75, 0.60, 0.42}}, {96, 4, 1, 8.0, {1.03, 0.95, 0.52}}, {128, 8, 1, 6.5, {1.75, 1.10, 0.75}}};
+    {64, 4, 2, 7.4, {0.68, 0.51, 0.32}}, {96, 4, 1, 9.8, {0.85, 0.73, 0.43}}, {128, 8, 1, 13.0, {1.33, 0.73, 0.56}}};
 constexpr int kKernelCount = sizeof(kKernels) / sizeof(kKernels[0]);
 constexpr int kUnits = 256;           // compute units
 constexpr int kChunks = 128;          // small matrices: workgroups that share the columns of one, at most
