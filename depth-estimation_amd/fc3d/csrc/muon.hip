@@ -1240,7 +1240,7 @@ void ops_of(const Call& k, int plan, const Scales& s, bool exact, PlanOps& to) {
 struct Layout {
     int64_t parts, halves, sum_tiles;
     int gram;                         // the Gram products' kernel
-    int order[kMaxItems];             // the group's matrices as they are worked on: deep ones first, they take longest
+    int order[kMaxItems];             // the group's matrices as they are worked on: deep ones first, they take longest (numbers in the call)
     Shape shape[kMaxItems];           // in that order, like split
     int split[kMaxItems];
     int64_t head() const { return (parts * 8 + kMaxItems * (4 + (int64_t)sizeof(Matrix)) + 255) / 256 * 256; }
@@ -1289,10 +1289,10 @@ int64_t Layout::bytes() const {
 }
 
 // `planes`: of the Gram products' operands; `small`: in three launches, if the matrices allow it
-int layout_of(const Call& k, int from, int count, int planes, bool small, Layout& l) {
+int layout_of(const Call& k, const int* list, int count, int planes, bool small, Layout& l) {
     for (int i = 0; i < count; ++i) {
         Shape s;
-        if (!shape_of(k.rows[from + i], k.cols[from + i], s)) return FC3D_ERANGE;
+        if (!shape_of(k.rows[list[i]], k.cols[list[i]], s)) return FC3D_ERANGE;
         if (s.m == 0) return FC3D_EINVAL;
         int at = i;                                           // insertion: equal ones keep their order
         for (; at > 0 && l.shape[at - 1].n < s.n; --at) {
@@ -1300,7 +1300,7 @@ int layout_of(const Call& k, int from, int count, int planes, bool small, Layout
             l.order[at] = l.order[at - 1];
         }
         l.shape[at] = s;
-        l.order[at] = i;
+        l.order[at] = list[i];
     }
     int64_t prep = 0, depth = 0;
     int64_t groups[kKernelCount] = {};
@@ -1377,13 +1377,13 @@ int by_type(int type, F&& f) {
     return type == FC3D_F32 ? f(float{}) : type == FC3D_BF16 ? f(__bf16{}) : f(_Float16{});
 }
 
-int run_small(const Call& k, int from, const Layout& l, int count) {
+int run_small(const Call& k, const Layout& l, int count) {
     Table t = {};
     t.count = count;
     int64_t sums = 0, gram_groups = 0, apply_groups = 0;
     for (int i = 0; i < count; ++i) {
         const Shape& s = l.shape[i];
-        const int at = from + l.order[i];
+        const int at = l.order[i];
         t.e[i] = Matrix{k.g[at], k.mom ? k.mom[at] : nullptr, k.out[at], 0, (int)s.m, (int)s.n, (int)s.mp, (int)s.np,
                         k.lr ? k.lr[at] : 0.0f, 0, l.split[i], (int)sums, k.rows[at] > k.cols[at], 0};
         sums += l.split[i] < 2 ? 2 : l.split[i];
@@ -1403,7 +1403,7 @@ int run_small(const Call& k, int from, const Layout& l, int count) {
     });
 }
 
-int run_group(const Call& k, int from, const Layout& l, const Scales& sc, int count) {
+int run_group(const Call& k, const Layout& l, const Scales& sc, int count) {
     Table t = {};
     t.count = count;
     const bool exact = is_exact(k);
@@ -1411,7 +1411,7 @@ int run_group(const Call& k, int from, const Layout& l, const Scales& sc, int co
     bool used[kPlans] = {};
     for (int i = 0; i < count; ++i) {
         const Shape& s = l.shape[i];
-        const int at = from + l.order[i], plan = plan_of(k, sc.gain, s);
+        const int at = l.order[i], plan = plan_of(k, sc.gain, s);
         t.e[i] = Matrix{k.g[at], k.mom ? k.mom[at] : nullptr, k.out[at], halves, (int)s.m, (int)s.n, (int)s.mp, (int)s.np,
                         k.lr ? k.lr[at] : 0.0f, (int)parts, l.split[i], (int)sums, k.rows[at] > k.cols[at], plan};
         used[plan] = true;
@@ -1489,35 +1489,62 @@ int run_group(const Call& k, int from, const Layout& l, const Scales& sc, int co
 bool known_type(int t) { return t >= FC3D_F32 && t <= FC3D_F16; }
 bool off_align(const void* p, int type) { return (reinterpret_cast<uintptr_t>(p) & (type == FC3D_F32 ? 3u : 1u)) != 0; }
 
-// Matrices in groups of kMaxItems, one group after the other in the same workspace
+// Matrices of up to kTiny rows in a list of fp32 results with larger ones go through three launches of their own in 64 bits:
+// a result of a few rows averages little, and pairs of fp16 values left some of them three times as far off as fp32 products
+// do (2.2e-6 against 6e-7).  One tile of rows: 20 us for all of them together.
+constexpr int kTiny = 16;
+int64_t rows_of(const Call& k, int i) { return k.rows[i] < k.cols[i] ? k.rows[i] : k.cols[i]; }
+bool mixed(const Call& k) {
+    bool tiny = false, large = false;
+    for (int i = 0; i < k.count; ++i) {
+        tiny = tiny || rows_of(k, i) <= kTiny;
+        large = large || rows_of(k, i) > kSmall;
+    }
+    return tiny && large;
+}
+
+// Matrices in groups of kMaxItems, one group after the other in the same workspace; `apart`: the tiny ones behind the rest
 template <typename F>
-int in_groups(const Call& k, F&& f) {
-    for (int from = 0; from < k.count; from += kMaxItems) {
-        const int count = k.count - from < kMaxItems ? k.count - from : kMaxItems;
-        if (const int rc = f(from, count)) return rc;
+int in_groups(const Call& k, bool apart, F&& f) {
+    int list[kMaxItems];
+    for (int turn = 0; turn < (apart ? 2 : 1); ++turn) {
+        int count = 0;
+        for (int i = 0; i < k.count; ++i) {
+            if (apart && (rows_of(k, i) <= kTiny) != (turn == 1)) continue;
+            list[count++] = i;
+            if (count < kMaxItems) continue;
+            if (const int rc = f(list, count)) return rc;
+            count = 0;
+        }
+        if (count > 0)
+            if (const int rc = f(list, count)) return rc;
     }
     return FC3D_OK;
 }
 // The workspace is sized for every layout that a call with these sizes may take
 int size_of(const Call& k, size_t& bytes) {
     bytes = 0;
-    return in_groups(k, [&](int from, int count) {
-        for (int way = 0; way < 3; ++way) {
-            Layout l = {};
-            if (const int rc = layout_of(k, from, count, way == 1 ? 2 : 0, way == 2, l)) return rc;
-            if ((size_t)l.bytes() > bytes) bytes = (size_t)l.bytes();
-        }
-        return (int)FC3D_OK;
-    });
+    for (int apart = 0; apart <= (int)mixed(k); ++apart)
+        if (const int rc = in_groups(k, apart != 0, [&](const int* list, int count) {
+                for (int way = 0; way < 3; ++way) {
+                    Layout l = {};
+                    if (const int rc = layout_of(k, list, count, way == 1 ? 2 : 0, way == 2, l)) return rc;
+                    if ((size_t)l.bytes() > bytes) bytes = (size_t)l.bytes();
+                }
+                return (int)FC3D_OK;
+            }))
+            return rc;
+    return FC3D_OK;
 }
 
 int run(const Call& k) {
     Scales sc = {};
     if (!scales_of(k, sc)) return FC3D_ERANGE;
-    return in_groups(k, [&](int from, int count) {
+    const bool small = small_of(k, sc.gain);
+    return in_groups(k, small && k.out_type == FC3D_F32 && mixed(k), [&](const int* list, int count) {
         Layout l = {};
-        if (const int rc = layout_of(k, from, count, is_exact(k) ? 2 : 0, small_of(k, sc.gain), l)) return rc;
-        return l.small ? run_small(k, from, l, count) : run_group(k, from, l, sc, count);
+        if (const int rc = layout_of(k, list, count, is_exact(k) ? 2 : 0, small, l)) return rc;
+        return l.small ? run_small(k, l, count) : run_group(k, l, sc, count);
     });
 }
 

@@ -538,3 +538,18 @@ def test_steps_in_graphs_and_on_streams():
     torch.cuda.synchronize()
     for i, x in enumerate(got):
         assert torch.equal(x, alone[i % 2])
+
+
+@gpu
+def test_small_matrices_beside_large_ones():
+    """What a matrix is listed with does not cost it: next to a large one, results of a few rows are as exact as alone.
+    Bound: they are worked on in 64 bits, so their rounding to fp32 alone, half a step of each value, doubled."""
+    from fc3d import ops
+    shapes = [(2, 3), (3, 2), (16, 5), (5, 40), (1, 30), (16, 16), (40, 12), (7, 1000)]
+    gs = [update(s, "gauss", 600 + i) for i, s in enumerate(shapes * 7)]           # more than a group of them
+    large = update((100, 150), "gauss", 599)
+    out = ops.orthogonalize([g.cuda() for g in gs[:20]] + [large.cuda()] + [g.cuda() for g in gs[20:]])
+    near(out.pop(20), large, "the large one")
+    for x, g in zip(out, gs):
+        ref = ns(g, torch.float64)
+        assert float((x.cpu().double() - ref).norm()) <= 2 * 2.0 ** -24 * float(ref.norm()), g.shape
