@@ -839,8 +839,8 @@ int elem_size(int type) { return type == FC3D_F32 ? 4 : 2; }
 // or five wavefronts a SIMD hide each other's waits instead of three (16384 x 2048 bf16 54 -> 49 us, 8192 x 4096 87 -> 56);
 // beyond 8192 values 512 lanes take 32, with twice the registers of 1024 lanes that take 16 (2048 x 16000 fp32 138 -> 116,
 // bf16 129 -> 100 us).  Planes, forward: 8 channels.  Planes, backward, the fastest of 4 and 8
-// channels a lane and of 128 to 1024 lanes: 16-bit images of 64 channels 395 us with 8, 271 with 4 (537 MB of values; its
-// registers are conversions'); fp32 332 and 356; fp32 of 512 channels 47 with 8, 46 with 4 on twice the lanes.
+// channels a lane and of 128 to 1024 lanes: 16 x 128 x 16384 bf16 51 us with 4 on 512 lanes, 66 on 256; 32 x 64 x 65536 fp32
+// 324 with 8, 356 with 4; 512 channels: fp32 46 with 4 on 1024 lanes, 47 with 8 on 512, bf16 50 and 47.
 Plan plan_of(bool fwd, int type, int64_t outer, int64_t C, int64_t inner) {
     Plan p = {};
     p.rows = inner == 1;
@@ -873,8 +873,8 @@ Plan plan_of(bool fwd, int type, int64_t outer, int64_t C, int64_t inner) {
             const int cl = C <= 8 ? 1 : C <= 32 ? 4 : C <= 64 ? 8 : C <= 128 ? 16 : C <= 256 ? 32 : C <= 512 ? 64 : 128;
             take(cl, cl <= 32 ? 256 / cl : cl == 64 ? 8 : 4, 8, kPlanesFwd);
         } else if (C <= 32) take(C <= 8 ? 2 : 8, C <= 8 ? 128 : 32, 4, 2 * kPlanesBwd);
-        else if (C <= 64) type == FC3D_F32 ? take(8, 32, 8, kPlanesBwd) : take(16, 16, 4, 2 * kPlanesBwd);
-        else if (C <= 128) type == FC3D_F32 ? take(32, 16, 4, kPlanesBwd) : take(32, 8, 4, 2 * kPlanesBwd);
+        else if (C <= 64) take(8, 32, 8, kPlanesBwd);
+        else if (C <= 128) take(32, 16, 4, kPlanesBwd);
         else if (C <= 256) take(64, 8, 4, kPlanesBwd);
         else if (C <= 512) type == FC3D_F32 ? take(128, 8, 4, kPlanesBwd) : take(64, 8, 8, kPlanesBwd);
         else take(128, 4, 8, kPlanesBwd);
@@ -967,14 +967,8 @@ int planes_of(const BwdArgs& a, const Plan& p, unsigned groups) {
     constexpr bool F32 = sizeof(T) == 4;
     switch (p.lanes) {
         case 2: return planes_launch<T, V, 2, 128, 4>(a, groups);
-        case 8:
-            if constexpr (F32)
-                if (p.each == 8) return planes_launch<T, V, 8, 32, 8>(a, groups);
-            return planes_launch<T, V, 8, 32, 4>(a, groups);
-        case 16:
-            if constexpr (!F32) return planes_launch<T, V, 16, 16, 4>(a, groups);
-            return FC3D_EINVAL;                               // (no plan of fp32)
-        case 32: return planes_launch<T, V, 32, F32 ? 16 : 8, 4>(a, groups);
+        case 8: return p.each == 8 ? planes_launch<T, V, 8, 32, 8>(a, groups) : planes_launch<T, V, 8, 32, 4>(a, groups);
+        case 32: return planes_launch<T, V, 32, 16, 4>(a, groups);
         case 64:
             if constexpr (!F32)
                 if (p.each == 8) return planes_launch<T, V, 64, 8, 8>(a, groups);
