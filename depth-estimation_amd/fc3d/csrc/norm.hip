@@ -653,39 +653,31 @@ __global__ __launch_bounds__(CL* PL) void ln_planes_bwd(const T* __restrict__ dy
 }
 
 // ---- channels beyond what a workgroup's registers hold ------------------------------------------------------
-// One workgroup per row (rows) or per PLL positions (planes), the values read once per sum and once for the
-// result; the repeats come from the caches.  Strides: consecutive channels lie `cs` values apart.
+// One workgroup per row (rows) or per 16 or 4 positions (planes), the values read once per sum and once for the
+// result; the repeats come from the caches.  Loads are unrolled, several in flight: the wait for each would be all of the
+// time of a small input.
 constexpr int kLongBlock = 1024;
-constexpr int kLongPos = 16;         // planes: positions a workgroup takes
 
-template <bool PLANES>
+// NP: positions of a workgroup (rows: 1).  The sum over its lanes of the same position, in all of them.
+template <int NP>
 __device__ __forceinline__ float long_sum(float v, float* red) {
     __syncthreads();
-    if constexpr (PLANES) {
-        v += __shfl_xor(v, 16, 64);
-        v += __shfl_xor(v, 32, 64);
-        if ((threadIdx.x & 63) < kLongPos) red[(threadIdx.x >> 6) * kLongPos + (threadIdx.x & 15)] = v;
-        __syncthreads();
-        v = 0.0f;
 #pragma unroll
-        for (int i = 0; i < kLongBlock / 64; ++i) v += red[i * kLongPos + (threadIdx.x & 15)];
-    } else {
-        v = wave_sum(v);
-        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-        __syncthreads();
-        v = 0.0f;
+    for (int o = NP; o < 64; o <<= 1) v += __shfl_xor(v, o, 64);
+    if ((threadIdx.x & 63) < NP) red[(threadIdx.x >> 6) * NP + (threadIdx.x & 63)] = v;
+    __syncthreads();
+    v = 0.0f;
 #pragma unroll
-        for (int i = 0; i < kLongBlock / 64; ++i) v += red[i];
-    }
+    for (int i = 0; i < kLongBlock / 64; ++i) v += red[i * NP + (threadIdx.x & (NP - 1))];
     return v;
 }
 
-template <typename T, bool PLANES>
+template <typename T, int NP>
 __global__ __launch_bounds__(kLongBlock) void ln_long_fwd(const T* __restrict__ x, const void* __restrict__ w, const void* __restrict__ b, bool w_f32, long positions, long C, long inner,
                                                           long x_stride, float eps, int relu, T* __restrict__ y,
                                                           float* __restrict__ mean, float* __restrict__ rstd) {
-    __shared__ float red[kLongBlock / 64 * kLongPos];
-    constexpr int NP = PLANES ? kLongPos : 1, STEP = kLongBlock / NP;
+    __shared__ float red[kLongBlock / 64 * NP];
+    constexpr int STEP = kLongBlock / NP;
     const int pl = threadIdx.x % NP, c0 = threadIdx.x / NP;
     for (long q0 = (long)blockIdx.x * NP; q0 < positions; q0 += (long)gridDim.x * NP) {
         const bool live = q0 + pl < positions;
@@ -693,16 +685,19 @@ __global__ __launch_bounds__(kLongBlock) void ln_long_fwd(const T* __restrict__ 
         const T* xp = x + img * x_stride + p;
         T* yp = y + img * inner * C + p;
         float s = 0.0f;
+#pragma unroll 8
         for (long c = c0; c < C; c += STEP) s += (float)xp[c * inner];
-        const float mu = long_sum<PLANES>(s, red) / (float)C;
+        const float mu = long_sum<NP>(s, red) / (float)C;
         s = 0.0f;
+#pragma unroll 8
         for (long c = c0; c < C; c += STEP) {
             const float d = (float)xp[c * inner] - mu;
             s = fmaf(d, d, s);
         }
-        const float rs = 1.0f / sqrtf(long_sum<PLANES>(s, red) / (float)C + eps);
+        const float rs = 1.0f / sqrtf(long_sum<NP>(s, red) / (float)C + eps);
         if (live) {
-            for (long c = c0; c < C; c += STEP) {
+#pragma unroll 8
+        for (long c = c0; c < C; c += STEP) {
                 float v = fmaf(((float)xp[c * inner] - mu) * rs, param<T>(w, w_f32, c, 1.0f), param<T>(b, w_f32, c, 0.0f));
                 if (relu) v = passes(v) ? v : 0.0f;
                 yp[c * inner] = (T)v;
@@ -715,14 +710,14 @@ __global__ __launch_bounds__(kLongBlock) void ln_long_fwd(const T* __restrict__ 
     }
 }
 
-template <typename T, bool PLANES>
+template <typename T, int NP>
 __global__ __launch_bounds__(kLongBlock) void ln_long_bwd(const T* __restrict__ dy, const T* __restrict__ x,
                                                           const void* __restrict__ w, const void* __restrict__ b, bool w_f32,
                                                           const float* __restrict__ mean, const float* __restrict__ rstd,
                                                           long positions, long C, long inner, long dy_stride,
                                                           long x_stride, int relu, T* __restrict__ dx) {
-    __shared__ float red[kLongBlock / 64 * kLongPos];
-    constexpr int NP = PLANES ? kLongPos : 1, STEP = kLongBlock / NP;
+    __shared__ float red[kLongBlock / 64 * NP];
+    constexpr int STEP = kLongBlock / NP;
     const int pl = threadIdx.x % NP, c0 = threadIdx.x / NP;
     for (long q0 = (long)blockIdx.x * NP; q0 < positions; q0 += (long)gridDim.x * NP) {
         const bool live = q0 + pl < positions;
@@ -731,6 +726,7 @@ __global__ __launch_bounds__(kLongBlock) void ln_long_bwd(const T* __restrict__ 
         const T* gp = dy + img * dy_stride + p;
         const float mu = mean[q], rs = rstd[q];
         float s1 = 0.0f, s2 = 0.0f;
+#pragma unroll 8
         for (long c = c0; c < C; c += STEP) {
             const float wc = param<T>(w, w_f32, c, 1.0f), h = ((float)xp[c * inner] - mu) * rs;
             float g = (float)gp[c * inner];
@@ -738,10 +734,11 @@ __global__ __launch_bounds__(kLongBlock) void ln_long_bwd(const T* __restrict__ 
             s1 += g * wc;
             s2 = fmaf(g * wc, h, s2);
         }
-        const float m1 = long_sum<PLANES>(s1, red) / (float)C, m2 = long_sum<PLANES>(s2, red) / (float)C;
+        const float m1 = long_sum<NP>(s1, red) / (float)C, m2 = long_sum<NP>(s2, red) / (float)C;
         if (live) {
             T* dp = dx + img * inner * C + p;
-            for (long c = c0; c < C; c += STEP) {
+#pragma unroll 8
+        for (long c = c0; c < C; c += STEP) {
                 const float wc = param<T>(w, w_f32, c, 1.0f), h = ((float)xp[c * inner] - mu) * rs;
                 float g = (float)gp[c * inner];
                 if (relu) g = passes(fmaf(h, wc, param<T>(b, w_f32, c, 0.0f))) ? g : 0.0f;
@@ -751,44 +748,37 @@ __global__ __launch_bounds__(kLongBlock) void ln_long_bwd(const T* __restrict__ 
     }
 }
 
-// Sums over positions for the same case: a workgroup takes one share of the positions (blockIdx.y of gridDim.y) and
-// 256 channels (rows: a lane per channel) or one channel (planes: a lane per position).
+// Sums over positions for the same case: a workgroup takes one share of the positions (blockIdx.y of gridDim.y) and 256
+// channels (rows: a lane per channel) or four (planes: a wavefront per channel, a lane per position).
 template <typename T, bool PLANES>
 __global__ __launch_bounds__(256) void ln_long_params(const T* __restrict__ dy, const T* __restrict__ x,
                                                       const void* __restrict__ w, const void* __restrict__ b, bool w_f32,
                                                       const float* __restrict__ mean, const float* __restrict__ rstd,
                                                       long positions, long C, long inner, long dy_stride, long x_stride,
                                                       int relu, float* __restrict__ partial) {
-    __shared__ float red[2][4];
-    const long c = PLANES ? (long)blockIdx.x : (long)blockIdx.x * 256 + threadIdx.x;
+    const long c = PLANES ? (long)blockIdx.x * 4 + (threadIdx.x >> 6) : (long)blockIdx.x * 256 + threadIdx.x;
     const long share = (positions + gridDim.y - 1) / gridDim.y;
     const long lo = (long)blockIdx.y * share, hi = lo + share < positions ? lo + share : positions;
+    if (c >= C) return;
     float sw = 0.0f, sb = 0.0f;
-    if (c < C) {
-        const float wc = param<T>(w, w_f32, c, 1.0f), bc = param<T>(b, w_f32, c, 0.0f);
-        for (long q = lo + (PLANES ? threadIdx.x : 0); q < hi; q += PLANES ? 256 : 1) {
-            const long img = q / inner, p = q - img * inner;
-            const float h = ((float)x[img * x_stride + c * inner + p] - mean[q]) * rstd[q];
-            float g = (float)dy[img * dy_stride + c * inner + p];
-            if (relu) g = passes(fmaf(h, wc, bc)) ? g : 0.0f;
-            sw = fmaf(g, h, sw);
-            sb += g;
-        }
+    const float wc = param<T>(w, w_f32, c, 1.0f), bc = param<T>(b, w_f32, c, 0.0f);
+#pragma unroll 4
+    for (long q = lo + (PLANES ? (threadIdx.x & 63) : 0); q < hi; q += PLANES ? 64 : 1) {
+        const long img = PLANES ? (long)((unsigned)q / (unsigned)inner) : q, p = PLANES ? q - img * inner : 0;
+        const float h = ((float)x[img * x_stride + c * inner + p] - mean[q]) * rstd[q];
+        float g = (float)dy[img * dy_stride + c * inner + p];
+        if (relu) g = passes(fmaf(h, wc, bc)) ? g : 0.0f;
+        sw = fmaf(g, h, sw);
+        sb += g;
     }
     float* pw = partial + (long)blockIdx.y * 2 * C;
     if constexpr (PLANES) {
         sw = wave_sum(sw);
         sb = wave_sum(sb);
-        if ((threadIdx.x & 63) == 0) {
-            red[0][threadIdx.x >> 6] = sw;
-            red[1][threadIdx.x >> 6] = sb;
-        }
-        __syncthreads();
-        if (threadIdx.x < 2) pw[threadIdx.x * C + c] = (red[threadIdx.x][0] + red[threadIdx.x][1]) + (red[threadIdx.x][2] + red[threadIdx.x][3]);
-    } else if (c < C) {
-        pw[c] = sw;
-        pw[C + c] = sb;
+        if ((threadIdx.x & 63) > 0) return;
     }
+    pw[c] = sw;
+    pw[C + c] = sb;
 }
 
 // dw, db = sums of the n partial sums, 32 columns per workgroup and n shared out over 32 lanes of each
@@ -831,6 +821,7 @@ struct Plan {
     int beside;           // rows, positions or vectors of positions of one workgroup
     int each;             // values (rows) or channels (planes) of a lane
     long units, most;     // workgroups that the positions fill once, and of a launch
+    int64_t positions;
 };
 
 int elem_size(int type) { return type == FC3D_F32 ? 4 : 2; }
@@ -844,6 +835,7 @@ int elem_size(int type) { return type == FC3D_F32 ? 4 : 2; }
 Plan plan_of(bool fwd, int type, int64_t outer, int64_t C, int64_t inner) {
     Plan p = {};
     p.rows = inner == 1;
+    p.positions = outer * inner;
     const auto take = [&](int lanes, int beside, int each, long most) {
         p.lanes = lanes;
         p.beside = beside;
@@ -879,7 +871,10 @@ Plan plan_of(bool fwd, int type, int64_t outer, int64_t C, int64_t inner) {
         else if (C <= 512) type == FC3D_F32 ? take(128, 8, 4, kPlanesBwd) : take(64, 8, 8, kPlanesBwd);
         else take(128, 4, 8, kPlanesBwd);
         const int64_t nq = p.wide ? outer * nv : outer * inner;
-        p.units = p.fits ? (nq + p.beside - 1) / p.beside : (outer * inner + kLongPos - 1) / kLongPos;
+        // beyond the registers: 16 positions fill the pieces that memory is read in (4 x 4096 x 1024 fp32 70 us, 277 with 4),
+        // 4 spread a small input over more lanes (52 x 2048 x 8 fp32 7 us, 13 with 16)
+        if (!p.fits) p.beside = p.positions * C > (1 << 20) ? 16 : 4;
+        p.units = ((p.fits ? nq : p.positions) + p.beside - 1) / p.beside;
     }
     if (!p.fits) p.most = kLong;
     return p;
@@ -887,7 +882,11 @@ Plan plan_of(bool fwd, int type, int64_t outer, int64_t C, int64_t inner) {
 
 unsigned groups_of(const Plan& p) { return (unsigned)(p.units < p.most ? p.units : p.most); }
 constexpr int kLongShares = 64;
-int64_t partials_of(const Plan& p) { return p.fits ? (int64_t)groups_of(p) : kLongShares; }      // of a backward plan
+// Of a backward plan.  Long axes: shares of 512 positions at least, eight for each lane of a wavefront
+int64_t partials_of(const Plan& p) {
+    const int64_t shares = (p.positions + 511) / 512;
+    return p.fits ? (int64_t)groups_of(p) : shares < kLongShares ? shares : kLongShares;
+}
 bool direct(const Plan& p) { return p.fits && groups_of(p) == 1; }       // the sums are the gradients: no workspace
 
 int check_sizes(int x_type, int w_type, int64_t outer, int64_t C, int64_t inner) {
@@ -1012,24 +1011,24 @@ int registers_of(const A& a, const Plan& p) {
     return p.wide ? planes_of<T, kVec>(a, p, groups) : planes_of<T, 1>(a, p, groups);
 }
 
-template <typename T, bool PLANES>
+template <typename T, int NP>
 int long_of(const FwdArgs& a, const Plan& p) {
-    FC3D_LAUNCH("layer_norm_fwd", (ln_long_fwd<T, PLANES>), dim3(groups_of(p)), dim3(kLongBlock), 0, a.s, (const T*)a.x, a.w,
+    FC3D_LAUNCH("layer_norm_fwd", (ln_long_fwd<T, NP>), dim3(groups_of(p)), dim3(kLongBlock), 0, a.s, (const T*)a.x, a.w,
                 a.b, a.w_f32, (long)(a.outer * a.inner), (long)a.C, (long)a.inner, (long)a.x_stride, a.eps, a.relu, (T*)a.y,
                 a.mean, a.rstd);
     return FC3D_OK;
 }
-template <typename T, bool PLANES>
+template <typename T, int NP>
 int long_of(const BwdArgs& a, const Plan& p) {
     const T *dy = (const T*)a.dy, *x = (const T*)a.x;
     const long positions = (long)(a.outer * a.inner);
     if (a.dx)
-        FC3D_LAUNCH("layer_norm_bwd", (ln_long_bwd<T, PLANES>), dim3(groups_of(p)), dim3(kLongBlock), 0, a.s, dy, x, a.w, a.b,
+        FC3D_LAUNCH("layer_norm_bwd", (ln_long_bwd<T, NP>), dim3(groups_of(p)), dim3(kLongBlock), 0, a.s, dy, x, a.w, a.b,
                     a.w_f32, a.mean, a.rstd, positions, (long)a.C, (long)a.inner, (long)a.dy_stride, (long)a.x_stride,
                     a.relu, (T*)a.dx);
     if (a.sums.wanted())
-        FC3D_LAUNCH("layer_norm_params", (ln_long_params<T, PLANES>),
-                    dim3((unsigned)(PLANES ? a.C : (a.C + 255) / 256), kLongShares), dim3(256), 0, a.s, dy, x, a.w, a.b,
+        FC3D_LAUNCH("layer_norm_params", (ln_long_params<T, (NP > 1)>),
+                    dim3((unsigned)(NP > 1 ? (a.C + 3) / 4 : (a.C + 255) / 256), (unsigned)partials_of(p)), dim3(256), 0, a.s, dy, x, a.w, a.b,
                     a.w_f32, a.mean, a.rstd, positions, (long)a.C, (long)a.inner, (long)a.dy_stride, (long)a.x_stride,
                     a.relu, a.sums.partial);
     return FC3D_OK;
@@ -1038,7 +1037,7 @@ int long_of(const BwdArgs& a, const Plan& p) {
 template <typename T, typename A>
 int kernel_of(const A& a, const Plan& p) {
     if (p.fits) return registers_of<T>(a, p);
-    return p.rows ? long_of<T, false>(a, p) : long_of<T, true>(a, p);
+    return p.rows ? long_of<T, 1>(a, p) : p.beside == 4 ? long_of<T, 4>(a, p) : long_of<T, 16>(a, p);
 }
 template <typename A>
 int type_of(const A& a, const Plan& p, int x_type) {

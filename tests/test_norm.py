@@ -469,3 +469,33 @@ def test_gradients_of_one_workgroup(dt):
                     terms = (dy.double().abs() * (1 + x.double().abs())).movedim(dim, -1).reshape(-1, C).sum(0) * 4
                     tol = (n + 16) * 2.0 ** -24 * terms + torch.finfo(pt).eps / 2 * r.grad.abs() + 1e-7
                     assert bool(((t.grad.cpu().double() - r.grad).abs() <= tol).all()), (shape, dt, pt)
+
+
+@gpu
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16], ids=lambda t: str(t).replace("torch.", ""))
+@pytest.mark.parametrize("shape", [(1, 1025, 1, 3), (2, 2048, 3, 1), (3, 1500, 16, 17), (2, 16390, 2, 3), (2, 1100, 31, 33)])
+def test_many_channels_of_planes(shape, dt):
+    """More channels than the registers hold, few and many positions: forward, and all gradients, against 64 bits."""
+    from fc3d import ops
+    g = torch.Generator().manual_seed(shape[1])
+    C = shape[1]
+    x, dy = (torch.randn(shape, generator=g).to(dt) for _ in range(2))
+    w, b = torch.randn(C, generator=g), torch.randn(C, generator=g)
+    xr, wr, br = (t.double().requires_grad_() for t in (x, w, b))
+    ref = torch.relu(torch.nn.functional.layer_norm(xr.movedim(1, -1), (C,), wr, br, 1e-5)).movedim(-1, 1)
+    # values within rounding of the ReLU's edge may fall on either side: their gradient is taken out on both
+    edge = torch.nn.functional.layer_norm(x.double().movedim(1, -1), (C,), w.double(), b.double(), 1e-5).movedim(-1, 1).abs() < 1e-4
+    dy[edge] = 0
+    ref.backward(dy.double())
+    xd, wd, bd = (t.cuda().requires_grad_() for t in (x, w, b))
+    y = ops.layer_norm(xd, wd, bd, dim=1, relu=True)
+    y.backward(dy.cuda())
+    half = torch.finfo(dt).eps / 2
+    # sums of C (or of all positions) terms in fp32, in lanes and wavefronts: a few half steps times the sum's depth, 64 here,
+    # relative to the 2-norm; one rounding to the type
+    for got, want, own in ((y, ref, half), (xd.grad, xr.grad, half), (wd.grad, wr.grad, 0.0), (bd.grad, br.grad, 0.0)):
+        off = float((got.detach().cpu().double() - want.detach()).norm() / want.detach().norm())
+        assert off <= own + 64 * 2.0 ** -24, (shape, off)
+    again = torch.autograd.grad(ops.layer_norm(xd, wd, bd, dim=1, relu=True), (xd, wd, bd), dy.cuda())
+    for p, q in zip(again, (xd.grad, wd.grad, bd.grad)):
+        assert torch.equal(p, q)
