@@ -882,9 +882,9 @@ Plan plan_of(bool fwd, int type, int64_t outer, int64_t C, int64_t inner) {
 
 unsigned groups_of(const Plan& p) { return (unsigned)(p.units < p.most ? p.units : p.most); }
 constexpr int kLongShares = 64;
-// Of a backward plan.  Long axes: shares of 512 positions at least, eight for each lane of a wavefront
+// Of a backward plan.  Long axes: shares of 16 rows at least, or of 512 positions of planes, eight for each lane
 int64_t partials_of(const Plan& p) {
-    const int64_t shares = (p.positions + 511) / 512;
+    const int64_t shares = p.rows ? (p.positions + 15) / 16 : (p.positions + 511) / 512;
     return p.fits ? (int64_t)groups_of(p) : shares < kLongShares ? shares : kLongShares;
 }
 bool direct(const Plan& p) { return p.fits && groups_of(p) == 1; }       // the sums are the gradients: no workspace
