@@ -15,12 +15,15 @@
 // buffer, from a bound on its norm, keeps both in fp16's range) and a product is hi hi + hi lo + lo hi with fp32
 // sums on the matrix units: the accuracy of fp32 products at three fp16 passes instead of the sixteen that the
 // fp32 matrix instructions take.  Forming A squares the singular values, so a segment of L Gram steps loses the
-// directions whose share of A is below its rounding, amplified a^(2L)-fold: five steps at once cost 1e-4 of the
-// result in bad cases (measured in emulation, low rank plus noise), which is below the rounding of a 16-bit result;
-// for fp32 results the segments are of two and three steps, or of one for matrices that are nearly square
-// (n < 2 m, where the smallest singular values sit near zero) and for those of up to 64 rows (where the squares saved
-// are cheap), as accurate as step by step.  Against 64 bits: 512 x 4608 1.2e-6 of the result (fp32 matrix products
-// 4.2e-6), 256 x 256 6e-7 (1.8e-6); 64 x 288 2.5e-8 (1.5e-6), worked on in 64 bits.
+// directions whose share of A is below its rounding, amplified a^(2L)-fold.  Measured against 64 bits on a few strong
+// directions over a noise floor (rank 4 and noise of 0.3 to 0.001, 128 x 128 to 2048 x 8192): five steps at once cost
+// 1e-4 to 2e-4 of the result, a tenth of a bf16 result's rounding (1.7e-3) but as much as an fp16 result's (2.1e-4).  So
+// bf16 results take all five at once, fp16 ones two and three (2e-6 to 4e-5, what fp32 products are off by there; 8e-5 at
+// 2048 x 8192, where those are off by 1.3e-4).  For fp32 results the segments are of two and three steps too, or of one for
+// matrices that are nearly square (n < 2 m, where the smallest singular values sit near zero) and for those of up to 64
+// rows (where the squares saved are cheap): 0.3 to 1.5 times the error of fp32 products on the same inputs (512 x 4608
+// without structure 1.4e-6 against 4.3e-6, 128 x 300 of rank 4 and noise of 0.1 3.8e-6 against 2.6e-6); 64 x 288 2.5e-8
+// (1.5e-6), worked on in 64 bits.
 #include "fc3d_common.h"
 
 #include <cmath>
@@ -1135,13 +1138,14 @@ bool shape_of(int64_t rows, int64_t cols, Shape& s) {
 
 float pow2_below(double bound) { return (float)std::exp2(14.0 - std::ceil(std::log2(bound))); }     // bound * it <= 2^14
 
-// How many steps the Gram form takes at once.  A segment of L amplifies what it rounded gain^(2L)-fold: 16-bit results
-// bear five of the usual steps (gain 3.4), fp32 ones three; steps that amplify more go two by two and one by one.  So do
-// more than five steps of an fp32 result: near one the usual polynomial spreads neighbouring values (its slope is -1.4 at
-// 0.75), and every further step amplifies what a segment rounded.
+// How many steps the Gram form takes at once.  A segment of L amplifies what it rounded gain^(2L)-fold: bf16 results
+// bear five of the usual steps (gain 3.4), fp16 and fp32 ones three; steps that amplify more go two by two and, of fp32
+// results, one by one.  So do more than five steps: near one the usual polynomial spreads neighbouring values (its slope is
+// -1.4 at 0.75), and every further step amplifies what a segment rounded.
 constexpr double kGain = 4.0;
 int segment_of(const Call& k, double gain) {                  // the longest one: the running products' scale follows from it
-    const int most = gain > kGain ? (k.out_type == FC3D_F32 ? 1 : 2) : k.out_type != FC3D_F32 ? 5 : k.steps <= 5 ? 3 : 1;
+    const int apart = k.out_type == FC3D_F32 ? 1 : 2;
+    const int most = gain > kGain ? apart : k.out_type == FC3D_BF16 ? 5 : k.steps <= 5 ? 3 : apart;
     return k.steps < most ? k.steps : most;
 }
 // Whether small matrices take all steps at once in 64 bits: what is rounded (1e-16) stays under 1e-5 when amplified, which
@@ -1185,10 +1189,11 @@ bool scales_of(const Call& k, Scales& s) {
     return true;
 }
 
-// Plan 0 goes through segments of `segment` steps, plan 1 (fp32, large matrices) through one of two steps and one of
-// three.
+// Plan 0 goes through segments of `segment` steps, plan 1 (fp16, and large matrices in fp32) through one of two steps and
+// one of three.
 int plan_of(const Call& k, double gain, const Shape& s) {
-    return k.out_type == FC3D_F32 && gain <= kGain && s.n >= 2 * s.m && s.m > 64 && k.steps <= 5;
+    if (gain > kGain || k.steps > 5 || k.out_type == FC3D_BF16) return 0;
+    return k.out_type == FC3D_F16 || (s.n >= 2 * s.m && s.m > 64);
 }
 bool starts(int segment, int plan, int step) {
     return plan == 0 ? step % segment == 0 : step == 0 || step == 2;
@@ -1460,7 +1465,7 @@ int run_group(const Call& k, const Layout& l, const Scales& sc, int count) {
                 rho_gram = rho_gram || (a.op[p][j].kind == GRAM && a.op[p][j].use_rho);
                 rho_apply = rho_apply || (a.op[p][j].kind == APPLY && a.op[p][j].use_rho);
             }
-        // an input taken as it is has one plane (its plan is the only one: 16-bit results)
+        // an input taken as it is has one plane (its plan is the only one: 16-bit results go through one plan, whatever their size)
         const int p1 = rho_gram ? 1 : 2, p2 = rho_gram || rho_apply ? 1 : 2;
         int64_t groups[kKernelCount], depth = 0;
         for (int c = 0; c < kKernelCount; ++c) groups[c] = groups_of(a, t, kKernels[c].tile);

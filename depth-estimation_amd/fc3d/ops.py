@@ -1421,8 +1421,9 @@ def orthogonalize(g, steps: int = 5, coefficients=NS_COEFFICIENTS, eps: float = 
     With the default ones the singular values of g end near one, its singular vectors are kept.
 
     g: float32, bfloat16 or float16 tensors of two axes or more on one GPU (a convolution's weight is
-    [out, in * kh * kw]), any sizes and strides; results in their shapes and types.  The products keep the accuracy
-    of fp32 whatever the type.  No gradient."""
+    [out, in * kh * kw]), any sizes and strides; results in their shapes and types.  What is rounded to the result is
+    about as exact as fp32 products make it; in front of a bf16 rounding up to a tenth of that rounding may be lost.
+    No gradient."""
     single = isinstance(g, torch.Tensor)
     mats = [g] if single else list(g)
     steps, a, b, c, eps = _ns_arguments(steps, coefficients, eps)

@@ -553,3 +553,45 @@ def test_small_matrices_beside_large_ones():
     for x, g in zip(out, gs):
         ref = ns(g, torch.float64)
         assert float((x.cpu().double() - ref).norm()) <= 2 * 2.0 ** -24 * float(ref.norm()), g.shape
+
+
+def second_segment_slope():
+    """The most that three default steps make of a relative error of A, in result: |P(l) - P(k)| / |l - k| s over the
+    squares l, k of singular values up to the polynomial's maximum, 1.21, and s = sqrt(k)."""
+    a, b, c = COEFFS
+
+    def p(lam):
+        out = torch.ones_like(lam)
+        for _ in range(3):
+            q = a + b * lam + c * lam * lam
+            out, lam = out * q, lam * q * q
+        return out
+    s = torch.linspace(0, 1.21, 1500, dtype=torch.float64)
+    lam = s * s
+    d = lam[:, None] - lam[None, :]
+    dd = (p(lam)[:, None] - p(lam)[None, :]) / d.masked_fill(d == 0, 1.0)
+    dd.diagonal().copy_((p(lam + 1e-7) - p(lam - 1e-7)) / 2e-7)
+    return float((dd.abs() * s[None, :]).max())
+
+
+@gpu
+@pytest.mark.parametrize("noise", [0.3, 0.1, 0.03])
+@pytest.mark.parametrize("m,n", [(128, 128), (128, 300), (256, 512), (512, 700)])
+def test_half_precision_results_lose_no_more_than_their_rounding(m, n, noise):
+    """Strong directions over a noise floor in fp16.  Rounding the exact result leaves r; in front of the rounding the
+    result may be off by e: four times what fp32 products are, 2^-20, and the Gram matrix of the segment of three steps,
+    whose values are off by 2 * 2^-23 of themselves.  The rounding does not know of e, so the squares add; of N values, the
+    sum of squares of a rounding scatters by 0.9 / sqrt(N) and the mixed term by less: 8 / sqrt(N) is four times both."""
+    from fc3d import ops
+    gen = torch.Generator().manual_seed(m + n)
+    g = (1e-3 * (torch.randn(m, 4, generator=gen) @ torch.randn(4, n, generator=gen) +
+                 noise * torch.randn(m, n, generator=gen))).half()
+    ref = ns(g, torch.float64)
+    norm = float(ref.norm())
+    x2 = ns(g, torch.float64, 2)
+    r = float((ref.half().double() - ref).norm()) / norm
+    e = 4 * float((ns(g, F32).double() - ref).norm()) / norm + 2.0 ** -20
+    e += second_segment_slope() * 2.0 ** -22 * float((x2 @ x2.t()).norm()) / norm
+    tol = math.sqrt((r * r + e * e) * (1 + 8 / math.sqrt(m * n)))
+    off = float((ops.orthogonalize(g.cuda()).cpu().double() - ref).norm()) / norm
+    assert off <= tol, (off, tol, r)
