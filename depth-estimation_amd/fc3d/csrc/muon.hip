@@ -1494,9 +1494,10 @@ int run_group(const Call& k, const Layout& l, const Scales& sc, int count) {
 bool known_type(int t) { return t >= FC3D_F32 && t <= FC3D_F16; }
 bool off_align(const void* p, int type) { return (reinterpret_cast<uintptr_t>(p) & (type == FC3D_F32 ? 3u : 1u)) != 0; }
 
-// Matrices of up to kTiny rows in a list of fp32 results with larger ones go through three launches of their own in 64 bits:
-// a result of a few rows averages little, and pairs of fp16 values left some of them three times as far off as fp32 products
-// do (2.2e-6 against 6e-7).  One tile of rows: 20 us for all of them together.
+// Matrices of up to kTiny rows in a list with larger ones go through three launches of their own in 64 bits: a result of a
+// few rows averages little.  Pairs of fp16 values left some fp32 results three times as far off as fp32 products do (2.2e-6
+// against 6e-7), and a bf16 result's five steps at once cost up to 2e-3, as much as its rounding, where its rows were nearly
+// dependent (rank 1 and noise of 0.01, 2 to 8 rows; 4e-4 from 17 rows on).  One tile of rows: 20 us for all of them together.
 constexpr int kTiny = 16;
 int64_t rows_of(const Call& k, int i) { return k.rows[i] < k.cols[i] ? k.rows[i] : k.cols[i]; }
 bool mixed(const Call& k) {
@@ -1546,7 +1547,7 @@ int run(const Call& k) {
     Scales sc = {};
     if (!scales_of(k, sc)) return FC3D_ERANGE;
     const bool small = small_of(k, sc.gain);
-    return in_groups(k, small && k.out_type == FC3D_F32 && mixed(k), [&](const int* list, int count) {
+    return in_groups(k, small && mixed(k), [&](const int* list, int count) {
         Layout l = {};
         if (const int rc = layout_of(k, list, count, is_exact(k) ? 2 : 0, small, l)) return rc;
         return l.small ? run_small(k, l, count) : run_group(k, l, sc, count);

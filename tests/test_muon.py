@@ -595,3 +595,24 @@ def test_half_precision_results_lose_no_more_than_their_rounding(m, n, noise):
     tol = math.sqrt((r * r + e * e) * (1 + 8 / math.sqrt(m * n)))
     off = float((ops.orthogonalize(g.cuda()).cpu().double() - ref).norm()) / norm
     assert off <= tol, (off, tol, r)
+
+
+@gpu
+@pytest.mark.parametrize("dt", [BF16, F16], ids=lambda t: str(t).replace("torch.", ""))
+def test_small_matrices_beside_large_ones_in_16_bits(dt):
+    """Rows that nearly depend on each other, next to a large matrix.  Worked on in 64 bits and rounded twice, to fp32 and to
+    the result's type: beside the rounding of the exact result 2 * 2^-24 of each value, where the first rounding moves it
+    across the second one's middle."""
+    from fc3d import ops
+    gs = []
+    for m in (1, 2, 3, 5, 8, 16):
+        for n in (m, m + 1, m + 40):
+            for noise in (0.1, 0.01, 0.001):
+                gen = torch.Generator().manual_seed(1000 * m + n)
+                x = torch.randn(m, 1, generator=gen) @ torch.randn(1, n, generator=gen) + noise * torch.randn(m, n, generator=gen)
+                gs.append((x.t() if n % 2 else x).contiguous().to(dt))
+    out = ops.orthogonalize([g.cuda() for g in gs] + [update((100, 150), "gauss", 598, dt).cuda()])
+    for x, g in zip(out, gs):
+        ref = ns(g, torch.float64)
+        norm, r = float(ref.norm()), float((ref.to(dt).double() - ref).norm())
+        assert float((x.cpu().double() - ref).norm()) <= r + 2 * 2.0 ** -24 * norm, tuple(g.shape)
