@@ -1220,6 +1220,8 @@ def _norm_out(x, dim, last):
 
 
 _get_device = torch._C._cuda_getDevice
+_tracing = torch._C._get_tracing_state
+_forward_ad = torch.autograd.forward_ad
 
 
 def _norm_forward(x, weight, bias, eps, dim, relu, want_stats):
@@ -1237,6 +1239,8 @@ def _norm_forward(x, weight, bias, eps, dim, relu, want_stats):
         last = _norm_last(x, dim)
         xd, outer, C, inner, step = _norm_layout(x, dim, last)
         y = _norm_out(x, dim, last)
+    if type(C) is not int:                                       # under a tracer sizes are tensors
+        outer, C, inner, step = int(outer), int(C), int(inner), int(step)
     code = _TYPES[x.dtype]
     p = weight if weight is not None else bias
     p_code = code if p is None or p.dtype == x.dtype else 0
@@ -1351,7 +1355,9 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
         weight = _dense(weight)
     if bias is not None:
         bias = _dense(bias)
-    if grad and torch.is_grad_enabled():
+    # The short way is for calls of which nothing but the result counts: a tracer would not see the kernel, and a forward-mode
+    # tangent would be left behind (the operator has none: apply says so).
+    if (grad and torch.is_grad_enabled()) or _tracing() is not None or _forward_ad._current_level >= 0:
         return LayerNormFn.apply(x, weight, bias, eps, dim, bool(relu))
     return _norm_forward(x, weight, bias, eps, dim, bool(relu), False)[0]
 
@@ -1396,6 +1402,11 @@ def _ns_arguments(steps, coefficients, eps):
     return steps, a, b, c, eps
 
 
+def _not_traced(what):
+    if _tracing() is not None:
+        raise RuntimeError(f"{what} cannot be traced: the tracer would record its empty results without the kernels")
+
+
 def _pointers(tensors):
     return (ctypes.c_void_p * len(tensors))(*[t.data_ptr() for t in tensors])
 
@@ -1424,6 +1435,7 @@ def orthogonalize(g, steps: int = 5, coefficients=NS_COEFFICIENTS, eps: float = 
     [out, in * kh * kw]), any sizes and strides; results in their shapes and types.  What is rounded to the result is
     about as exact as fp32 products make it; in front of a bf16 rounding a tenth of that rounding may be lost, a
     quarter of it for matrices of 17 to 64 rows beside larger ones.  No gradient."""
+    _not_traced("orthogonalize")
     single = isinstance(g, torch.Tensor)
     mats = [g] if single else list(g)
     steps, a, b, c, eps = _ns_arguments(steps, coefficients, eps)
@@ -1477,6 +1489,7 @@ def muon_step(params, grads, momenta, lr: float = 0.02, momentum: float = 0.95, 
     params: float32, bfloat16 or float16 tensors of two axes or more, dense in memory (the first axis outermost, or a
     transposed matrix), on one GPU, each of them once.  grads: the same shapes, any of the three types; copied where
     they lie in another order than their weight.  momenta: float32, in their weight's memory order."""
+    _not_traced("muon_step")
     params, grads, momenta = list(params), list(grads), list(momenta)
     if not len(params) == len(grads) == len(momenta):
         raise ValueError(f"{len(params)} weights, {len(grads)} gradients, {len(momenta)} momenta")

@@ -616,3 +616,12 @@ def test_small_matrices_beside_large_ones_in_16_bits(dt):
         ref = ns(g, torch.float64)
         norm, r = float(ref.norm()), float((ref.to(dt).double() - ref).norm())
         assert float((x.cpu().double() - ref).norm()) <= r + 2 * 2.0 ** -24 * norm, tuple(g.shape)
+
+
+def test_tracing_is_refused():
+    """A tracer would record the results' allocation alone."""
+    from fc3d import ops
+    with pytest.raises(RuntimeError, match="traced"):
+        torch.jit.trace(lambda t: ops.orthogonalize(t), (torch.zeros(4, 4),), check_trace=False)
+    with pytest.raises(RuntimeError, match="traced"):
+        torch.jit.trace(lambda t: ops.muon_step([t], [t], [t]), (torch.zeros(4, 4),), check_trace=False)

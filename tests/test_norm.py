@@ -499,3 +499,44 @@ def test_many_channels_of_planes(shape, dt):
     again = torch.autograd.grad(ops.layer_norm(xd, wd, bd, dim=1, relu=True), (xd, wd, bd), dy.cuda())
     for p, q in zip(again, (xd.grad, wd.grad, bd.grad)):
         assert torch.equal(p, q)
+
+
+def test_tracers_and_tangents_go_through_autograd(monkeypatch):
+    """Without a gradient too: a tracer records the call itself, not the kernel's empty output, and forward mode is refused
+    as by the other operators.  On the CPU, with a stand-in for the launch."""
+    import torch.autograd.forward_ad as fw
+    import torch.nn.functional as F
+    from fc3d import ops
+
+    def stand_in(x, weight, bias, eps, dim, relu, want_stats):
+        y = torch.empty_like(x)
+        y.data.numpy()[:] = F.layer_norm(x.detach(), (8,), weight, bias, eps).numpy()      # behind the tracer's back
+        return y, x, torch.zeros(1), None
+    monkeypatch.setattr(ops, "_need_gpu_float", lambda t, what: 0)
+    monkeypatch.setattr(ops, "_norm_forward", stand_in)
+    w, b = torch.rand(8) + 0.5, torch.rand(8)
+    x = torch.randn(4, 8)
+    with torch.no_grad():
+        traced = torch.jit.trace(lambda t: ops.layer_norm(t, w, b) * 2.0, (torch.randn(4, 8),), check_trace=False)
+        assert "LayerNormFn" in str(traced.graph)
+        assert torch.equal(traced(x), F.layer_norm(x, (8,), w, b, 1e-5) * 2.0)
+    with fw.dual_level():
+        assert torch.equal(ops.layer_norm(x, w, b), F.layer_norm(x, (8,), w, b, 1e-5))         # no tangent: nothing lost
+        for args in ((fw.make_dual(x, torch.ones_like(x)), w, b), (x, fw.make_dual(w, torch.ones_like(w)), b)):
+            with pytest.raises(NotImplementedError):
+                ops.layer_norm(*args)
+
+
+@gpu
+@pytest.mark.parametrize("shape,dim", [((6, 40), -1), ((2, 16, 9, 7), 1)])
+def test_traced_and_forward_mode_on_the_gpu(shape, dim):
+    import torch.autograd.forward_ad as fw
+    from fc3d import ops
+    x, w, b, _ = (t.cuda() for t in inputs(shape, dim, F32, F32, 71))
+    f = lambda t: ops.layer_norm(t, w, b, dim=dim, relu=True) + 1.0  # noqa: E731
+    with torch.no_grad():
+        traced = torch.jit.trace(f, (torch.zeros_like(x),), check_trace=False)
+        for t in (x, 2.0 * x, x[:1], x.transpose(0, -1).contiguous().transpose(0, -1)):        # other values, sizes, orders
+            assert torch.equal(traced(t), f(t))
+    with fw.dual_level(), pytest.raises(NotImplementedError):
+        f(fw.make_dual(x, x))
