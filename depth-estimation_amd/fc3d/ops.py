@@ -1232,7 +1232,10 @@ def _norm_forward(x, weight, bias, eps, dim, relu, want_stats):
         inner = 1
         for n in shape[dim + 1:]:
             inner *= n
-        outer = x.numel() // (C * inner) if inner else 0
+        if inner:
+            outer = x.numel() // (C * inner)
+        else:                                                    # empty planes: no position, like an empty batch
+            outer, inner = 0, 1
         last, xd, step = dim == len(shape) - 1, x, C * inner
         y = torch.empty_like(x)
     else:

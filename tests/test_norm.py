@@ -540,3 +540,41 @@ def test_traced_and_forward_mode_on_the_gpu(shape, dim):
             assert torch.equal(traced(t), f(t))
     with fw.dual_level(), pytest.raises(NotImplementedError):
         f(fw.make_dual(x, x))
+
+
+def test_empty_planes_have_no_position(monkeypatch):
+    """What reaches the entry points of a tensor without values: no outer index, wherever the empty axis is.  On the CPU,
+    with a stand-in for the launch, and the entry point itself (nothing is launched)."""
+    from fc3d import _native, ops
+    lib, seen = _native.load(), []
+
+    class Lib:
+        @staticmethod
+        def fc3d_layer_norm_fwd(stream, *args):
+            seen.append((args[5], args[6], args[7]))
+            return lib.fc3d_layer_norm_fwd(None, *args)
+    monkeypatch.setattr(ops, "_lib", Lib)
+    monkeypatch.setattr(ops, "_need_gpu_float", lambda t, what: 0)
+    monkeypatch.setattr(ops, "_raw_stream", lambda dev: 0)
+    monkeypatch.setattr(ops, "_get_device", lambda: -1)
+    for shape in ((2, 8, 0, 5), (2, 8, 5, 0), (2, 8, 0), (0, 8, 3, 3), (0, 8)):
+        for x in (torch.zeros(shape), torch.zeros(shape).transpose(0, -1).contiguous().transpose(0, -1)):
+            assert ops.layer_norm(x, dim=1).shape == shape
+            outer, C, inner = seen.pop()
+            assert outer == 0 and C == 8 and inner >= 1
+
+
+@gpu
+@pytest.mark.parametrize("dt", [F32, BF16])
+@pytest.mark.parametrize("shape", [(2, 8, 0, 5), (2, 8, 5, 0), (2, 8, 0)])
+def test_empty_planes(shape, dt):
+    from fc3d import ops
+    w, b = (torch.ones(8, device="cuda", dtype=dt, requires_grad=True) for _ in range(2))
+    x = torch.zeros(shape, device="cuda", dtype=dt, requires_grad=True)
+    for relu in (False, True):
+        y = ops.layer_norm(x, w, b, dim=1, relu=relu)
+        assert y.shape == shape and y.dtype == dt
+        dx, dw, db = torch.autograd.grad(y, (x, w, b), torch.zeros_like(y))
+        assert dx.shape == shape and not dw.any() and not db.any()
+    with torch.no_grad():
+        assert ops.layer_norm(x, w, b, dim=1).shape == shape
