@@ -1185,7 +1185,7 @@ def _norm_layout(x, dim, last):
         for n in rest:
             outer *= n
         if step is None:
-            return x.movedim(dim, -1).contiguous(), outer, C, 1, C
+            return x.movedim(dim, -1).contiguous().movedim(-1, dim), outer, C, 1, C
         return x, outer, C, 1, step
     outer = inner = 1
     for n in sizes[:dim]:
@@ -1264,7 +1264,7 @@ def _norm_forward(x, weight, bias, eps, dim, relu, want_stats):
             ctx.__exit__(None, None, None)
     if status:
         _check(status, "fc3d_layer_norm_fwd")
-    return y, xd, stats, (dim, last, relu, outer, C, inner, step, code, p_code, dev)
+    return y, xd, stats, (dim, last, relu, outer, C, inner, step, code, p_code, dev, xd.stride() if want_stats else None)
 
 
 class LayerNormFn(torch.autograd.Function):
@@ -1285,8 +1285,14 @@ class LayerNormFn(torch.autograd.Function):
     @staticmethod
     def gradients(ctx, dy):
         xd, weight, bias, stats = ctx.saved_tensors
-        dim, last, relu, outer, C, inner, x_step, code, p_code, dev = ctx.meta
+        dim, last, relu, outer, C, inner, x_step, code, p_code, dev, strides = ctx.meta
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
+        # hooks on saved tensors may hand back a copy in another memory order (save_on_cpu does)
+        if xd.dtype != dy.dtype or stats.dtype != torch.float32 or xd.get_device() != dev or stats.get_device() != dev:
+            raise RuntimeError(f"layer_norm: its saved tensors came back as {xd.dtype} and {stats.dtype} on {xd.device} and "
+                               f"{stats.device}")
+        if xd.stride() != strides:
+            xd, _, _, _, x_step = _norm_layout(xd, dim, last)
         if dy.is_contiguous() and (not last or dim == dy.dim() - 1):
             g, g_step = dy, C * inner
         else:

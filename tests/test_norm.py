@@ -578,3 +578,84 @@ def test_empty_planes(shape, dt):
         assert dx.shape == shape and not dw.any() and not db.any()
     with torch.no_grad():
         assert ops.layer_norm(x, w, b, dim=1).shape == shape
+
+
+@pytest.mark.parametrize("case", ["channels_last", "padded planes", "padded rows", "copied", "dense"])
+def test_saved_tensors_in_another_memory_order(case, monkeypatch):
+    """Hooks that keep saved tensors elsewhere hand them back dense, whatever their strides were: the backward pass has to
+    read them as they come.  On the CPU, with the formula in place of the launches, its reads kept inside the tensors."""
+    import ctypes
+    from fc3d import ops
+    room = {}                                                      # address -> values behind it
+
+    def at(ptr, count):
+        assert count <= room[ptr], f"{count} values read of {room[ptr]}"
+        return torch.frombuffer((ctypes.c_float * count).from_address(ptr), dtype=F32)
+
+    def normalised(ptr, outer, C, inner, step):
+        t = at(ptr, step * (outer - 1) + C * inner if outer else 0).as_strided((outer, C, inner), (step, inner, 1))
+        return t, t.mean(1, keepdim=True), t.var(1, unbiased=False, keepdim=True)
+
+    class Lib:
+        @staticmethod
+        def fc3d_layer_norm_fwd(s, x, xt, w, b, wt, outer, C, inner, step, eps, relu, y, m, r):
+            t, mu, var = normalised(x, outer, C, inner, step)
+            ctypes.memmove(y, ((t - mu) / (var + eps).sqrt()).contiguous().data_ptr(), 4 * outer * C * inner)
+            return 0
+
+        @staticmethod
+        def fc3d_layer_norm_bwd_workspace(*a):
+            return 0
+
+        @staticmethod
+        def fc3d_layer_norm_bwd(s, dy, x, xt, w, b, wt, m, r, outer, C, inner, g_step, step, relu, dx, dw, db, ws):
+            t, mu, var = normalised(x, outer, C, inner, step)
+            g = at(dy, g_step * (outer - 1) + C * inner).as_strided((outer, C, inner), (g_step, inner, 1))
+            rs = 1 / (var + 1e-5).sqrt()
+            h = (t - mu) * rs
+            out = rs * (g - g.mean(1, keepdim=True) - h * (g * h).mean(1, keepdim=True))
+            ctypes.memmove(dx, out.contiguous().data_ptr(), 4 * outer * C * inner)
+            return 0
+    monkeypatch.setattr(ops, "_lib", Lib)
+    monkeypatch.setattr(ops, "_need_gpu_float", lambda t, what: 0)
+    monkeypatch.setattr(ops, "_raw_stream", lambda dev: 0)
+    monkeypatch.setattr(ops, "_get_device", lambda: -1)
+    pointer = torch.Tensor.data_ptr
+
+    def counted(t):
+        room[pointer(t)] = (t.untyped_storage().nbytes() - 4 * t.storage_offset()) // t.element_size()
+        return pointer(t)
+    monkeypatch.setattr(torch.Tensor, "data_ptr", counted)
+    base = torch.randn(3, 6, 4, 10)
+    x, dim = {"channels_last": (base.contiguous(memory_format=torch.channels_last), 1), "padded planes": (base[:, :3], 1),
+              "padded rows": (torch.randn(7, 20)[:, :9], -1), "copied": (base[:, :, :, ::2], 1), "dense": (base, 1)}[case]
+    g = torch.randn(3, 6, 4, 10)[tuple(slice(n) for n in x.shape)] if x.dim() == 4 else torch.randn(x.shape)
+    x = x.detach().requires_grad_()
+    want = formula(x.detach(), None, None, g, dim, 1e-5)["dx"]
+    for pack in (lambda t: t, lambda t: t.clone(memory_format=torch.contiguous_format)):
+        with torch.autograd.graph.saved_tensors_hooks(pack, lambda t: t):
+            y = ops.layer_norm(x, dim=dim)
+        (dx,) = torch.autograd.grad(y, x, g)
+        assert float((dx.double() - want).abs().max()) <= 1e-4
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: t.half()):
+        y = ops.layer_norm(x, dim=dim)
+    with pytest.raises(RuntimeError, match="came back"):
+        torch.autograd.grad(y, x, g)
+
+
+@gpu
+@pytest.mark.parametrize("shape,dim,cut", [((2, 16, 9, 7), 1, None), ((2, 48, 9, 7), 1, 16), ((40, 96), -1, 50)])
+def test_saved_tensors_on_the_host(shape, dim, cut):
+    from fc3d import ops
+    x, w, b, dy = (t.cuda() for t in inputs(shape, dim, F32, F32, 72))
+    if cut is None:
+        x = x.contiguous(memory_format=torch.channels_last)
+    else:
+        x, w, b, dy = x.narrow(dim, 0, cut), w[:cut], b[:cut], dy.narrow(dim, 0, cut)
+    leaves = [t.detach().requires_grad_() for t in (x, w, b)]
+    want = torch.autograd.grad(ops.layer_norm(*leaves, dim=dim, relu=True), leaves, dy)
+    with torch.autograd.graph.save_on_cpu(pin_memory=True):
+        y = ops.layer_norm(*leaves, dim=dim, relu=True)
+    for a, c, r in zip(torch.autograd.grad(y, leaves, dy), want, (x, w, b)):
+        # the same values in another order of the sums
+        assert float((a - c).abs().max()) <= KP * 8 * float(c.abs().max()) and a.shape == r.shape
