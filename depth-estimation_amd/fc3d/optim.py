@@ -13,14 +13,14 @@ def split_parameters(modules, leave=()):
     """(matrices, others): the modules' weights of two axes or more, which Muon takes, and all other parameters, among
     them everything below a submodule that `leave` names (the first layer, the head).  Each parameter once, in order."""
     modules = [modules] if isinstance(modules, torch.nn.Module) else list(modules)
+    # a shared parameter goes by all its names, in all modules
+    named = [(name, p) for module in modules for name, p in module.named_parameters(remove_duplicate=False)]
+    kept = {id(p) for name, p in named if any(name == n or name.startswith(n + ".") for n in leave)}
     matrices, others, seen = [], [], set()
-    for module in modules:
-        for name, p in module.named_parameters():
-            if id(p) in seen:
-                continue
+    for _, p in named:
+        if id(p) not in seen:
             seen.add(id(p))
-            kept = any(name == n or name.startswith(n + ".") for n in leave)
-            (others if kept or p.dim() < 2 else matrices).append(p)
+            (others if id(p) in kept or p.dim() < 2 else matrices).append(p)
     return matrices, others
 
 

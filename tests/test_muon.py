@@ -625,3 +625,27 @@ def test_tracing_is_refused():
         torch.jit.trace(lambda t: ops.orthogonalize(t), (torch.zeros(4, 4),), check_trace=False)
     with pytest.raises(RuntimeError, match="traced"):
         torch.jit.trace(lambda t: ops.muon_step([t], [t], [t]), (torch.zeros(4, 4),), check_trace=False)
+
+
+def test_shared_parameters_that_are_left_under_a_later_name():
+    from fc3d import optim
+
+    class Net(torch.nn.Module):
+        def __init__(self, shared=None):
+            super().__init__()
+            self.embed = torch.nn.Embedding(10, 4)
+            self.hidden = torch.nn.Linear(4, 4)
+            self.head = torch.nn.Linear(4, 10, bias=False)
+            self.head.weight = self.embed.weight
+            if shared is not None:
+                self.hidden.weight = shared
+    a = Net()
+    matrices, others = optim.split_parameters(a, leave=("head",))
+    assert [id(p) for p in matrices] == [id(a.hidden.weight)]
+    assert [id(p) for p in others] == [id(a.embed.weight), id(a.hidden.bias)]
+    b = Net(shared=a.hidden.weight)
+    b.last = b.hidden                                                  # one more name of a module in both
+    matrices, others = optim.split_parameters([a, b], leave=("head", "last"))
+    assert matrices == []
+    assert [id(p) for p in others] == [id(p) for p in (a.embed.weight, a.hidden.weight, a.hidden.bias, b.embed.weight, b.hidden.bias)]
+    assert len(optim.split_parameters([a, b])[0]) == 3
