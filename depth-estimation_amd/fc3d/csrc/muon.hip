@@ -200,13 +200,25 @@ __device__ __forceinline__ void split8(_Float16* p, size_t plane, const float (&
     *reinterpret_cast<half8*>(p + plane) = l;
 }
 
-// X and its transpose, scaled by sx / (norm + eps), zero beyond the matrix, one 64 x 64 tile per workgroup.
+// What the products need to know of a matrix's norm.
+struct Norm {
+    float rest;                       // see ns_prepare_kernel
+    int low;                          // the norm of X_0 is at most 2^-low
+};
+// Where eps is far above the norm, X starts small and its pairs would fall below fp16's range: after `steps` steps, each of
+// which multiplies it by 2^gain at most, X is kept times 2^lift.  (Up to 2^96, whose inverse leaves fp32 its precision.)
+__device__ __forceinline__ int lift(int low, float gain, int steps) {
+    const int e = (int)floorf((float)low - gain * (float)steps);
+    return e < 0 ? 0 : e > 96 ? 96 : e;
+}
+
+// X and its transpose, scaled by sx 2^lift / (norm + eps), zero beyond the matrix, one 64 x 64 tile per workgroup.
 // `exact` (16-bit input taken as it is): one plane that holds the input times a power of two, without rounding; the
-// remaining factor in [1, 2) goes to rho and into the products that read X.
+// remaining factor in [1, 2) goes to Norm::rest and into the products that read X.
 template <typename T>
 __global__ __launch_bounds__(256) void ns_prepare_kernel(const Matrix* __restrict__ t, int matrices, Blend k,
                                                          const double* __restrict__ parts, double eps, float sx, int exact,
-                                                         _Float16* __restrict__ planes, float* __restrict__ rho) {
+                                                         _Float16* __restrict__ planes, Norm* __restrict__ norms) {
     __shared__ float tile[64][65];
     __shared__ double red[4];
     const int lane = threadIdx.x & 63;
@@ -244,7 +256,12 @@ __global__ __launch_bounds__(256) void ns_prepare_kernel(const Matrix* __restric
     for (int q = 32; q > 0; q >>= 1) s += __shfl_xor(s, q, 64);
     if (lane == 0) red[threadIdx.x >> 6] = s;
     __syncthreads();
-    const double factor = (double)sx / (sqrt((red[0] + red[1]) + (red[2] + red[3])) + eps);
+    const double norm = sqrt((red[0] + red[1]) + (red[2] + red[3]));
+    int above = 0, below = 0;                                // norm + eps and norm, below 2^ these and not below half of it
+    frexp(norm + eps, &above);
+    frexp(norm, &below);
+    const int low = norm > 0.0 && norm < 1e300 && above - 1 > below ? above - 1 - below : 0;
+    const double factor = ldexp((double)sx / (norm + eps), lift(low, 0.0f, 0));
     int shift = 0;
     float rest = 1.0f;
     if (exact) {
@@ -255,7 +272,7 @@ __global__ __launch_bounds__(256) void ns_prepare_kernel(const Matrix* __restric
             rest = (float)factor;
         }
     }
-    if (block == 0 && threadIdx.x == 0) rho[w] = rest;
+    if (block == 0 && threadIdx.x == 0) norms[w] = Norm{rest, low};
 #pragma unroll
     for (int q = 0; q < 16; ++q) {
         const int fast = lane, slow = q * 4 + ty, r = e.tall ? fast : slow, c = e.tall ? slow : fast;
@@ -295,20 +312,31 @@ enum Kind : uint8_t { NONE, GRAM, POLY, MUL, APPLY };
 struct Op {
     uint8_t kind, src1, src2, dst;
     float alpha;                      // sum -> stored value (scales of the operands and of the result)
-    uint8_t use_rho, last;            // the first segment of an input taken as it is; APPLY: to the tensors
+    uint8_t exact, last;              // the first segment of an input taken as it is; APPLY: to the tensors
+    uint8_t from, to;                 // GRAM, APPLY: steps that X has behind it, and that the result has
 };
 constexpr int kPlans = 2;
 struct Launch {
     Op op[kPlans][2];                 // up to two products of a matrix that do not need each other
     float a, b;                       // POLY: Q = a I + b A + c A A, in units of the stored result
+    float gain;                       // log2 of the most that a step multiplies X by
     int out_type, step;               // step: weights := decay * weights - lr * result
     float decay;
     int matrices;
     const Matrix* table;
     _Float16* planes;
-    const float* rho;
+    const Norm* norms;
     float* sums;                      // Gram tiles of shared depth: [tile][share][TILE * TILE]
 };
+
+// The factor of a product's sums that depends on its matrix: X is kept lifted, and may lack Norm::rest
+__device__ __forceinline__ float alpha_of(const Op& o, const Norm& n, float gain) {
+    if (o.kind != GRAM && o.kind != APPLY) return o.alpha;
+    const float rest = o.exact ? n.rest : 1.0f;
+    const int up = lift(n.low, gain, o.from);
+    if (o.kind == GRAM) return ldexpf(o.alpha * (rest * rest), -2 * up);
+    return ldexpf(o.alpha * rest, (o.last ? 0 : lift(n.low, gain, o.to)) - up);
+}
 
 __device__ __forceinline__ _Float16* buffer(const Matrix& e, _Float16* planes, int id, int& ld, size_t& plane) {
     ld = id == BUF_X ? e.np : e.mp;
@@ -387,6 +415,7 @@ __global__ __launch_bounds__(WAVES * 64, TILE == 64 && WAVES == 4 ? 2 : 1) void 
     int n0 = tiles_of(k0, e.mp, e.np, e.split, TILE);
     const int w = find_matrix(lane < a.matrices ? n0 + tiles_of(k1, e.mp, e.np, e.split, TILE) : 0, block);
     e.from_lane(w);
+    const Norm norm = a.norms[w];                             // (on its way while the stages run)
     n0 = __builtin_amdgcn_readlane(n0, w);
     Op o = e.plan ? o10 : o00;
     if (block >= n0) {
@@ -587,8 +616,7 @@ __global__ __launch_bounds__(WAVES * 64, TILE == 64 && WAVES == 4 ? 2 : 1) void 
 
     // ---- the result.  The wavefronts that share a block's depth exchange their sums as they hold them, 16 bytes at a
     // time, and each is left with the whole sum of its rows.
-    float alpha = o.alpha;
-    if (o.use_rho) alpha *= o.kind == GRAM ? a.rho[w] * a.rho[w] : a.rho[w];
+    const float alpha = alpha_of(o, norm, a.gain);
     float4v sum[BLK * BLK][OWN];
     float4v* swap = reinterpret_cast<float4v*>(shared);
     const auto slot = [&](int to, int from, int q, int k) {   // of the share `from` (without the receiver's own) for wavefront `to`
@@ -792,8 +820,7 @@ __global__ __launch_bounds__(256) void ns_gram_sum_kernel(Launch a) {
     int ti, tj;
     upper_tile(block, (e.mp + TILE - 1) / TILE, ti, tj);
     const float4* from = reinterpret_cast<const float4*>(a.sums + ((size_t)e.sums0 + (size_t)block * e.split) * TILE * TILE);
-    float alpha = o.alpha;
-    if (o.use_rho) alpha *= a.rho[w] * a.rho[w];
+    const float alpha = alpha_of(o, a.norms[w], a.gain);
     constexpr int QUARTS = TILE * TILE / 4, EACH = QUARTS / 256 % 4 == 0 ? 4 : 3;
     static_assert(QUARTS % (256 * EACH) == 0, "loads in flight per lane");
     for (int g = 0; g < QUARTS / 256; g += EACH) {
@@ -1207,7 +1234,7 @@ struct PlanOps {
 // Every launch's products of one plan
 void ops_of(const Call& k, int plan, const Scales& s, bool exact, PlanOps& to) {
     to.count = 0;
-    uint8_t xt = BUF_XT0, p = BUF_P0;
+    uint8_t xt = BUF_XT0, p = BUF_P0, at = 0;                 // at: steps in front of the segment
     const auto put = [&](Op first, Op second) {
         to.op[to.count][0] = first;
         to.op[to.count++][1] = second;
@@ -1217,24 +1244,27 @@ void ops_of(const Call& k, int plan, const Scales& s, bool exact, PlanOps& to) {
     const int segment = k.out_type == FC3D_F32 ? 1 : s.segment;     // plan 0 of an fp32 result: one by one
     for (int step = 0; step < k.steps; ++step) {
         const bool begin = starts(segment, plan, step), end = step + 1 == k.steps || starts(segment, plan, step + 1);
-        const uint8_t rho = exact && first_segment;
-        if (begin) put(Op{GRAM, BUF_X, BUF_X, BUF_A, s.a / (s.x * s.x), rho, 0}, none);
+        const uint8_t whole = exact && first_segment, done = (uint8_t)step;
+        if (begin) {
+            at = done;
+            put(Op{GRAM, BUF_X, BUF_X, BUF_A, s.a / (s.x * s.x), whole, 0, at, at}, none);
+        }
         const uint8_t q = begin ? BUF_P0 : BUF_Q;              // the first of a segment is its running product too
         if (begin) p = BUF_P0;
-        put(Op{POLY, BUF_A, BUF_A, q, (float)k.c * s.q / (s.a * s.a), 0, 0}, none);
+        put(Op{POLY, BUF_A, BUF_A, q, (float)k.c * s.q / (s.a * s.a), 0, 0, 0, 0}, none);
         Op running = none;
         if (!begin) {
             const uint8_t np = p == BUF_P0 ? BUF_P1 : BUF_P0;
-            running = Op{MUL, p, q, np, 1.0f / s.q, 0, 0};
+            running = Op{MUL, p, q, np, 1.0f / s.q, 0, 0, 0, 0};
             p = np;
         }
         if (!end) {
-            put(Op{MUL, BUF_A, q, BUF_R, s.r / (s.a * s.q), 0, 0}, running);
-            put(Op{MUL, BUF_R, q, BUF_A, s.a / (s.r * s.q), 0, 0}, none);
+            put(Op{MUL, BUF_A, q, BUF_R, s.r / (s.a * s.q), 0, 0, 0, 0}, running);
+            put(Op{MUL, BUF_R, q, BUF_A, s.a / (s.r * s.q), 0, 0, 0, 0}, none);
         } else {
             if (running.kind != NONE) put(running, none);
             const uint8_t last = step + 1 == k.steps, nxt = xt == BUF_XT0 ? BUF_XT1 : BUF_XT0;
-            put(Op{APPLY, p, xt, nxt, (last ? 1.0f : s.x) / (s.q * s.x), rho, last}, none);
+            put(Op{APPLY, p, xt, nxt, (last ? 1.0f : s.x) / (s.q * s.x), whole, last, at, (uint8_t)(done + 1)}, none);
             xt = nxt;
             first_segment = false;
         }
@@ -1248,7 +1278,7 @@ struct Layout {
     int order[kMaxItems];             // the group's matrices as they are worked on: deep ones first, they take longest (numbers in the call)
     Shape shape[kMaxItems];           // in that order, like split
     int split[kMaxItems];
-    int64_t head() const { return (parts * 8 + kMaxItems * (4 + (int64_t)sizeof(Matrix)) + 255) / 256 * 256; }
+    int64_t head() const { return (parts * 8 + kMaxItems * (int64_t)(sizeof(Norm) + sizeof(Matrix)) + 255) / 256 * 256; }
     int64_t sums_at() const { return head() + (halves * 2 + 255) / 256 * 256; }
     bool small;                       // all of up to kSmall rows: sum_tiles is the number of partial Gram matrices
     int64_t bytes() const;
@@ -1427,13 +1457,13 @@ int run_group(const Call& k, const Layout& l, const Scales& sc, int count) {
     }
     double* squares = reinterpret_cast<double*>(k.ws);
     Matrix* table = reinterpret_cast<Matrix*>(k.ws + parts * 8);
-    float* rho = reinterpret_cast<float*>(table + kMaxItems);
+    Norm* norms = reinterpret_cast<Norm*>(table + kMaxItems);
     _Float16* planes = reinterpret_cast<_Float16*>(k.ws + l.head());
     const auto first = [&](auto zero) {
         typedef decltype(zero) T;
         FC3D_LAUNCH("ns_norm", ns_norm_kernel<T>, dim3((unsigned)parts), dim3(256), 0, k.s, t, k.blend, squares, table);
         FC3D_LAUNCH("ns_prepare", ns_prepare_kernel<T>, dim3((unsigned)prep), dim3(256), 0, k.s, table, count, k.blend, squares,
-                    k.eps, sc.x, (int)exact, planes, rho);
+                    k.eps, sc.x, (int)exact, planes, norms);
         return FC3D_OK;
     };
     if (const int rc = by_type(k.g_type, first)) return rc;
@@ -1454,19 +1484,20 @@ int run_group(const Call& k, const Layout& l, const Scales& sc, int count) {
     a.matrices = count;
     a.table = table;
     a.planes = planes;
-    a.rho = rho;
+    a.norms = norms;
+    a.gain = (float)std::log2(sc.gain);
     a.sums = reinterpret_cast<float*>(k.ws + l.sums_at());
     for (int i = 0; i < launches; ++i) {
-        bool gram = false, rho_gram = false, rho_apply = false;
+        bool gram = false, exact_gram = false, exact_apply = false;
         for (int p = 0; p < kPlans; ++p)
             for (int j = 0; j < 2; ++j) {
                 a.op[p][j] = i < ops[p].count ? ops[p].op[i][j] : Op{};
                 gram = gram || a.op[p][j].kind == GRAM;
-                rho_gram = rho_gram || (a.op[p][j].kind == GRAM && a.op[p][j].use_rho);
-                rho_apply = rho_apply || (a.op[p][j].kind == APPLY && a.op[p][j].use_rho);
+                exact_gram = exact_gram || (a.op[p][j].kind == GRAM && a.op[p][j].exact);
+                exact_apply = exact_apply || (a.op[p][j].kind == APPLY && a.op[p][j].exact);
             }
         // an input taken as it is has one plane (its plan is the only one: 16-bit results go through one plan, whatever their size)
-        const int p1 = rho_gram ? 1 : 2, p2 = rho_gram || rho_apply ? 1 : 2;
+        const int p1 = exact_gram ? 1 : 2, p2 = exact_gram || exact_apply ? 1 : 2;
         int64_t groups[kKernelCount], depth = 0;
         for (int c = 0; c < kKernelCount; ++c) groups[c] = groups_of(a, t, kKernels[c].tile);
         for (int j = 0; j < count; ++j) {

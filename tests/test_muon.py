@@ -649,3 +649,40 @@ def test_shared_parameters_that_are_left_under_a_later_name():
     assert matrices == []
     assert [id(p) for p in others] == [id(p) for p in (a.embed.weight, a.hidden.weight, a.hidden.bias, b.embed.weight, b.hidden.bias)]
     assert len(optim.split_parameters([a, b])[0]) == 3
+
+
+@gpu
+@pytest.mark.parametrize("dt", [F32, BF16, F16], ids=lambda t: str(t).replace("torch.", ""))
+@pytest.mark.parametrize("steps", [5, 8])
+def test_eps_far_above_the_norm(dt, steps):
+    """X starts at norm / eps of its usual size and grows by a step after step; what it loses stays a share of itself.  (In
+    fp16 only as far as the results are normal numbers.)"""
+    from fc3d import ops
+    for shape in ((100, 130), (96, 300), (300, 70)):
+        g = update(shape, "gauss", 700 + shape[0], dt)
+        norm = float(g.double().norm())
+        for ratio in ((1.0, 3.0, 40.0) if dt == F16 else (1.0, 3.0, 40.0, 1e3, 1e5, 1e8, 1e12, 1e20)):
+            near(ops.orthogonalize(g.cuda(), steps=steps, eps=ratio * norm), g, f"{shape} {ratio} {steps}", steps, eps=ratio * norm)
+        # beside a matrix that eps does not reach: no other bits than without eps
+        big = (g.float() * 2.0 ** 60).to(dt) if dt != F16 else g
+        pair = ops.orthogonalize([big.cuda(), g.cuda()], steps=steps, eps=norm * (1e5 if dt != F16 else 1.0))
+        near(pair[1], g, f"{shape} beside another", steps, eps=norm * (1e5 if dt != F16 else 1.0))
+        if dt != F16:
+            near(pair[0], big, f"{shape} large", steps)
+
+
+@gpu
+def test_step_with_eps_far_above_the_norm():
+    from fc3d import ops
+    w, g = (torch.randn(90, 200, generator=torch.Generator().manual_seed(710)) / 8), update((90, 200), "gauss", 711)
+    for ratio in (1e3, 1e7):
+        wd, md = w.cuda(), torch.zeros(90, 200, device="cuda")
+        u = 0.05 * g.double() + 0.95 * 0.05 * g.double()               # Nesterov's from a momentum of zero
+        eps = ratio * float(u.norm())
+        ops.muon_step([wd], [g.cuda()], [md], lr=ratio, eps=eps)
+        o = ns(u, torch.float64, eps=eps)
+        ref = w.double() - ratio * o
+        # as in test_step_against_definition
+        tol = ratio * float(o.norm()) * (bound(u.float(), o, eps=eps) + 2.0 ** -20)
+        tol += 5 * 2.0 ** -24 * float(ref.norm() + (w.double() - ref).norm())
+        assert float((wd.cpu().double() - ref).norm()) <= tol, ratio
