@@ -1160,6 +1160,8 @@ bool shape_of(int64_t rows, int64_t cols, Shape& s) {
     if (rows < 0 || cols < 0 || rows >= most || cols >= most) return false;
     s.m = rows < cols ? rows : cols;
     s.n = rows < cols ? cols : rows;
+    s.mp = (s.m + kSlice - 1) / kSlice * kSlice;
+    s.np = (s.n + kSlice - 1) / kSlice * kSlice;
     return (s.m / 64 + 2) * (s.n / 64 + 2) < (1 << 22);       // workgroups of a launch
 }
 
@@ -1355,9 +1357,7 @@ int layout_of(const Call& k, const int* list, int count, int planes, bool small,
         return prep >= (1 << 23) ? FC3D_ERANGE : FC3D_OK;
     }
     for (int i = 0; i < count; ++i) {
-        Shape& s = l.shape[i];
-        s.mp = (s.m + kSlice - 1) / kSlice * kSlice;
-        s.np = (s.n + kSlice - 1) / kSlice * kSlice;
+        const Shape& s = l.shape[i];
         l.parts += s.parts();
         l.halves += s.halves();
         prep += s.mp / 64 * (s.np / 64);
@@ -1540,18 +1540,31 @@ bool mixed(const Call& k) {
     return tiny && large;
 }
 
-// Matrices in groups of kMaxItems, one group after the other in the same workspace; `apart`: the tiny ones behind the rest
+// Matrices in groups of up to kMaxItems, one group after the other in the same workspace; `apart`: the tiny ones behind the
+// rest.  A group ends too where its buffers, eight times its weights in fp32, would pass a GiB: what fills that fills the
+// compute units several times over (32 matrices of 1024 x 1024), and 48 matrices of 4096 x 4096 would take 24 GiB.  `small`:
+// of matrices of up to kSmall rows alone, which then need no such buffers.
+constexpr int64_t kGroupBytes = (int64_t)1 << 30;
 template <typename F>
-int in_groups(const Call& k, bool apart, F&& f) {
+int in_groups(const Call& k, bool apart, bool small, F&& f) {
     int list[kMaxItems];
+    bool large = false;
+    for (int i = 0; i < k.count; ++i) large = large || rows_of(k, i) > kSmall;
     for (int turn = 0; turn < (apart ? 2 : 1); ++turn) {
         int count = 0;
+        int64_t bytes = 0;
         for (int i = 0; i < k.count; ++i) {
             if (apart && (rows_of(k, i) <= kTiny) != (turn == 1)) continue;
+            Shape s;
+            if (!shape_of(k.rows[i], k.cols[i], s)) return FC3D_ERANGE;
+            const int64_t own = small && (turn == 1 || !large) ? 0 : 2 * s.halves();
+            if (count == kMaxItems || (count > 0 && bytes + own > kGroupBytes)) {
+                if (const int rc = f(list, count)) return rc;
+                count = 0;
+                bytes = 0;
+            }
             list[count++] = i;
-            if (count < kMaxItems) continue;
-            if (const int rc = f(list, count)) return rc;
-            count = 0;
+            bytes += own;
         }
         if (count > 0)
             if (const int rc = f(list, count)) return rc;
@@ -1561,16 +1574,17 @@ int in_groups(const Call& k, bool apart, F&& f) {
 // The workspace is sized for every layout that a call with these sizes may take
 int size_of(const Call& k, size_t& bytes) {
     bytes = 0;
-    for (int apart = 0; apart <= (int)mixed(k); ++apart)
-        if (const int rc = in_groups(k, apart != 0, [&](const int* list, int count) {
-                for (int way = 0; way < 3; ++way) {
-                    Layout l = {};
-                    if (const int rc = layout_of(k, list, count, way == 1 ? 2 : 0, way == 2, l)) return rc;
-                    if ((size_t)l.bytes() > bytes) bytes = (size_t)l.bytes();
-                }
-                return (int)FC3D_OK;
-            }))
-            return rc;
+    for (int small = 0; small < 2; ++small)
+        for (int apart = 0; apart <= (int)(small && mixed(k)); ++apart)
+            if (const int rc = in_groups(k, apart != 0, small != 0, [&](const int* list, int count) {
+                    for (int planes = 0; planes <= 2; planes += 2) {
+                        Layout l = {};
+                        if (const int rc = layout_of(k, list, count, planes, small != 0, l)) return rc;
+                        if ((size_t)l.bytes() > bytes) bytes = (size_t)l.bytes();
+                    }
+                    return (int)FC3D_OK;
+                }))
+                return rc;
     return FC3D_OK;
 }
 
@@ -1578,7 +1592,7 @@ int run(const Call& k) {
     Scales sc = {};
     if (!scales_of(k, sc)) return FC3D_ERANGE;
     const bool small = small_of(k, sc.gain);
-    return in_groups(k, small && mixed(k), [&](const int* list, int count) {
+    return in_groups(k, small && mixed(k), small, [&](const int* list, int count) {
         Layout l = {};
         if (const int rc = layout_of(k, list, count, is_exact(k) ? 2 : 0, small, l)) return rc;
         return l.small ? run_small(k, l, count) : run_group(k, l, sc, count);

@@ -470,7 +470,8 @@ int fc3d_layer_norm_bwd(void *stream, const void *dy, const void *x, int x_type,
  * g[i], nothing else may overlap), rows, cols; they may be freed after the call.  A matrix must
  * have a row and a column.
  * FC3D_ERANGE: sizes beyond 2^23, or coefficients that let singular values grow beyond 16.
- * workspace: fc3d_orthogonalize_workspace() bytes, 256-byte aligned, need not be initialised;
+ * workspace: fc3d_orthogonalize_workspace() bytes (eight times a matrix in fp32 at most, several
+ * share up to 1 GiB at a time), 256-byte aligned, need not be initialised;
  * calls that may run at the same time need one each.                                          */
 size_t fc3d_orthogonalize_workspace(int count, const int64_t *rows, const int64_t *cols);
 int fc3d_orthogonalize(void *stream, int count, const void *const *g, void *const *out, const int64_t *rows,

@@ -686,3 +686,53 @@ def test_step_with_eps_far_above_the_norm():
         tol = ratio * float(o.norm()) * (bound(u.float(), o, eps=eps) + 2.0 ** -20)
         tol += 5 * 2.0 ** -24 * float(ref.norm() + (w.double() - ref).norm())
         assert float((wd.cpu().double() - ref).norm()) <= tol, ratio
+
+
+def workspace(shapes):
+    import ctypes
+    from fc3d import _native
+    n, I64 = len(shapes), ctypes.c_int64
+    return _native.load().fc3d_orthogonalize_workspace(n, (I64 * n)(*[s[0] for s in shapes]), (I64 * n)(*[s[1] for s in shapes]))
+
+
+def test_workspace_of_long_lists_is_bounded():
+    """Matrices go through the workspace group after group: a GiB and the sums of shared depth (256 tiles of 128 x 128 at
+    most), or what one matrix alone needs."""
+    most = 2 ** 30 + 2 ** 25
+    for shape, count in (((4096, 4096), 48), ((1024, 1024), 200), ((4096, 1024), 48), ((64, 40000), 48), ((9, 50), 1000)):
+        assert workspace([shape]) <= workspace([shape] * count) <= max(most, workspace([shape]))
+    assert workspace([(8192, 8192)] * 48) == workspace([(8192, 8192)])
+    assert workspace([(8192, 8192), (5, 7), (64, 288)]) <= workspace([(8192, 8192)]) + 2 ** 25
+    # as ever: lists that fit go in one group
+    assert workspace([(1024, 1024)] * 20) > 19 * workspace([(1024, 1024)])
+
+
+@gpu
+def test_lists_beyond_one_group_of_a_gib():
+    """2048 x 4096 takes 176 MiB: groups of five.  The same bits as the groups by themselves, nothing written behind the
+    workspace."""
+    import ctypes
+    from fc3d import _native
+    lib, I64, VP = _native.load(), ctypes.c_int64, ctypes.c_void_p
+    gen = torch.Generator(device="cuda").manual_seed(720)
+    gs = [torch.randn(2048, 4096, generator=gen, device="cuda").bfloat16() for _ in range(7)]
+
+    def call(gs):
+        n = len(gs)
+        size = workspace([tuple(g.shape) for g in gs])
+        ws = torch.full((size + 512,), 77, dtype=torch.uint8, device="cuda")
+        out = [torch.empty_like(g) for g in gs]
+        at = lambda ts: (VP * n)(*[t.data_ptr() for t in ts])  # noqa: E731
+        sizes = lambda d: (I64 * n)(*[g.shape[d] for g in gs])  # noqa: E731
+        assert (ws.data_ptr() + 256) % 256 == 0
+        assert lib.fc3d_orthogonalize(torch.cuda.current_stream().cuda_stream, n, at(gs), at(out), sizes(0), sizes(1), 1, 5, *COEFFS, 1e-7,
+                                      ws.data_ptr() + 256) == 0
+        torch.cuda.synchronize()
+        assert bool((ws[:256] == 77).all()) and bool((ws[256 + size:] == 77).all())
+        return out
+    together = call(gs)
+    for x, y in zip(together, call(gs[:5]) + call(gs[5:])):
+        assert torch.equal(x, y) and bool(torch.isfinite(x).all())
+    # singular values of a square Gaussian half: 0.67 to 1.21 of the polynomial, and a bf16 rounding
+    s = torch.linalg.svdvals(together[6].float())
+    assert 0.65 <= float(s[-1]) and float(s[0]) <= 1.22
