@@ -1398,12 +1398,22 @@ int64_t groups_of(const Launch& a, const Table& t, int tile) {
     return n;
 }
 
+// (the names tell the kernels apart in a profile: tile, and planes of the operands)
 template <int TILE, int WAVES>
 int product(const Call& k, const Launch& a, int64_t groups, int p1, int p2) {
+    constexpr const char* names[3] = {TILE == 64 ? "ns_product_64_1x1" : TILE == 96 ? "ns_product_96_1x1" : "ns_product_128_1x1",
+                                      TILE == 64 ? "ns_product_64_2x1" : TILE == 96 ? "ns_product_96_2x1" : "ns_product_128_2x1",
+                                      TILE == 64 ? "ns_product_64_2x2" : TILE == 96 ? "ns_product_96_2x2" : "ns_product_128_2x2"};
     const dim3 grid((unsigned)groups), block(WAVES * 64);
-    if (p1 == 1) FC3D_LAUNCH("ns_product", (ns_product_kernel<TILE, WAVES, 1, 1>), grid, block, 0, k.s, a);
-    else if (p2 == 1) FC3D_LAUNCH("ns_product", (ns_product_kernel<TILE, WAVES, 2, 1>), grid, block, 0, k.s, a);
-    else FC3D_LAUNCH("ns_product", (ns_product_kernel<TILE, WAVES, 2, 2>), grid, block, 0, k.s, a);
+    if (p1 == 1) FC3D_LAUNCH(names[0], (ns_product_kernel<TILE, WAVES, 1, 1>), grid, block, 0, k.s, a);
+    else if (p2 == 1) FC3D_LAUNCH(names[1], (ns_product_kernel<TILE, WAVES, 2, 1>), grid, block, 0, k.s, a);
+    else FC3D_LAUNCH(names[2], (ns_product_kernel<TILE, WAVES, 2, 2>), grid, block, 0, k.s, a);
+    return FC3D_OK;
+}
+template <int TILE>
+int gram_sum(const Call& k, const Launch& a, int64_t groups) {
+    constexpr const char* name = TILE == 64 ? "ns_gram_sum_64" : TILE == 96 ? "ns_gram_sum_96" : "ns_gram_sum_128";
+    FC3D_LAUNCH(name, ns_gram_sum_kernel<TILE>, dim3((unsigned)groups), dim3(256), 0, k.s, a);
     return FC3D_OK;
 }
 
@@ -1513,10 +1523,10 @@ int run_group(const Call& k, const Layout& l, const Scales& sc, int count) {
         for (int j = 0; j < count; ++j)
             if (a.op[t.e[j].plan][0].kind == GRAM && t.e[j].split > 1) sum_groups += tiles_of(MUL, t.e[j].mp, 0, 1, kKernels[c].tile);
         if (sum_groups) {
-            const dim3 grid((unsigned)sum_groups);
-            if (kKernels[c].tile == 64) FC3D_LAUNCH("ns_gram_sum", ns_gram_sum_kernel<64>, grid, dim3(256), 0, k.s, a);
-            else if (kKernels[c].tile == 96) FC3D_LAUNCH("ns_gram_sum", ns_gram_sum_kernel<96>, grid, dim3(256), 0, k.s, a);
-            else FC3D_LAUNCH("ns_gram_sum", ns_gram_sum_kernel<128>, grid, dim3(256), 0, k.s, a);
+            const int tile = kKernels[c].tile;
+            if (const int rc = tile == 64 ? gram_sum<64>(k, a, sum_groups) : tile == 96 ? gram_sum<96>(k, a, sum_groups)
+                                                                                       : gram_sum<128>(k, a, sum_groups))
+                return rc;
         }
     }
     return FC3D_OK;

@@ -736,3 +736,102 @@ def test_lists_beyond_one_group_of_a_gib():
     # singular values of a square Gaussian half: 0.67 to 1.21 of the polynomial, and a bf16 rounding
     s = torch.linalg.svdvals(together[6].float())
     assert 0.65 <= float(s[-1]) and float(s[0]) <= 1.22
+
+
+def ns_device(g, dt, eps=1e-7):
+    """The definition on the GPU, for sizes that take the CPU too long."""
+    a, b, c = COEFFS
+    x = g.to(dt)
+    tall = x.shape[0] > x.shape[1]
+    if tall:
+        x = x.t().contiguous()
+    x = x / (torch.linalg.vector_norm(x) + eps)
+    for _ in range(5):
+        s = torch.mm(x, x.t().contiguous())
+        x = a * x + torch.mm(b * s + c * torch.mm(s, s), x)
+    return x.t() if tall else x
+
+
+RAGGED = [(2003, 2153), (513, 113), (888, 929)]
+DEEP_128 = [(424, 2304), (71, 451), (437, 271), (2334, 2092), (64, 3595)]
+DEEP_96 = [(2933, 1964), (74, 11861), (1024, 148), (70, 4139), (312, 133)]
+
+
+@gpu
+@pytest.mark.parametrize("op,dt,shapes,kernels", [
+    ("orthogonalize", BF16, [(2370, 2019)], {"ns_product_96_1x1", "ns_product_96_2x2", "ns_product_128_2x1"}),
+    ("orthogonalize", BF16, [(135, 10871), (403, 172), (245, 68)], {"ns_product_64_1x1", "ns_gram_sum_64", "ns_product_96_2x1"}),
+    ("orthogonalize", BF16, RAGGED, {"ns_product_128_1x1", "ns_product_128_2x2", "ns_product_64_2x2", "ns_product_128_2x1"}),
+    ("orthogonalize", F16, RAGGED, {"ns_product_128_1x1", "ns_product_128_2x2", "ns_product_64_2x2", "ns_product_128_2x1"}),
+    ("orthogonalize", BF16, [(90, 150)], {"ns_product_64_2x1"}),
+    ("orthogonalize", F32, DEEP_96, {"ns_product_96_2x2", "ns_gram_sum_96", "ns_product_128_2x2"}),
+    ("step", BF16, [(129, 7250), (545, 258), (343, 1711)], {"ns_product_64_2x2", "ns_product_96_2x2"}),
+    ("step", BF16, DEEP_128, {"ns_product_128_2x2", "ns_gram_sum_128", "ns_product_64_2x2"}),
+    ("step", BF16, DEEP_96, {"ns_product_96_2x2", "ns_gram_sum_96"}),
+    ("step", F32, RAGGED, set()),
+], ids=lambda v: str(v).replace("torch.", "") if not isinstance(v, (list, set)) else str(len(v)))
+def test_every_product_kernel(op, dt, shapes, kernels):
+    """Every kernel that the rules pick, at sizes that are no multiples of its tile: the names in the profile say that it
+    ran, the definition what it should give, and guards that nothing beyond the tensors and the workspace is written."""
+    import ctypes
+    from fc3d import _native, ops, profiler
+    lib, n = _native.load(), len(shapes)
+    I64, VP, FL = ctypes.c_int64, ctypes.c_void_p, ctypes.c_float
+    pad, code = 64, {F32: 0, BF16: 1, F16: 2}[dt]
+    gen = torch.Generator(device="cuda").manual_seed(730 + n)
+
+    def guarded(values):
+        buf = torch.full((values.numel() + 2 * pad,), 512.0, dtype=values.dtype, device="cuda")
+        buf[pad:-pad] = values.reshape(-1)
+        return buf
+
+    def inside(buf, shape):
+        assert bool((buf[:pad] == 512.0).all()) and bool((buf[-pad:] == 512.0).all())
+        return buf[pad:-pad].view(shape)
+    at = lambda bufs: (VP * n)(*[b.data_ptr() + pad * b.element_size() for b in bufs])  # noqa: E731
+    rows, cols = (I64 * n)(*[s[0] for s in shapes]), (I64 * n)(*[s[1] for s in shapes])
+    size = lib.fc3d_orthogonalize_workspace(n, rows, cols)
+    ws = torch.full((size + 512,), 77, dtype=torch.uint8, device="cuda")
+    base, stream = ws.data_ptr() + 256, torch.cuda.current_stream().cuda_stream
+    assert base % 256 == 0
+    gs = [(1e-3 * torch.randn(s, generator=gen, device="cuda")).to(dt) for s in shapes]
+    gb = [guarded(g) for g in gs]
+    out = [guarded((torch.randn(s, generator=gen, device="cuda") / 16).to(dt)) for s in shapes]
+    old = [inside(o, s).double().clone() for o, s in zip(out, shapes)]
+    mom = [guarded(1e-3 * torch.randn(s, generator=gen, device="cuda")) for s in shapes]
+    before = [inside(m, s).double().clone() for m, s in zip(mom, shapes)]
+    lr, beta, decay = 0.02, 0.9, 0.998
+    profiler.report()
+    profiler.enable()
+    try:
+        if op == "step":
+            status = lib.fc3d_muon_step(stream, n, at(out), at(gb), at(mom), rows, cols, (FL * n)(*[lr] * n), code, code, beta, 1, decay, 5,
+                                        *COEFFS, 1e-7, base)
+        else:
+            status = lib.fc3d_orthogonalize(stream, n, at(gb), at(out), rows, cols, code, 5, *COEFFS, 1e-7, base)
+        ran = set(profiler.report())
+    finally:
+        profiler.enable(False)
+    torch.cuda.synchronize()
+    assert status == 0 and kernels <= ran, (status, ran)
+    assert bool((ws[:256] == 77).all()) and bool((ws[256 + size:] == 77).all())
+    for i, s in enumerate(shapes):
+        g, got = gs[i].double(), inside(out[i], s).double()
+        assert torch.equal(inside(gb[i], s), gs[i])
+        u, half = g, torch.finfo(dt).eps / 2
+        if op == "step":
+            m = beta * before[i] + (1 - beta) * g
+            # as in test_step_against_definition
+            off = (inside(mom[i], s).double() - m).abs()
+            assert bool((off <= 4 * 2.0 ** -24 * (beta * before[i].abs() + (1 - beta) * g.abs()) + 2.0 ** -149).all()), s
+            u = (1 - beta) * g + beta * m
+        ref = ns_device(u, torch.float64)
+        norm = float(ref.norm())
+        tol = 4 * float((ns_device(u, F32).double() - ref).norm()) / norm + 2.0 ** -20 + \
+            (0.0 if dt == F32 else half + 6e-3 / math.sqrt(min(s)))
+        if op == "step":
+            want = decay * old[i] - lr * ref
+            tol = lr * norm * (tol + 2.0 ** -20) + (half + 4 * 2.0 ** -24) * float(want.norm() + (old[i] - want).norm())
+        else:
+            want, tol = ref, tol * norm
+        assert float((got - want).norm()) <= tol, (s, float((got - want).norm()), tol)
