@@ -659,3 +659,55 @@ def test_saved_tensors_on_the_host(shape, dim, cut):
     for a, c, r in zip(torch.autograd.grad(y, leaves, dy), want, (x, w, b)):
         # the same values in another order of the sums
         assert float((a - c).abs().max()) <= KP * 8 * float(c.abs().max()) and a.shape == r.shape
+
+
+# Row lengths of the kernels that SHAPES leaves out: 2049 to 4096 (256 lanes a row forward, 512 backward), and 8193 to
+# 16383 with rows that end inside a vector.
+WIDTHS = [(600, 2560), (1030, 4096), (521, 3001), (700, 2049), (5, 9001), (3, 16383)]
+
+
+@gpu
+@pytest.mark.parametrize("types", TYPES, ids=lambda t: "-".join(str(v).replace("torch.", "") for v in t))
+@pytest.mark.parametrize("shape", WIDTHS, ids=lambda v: "x".join(map(str, v)))
+def test_more_row_lengths(shape, types):
+    test_against_formula(shape, -1, types)
+
+
+# More positions than the workgroups of a launch hold at a time, two to six rounds of them, for every number of lanes per
+# row and of channel groups: the next row on its way, the LDS areas that take turns, the last round part full.
+ROUNDS = [((90001, 33), -1), ((90001, 96), -1), ((50001, 200), -1), ((25001, 500), -1), ((12001, 1000), -1), ((6001, 2000), -1),
+          ((3001, 3999), -1), ((3001, 5000), -1), ((2999, 9001), -1), ((1300, 16384), -1),
+          ((5, 7, 601, 701), 1), ((5, 20, 301, 401), 1), ((5, 50, 201, 301), 1), ((5, 100, 101, 301), 1), ((5, 200, 101, 131), 1),
+          ((5, 500, 81, 101), 1), ((5, 900, 61, 101), 1), ((3001, 40, 5), 1), ((2001, 300, 1, 2), 1)]
+
+
+@gpu
+@pytest.mark.parametrize("types", [(F32, F32), (BF16, BF16), (F16, F32)], ids=lambda t: "-".join(str(v).replace("torch.", "") for v in t))
+@pytest.mark.parametrize("shape,dim", ROUNDS, ids=lambda v: "x".join(map(str, v)) if isinstance(v, tuple) else None)
+def test_several_rounds(shape, dim, types):
+    """Chains of the sums over positions: six rounds of four positions a lane, 64 row groups or wavefronts, 32 + 32 partial
+    sums: 128 at most, as above.  The formula on the device.
+
+    Which values pass the ReLU is read off y, except where y is zero in fp16 and the value before it may be positive and
+    below the type's range (half of 2^-24; among millions of values a few are).  The bounds bear both there: with d the
+    gradients in question, dx moves by rs (|d w| + mean|d w| + |h| mean|d w h|), dw by the sum of |d h|, db by that of |d|."""
+    from fc3d import ops
+    dt, wdt = types
+    x, w, b, dy = (t.cuda() for t in inputs(shape, dim, dt, wdt, 13))
+    for relu in (False, True):
+        y, (dx, dw, db) = run(ops, x, w, b, dy, dim, relu)
+        mask = (y.detach() > 0).double() if relu else None
+        r = formula(x, w, b, dy, dim, 1e-5, mask)
+        if relu and dt == F16:
+            pre = formula(x, w, b, None, dim, 1e-5)
+            d = (dy.double() * ((y.detach() == 0) & (pre["y"] > -pre["ey"]))).abs().movedim(dim, -1)
+            xm = x.double().movedim(dim, -1)
+            rs = 1 / torch.sqrt(xm.var(-1, unbiased=False, keepdim=True) + 1e-5)
+            h = (rs * (xm - xm.mean(-1, keepdim=True))).abs()
+            gw = d * w.double().abs()
+            r["edx"] += (rs * (gw + gw.mean(-1, keepdim=True) + h * (gw * h).mean(-1, keepdim=True))).movedim(-1, dim)
+            pos = tuple(range(xm.dim() - 1))
+            r["edw"] += (d * h).sum(pos)
+            r["edb"] += d.sum(pos)
+        for name, got, t in (("y", y, dt), ("dx", dx, dt), ("dw", dw, wdt), ("db", db, wdt)):
+            close(got, r[name].cpu(), r["e" + name].cpu(), t, f"{name} relu={relu}")
