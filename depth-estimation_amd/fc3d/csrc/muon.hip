@@ -1167,14 +1167,15 @@ bool shape_of(int64_t rows, int64_t cols, Shape& s) {
 
 float pow2_below(double bound) { return (float)std::exp2(14.0 - std::ceil(std::log2(bound))); }     // bound * it <= 2^14
 
-// How many steps the Gram form takes at once.  A segment of L amplifies what it rounded gain^(2L)-fold: bf16 results
-// bear five of the usual steps (gain 3.4), fp16 and fp32 ones three; steps that amplify more go two by two and, of fp32
-// results, one by one.  So do more than five steps: near one the usual polynomial spreads neighbouring values (its slope is
-// -1.4 at 0.75), and every further step amplifies what a segment rounded.
+// How many steps the Gram form takes at once.  A segment of L amplifies what it rounded gain^(2L)-fold: bf16 results bear
+// five of the usual steps (gain 3.4), fp16 and fp32 ones three; steps that amplify more go two by two and, of fp32 results,
+// one by one.  So do more than five steps: near one the usual polynomial spreads neighbouring values (its slope is -1.4 at
+// 0.75), and every further step amplifies what a segment rounded (ten steps of a bf16 result five by five left it off by
+// 1.1e-3 in front of its rounding, 1.7e-3).
 constexpr double kGain = 4.0;
 int segment_of(const Call& k, double gain) {                  // the longest one: the running products' scale follows from it
     const int apart = k.out_type == FC3D_F32 ? 1 : 2;
-    const int most = gain > kGain ? apart : k.out_type == FC3D_BF16 ? 5 : k.steps <= 5 ? 3 : apart;
+    const int most = gain > kGain || k.steps > 5 ? apart : k.out_type == FC3D_BF16 ? 5 : 3;
     return k.steps < most ? k.steps : most;
 }
 // Whether small matrices take all steps at once in 64 bits: what is rounded (1e-16) stays under 1e-5 when amplified, which

@@ -835,3 +835,41 @@ def test_every_product_kernel(op, dt, shapes, kernels):
         else:
             want, tol = ref, tol * norm
         assert float((got - want).norm()) <= tol, (s, float((got - want).norm()), tol)
+
+
+def ns_gram32(g, steps, segment):
+    """The definition's Gram form in fp32, `segment` steps to a Gram matrix."""
+    a, b, c = COEFFS
+    x = g.float()
+    x = x / (x.norm() + 1e-7)
+    tall = x.shape[0] > x.shape[1]
+    if tall:
+        x = x.t()
+    eye = torch.eye(x.shape[0])
+    for start in range(0, steps, segment):
+        s, p = x @ x.t(), eye
+        for _ in range(min(segment, steps - start)):
+            q = a * eye + b * s + c * (s @ s)
+            p, s = q @ p, q @ s @ q
+        x = p @ x
+    return x.t() if tall else x
+
+
+@gpu
+@pytest.mark.parametrize("dt", [BF16, F16], ids=lambda t: str(t).replace("torch.", ""))
+@pytest.mark.parametrize("steps", [6, 8, 10, 16])
+def test_many_steps_lose_no_more_than_their_rounding(dt, steps):
+    """As test_half_precision_results_lose_no_more_than_their_rounding, with what may be lost in front of the rounding taken
+    from fp32 again, four times: from fp32 products step by step and from the Gram form of two steps at a time in fp32."""
+    from fc3d import ops
+    for m, n in ((128, 300), (300, 77), (256, 1024)):
+        gen = torch.Generator().manual_seed(m + n)
+        g = (1e-3 * (torch.randn(m, 4, generator=gen) @ torch.randn(4, n, generator=gen) +
+                     0.1 * torch.randn(m, n, generator=gen))).to(dt)
+        ref = ns(g, torch.float64, steps)
+        norm = float(ref.norm())
+        r = float((ref.to(dt).double() - ref).norm()) / norm
+        e = 4 * max(float((y.double() - ref).norm()) / norm for y in (ns(g, F32, steps), ns_gram32(g, steps, 2))) + 2.0 ** -20
+        tol = math.sqrt((r * r + e * e) * (1 + 8 / math.sqrt(m * n)))
+        off = float((ops.orthogonalize(g.cuda(), steps=steps).cpu().double() - ref).norm()) / norm
+        assert off <= tol, (m, n, off, tol, r, e)
