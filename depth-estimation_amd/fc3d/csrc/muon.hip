@@ -17,11 +17,11 @@
 // fp32 matrix instructions take.  Forming A squares the singular values, so a segment of L Gram steps loses the
 // directions whose share of A is below its rounding, amplified a^(2L)-fold.  Measured against 64 bits on a few strong
 // directions over a noise floor (rank 4 and noise of 0.3 to 0.001, 128 x 128 to 2048 x 8192): five steps at once cost
-// 1e-4 to 2e-4 of the result, a tenth of a bf16 result's rounding (1.7e-3) but as much as an fp16 result's (2.1e-4).  So
+// 1e-4 to 2e-4 of the result, an eighth of a bf16 result's rounding (1.7e-3) but as much as an fp16 result's (2.1e-4).  So
 // bf16 results take all five at once, fp16 ones two and three (2e-6 to 4e-5, what fp32 products are off by there; 8e-5 at
 // 2048 x 8192, where those are off by 1.3e-4).  For fp32 results the segments are of two and three steps too, or of one for
 // matrices that are nearly square (n < 2 m, where the smallest singular values sit near zero) and for those of up to 64
-// rows (where the squares saved are cheap): 0.3 to 1.5 times the error of fp32 products on the same inputs (512 x 4608
+// rows (where the squares saved are cheap): 0.3 to 1.9 times the error of fp32 products on the same inputs (512 x 4608
 // without structure 1.4e-6 against 4.3e-6, 128 x 300 of rank 4 and noise of 0.1 3.8e-6 against 2.6e-6); 64 x 288 2.5e-8
 // (1.5e-6), worked on in 64 bits.
 #include "fc3d_common.h"

@@ -1335,7 +1335,7 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
     x: float32, bfloat16 or float16, any number of axes; dim=-1 for sequences, dim=1 for NCHW images (dense or
     channels_last).  x is read through its strides where the other axes are walked with one stride, and copied
     otherwise; y keeps the memory order.  weight, bias: [x.shape[dim]], in x's type or float32 (both alike), or None.
-    Statistics and sums are float32; differentiable once w.r.t. x, weight and bias, bit-reproducible."""
+    Statistics and sums are float32; differentiable once w.r.t. x, weight and bias (in reverse mode), bit-reproducible."""
     code = _need_gpu_float(x, "x")
     nd = x.dim()
     if nd == 0 or not -nd <= dim < nd:
@@ -1371,7 +1371,9 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
     return _norm_forward(x, weight, bias, eps, dim, bool(relu), False)[0]
 
 
-NS_COEFFICIENTS = (3.4445, -4.7750, 2.0315)     # one step takes small singular values up by 3.4, large ones near one
+# K. Jordan et al., Muon: an optimizer for hidden layers in neural networks (2024): one step takes small singular values up
+# by 3.4, large ones near one
+NS_COEFFICIENTS = (3.4445, -4.7750, 2.0315)
 
 
 def _matrix_order(t):
@@ -1442,8 +1444,8 @@ def orthogonalize(g, steps: int = 5, coefficients=NS_COEFFICIENTS, eps: float = 
 
     g: float32, bfloat16 or float16 tensors of two axes or more on one GPU (a convolution's weight is
     [out, in * kh * kw]), any sizes and strides; results in their shapes and types.  What is rounded to the result is
-    about as exact as fp32 products make it; in front of a bf16 rounding a tenth of that rounding may be lost, a
-    quarter of it for matrices of 17 to 64 rows beside larger ones.  No gradient."""
+    about as exact as fp32 products make it; in front of a bf16 rounding an eighth of that rounding may be lost, a
+    quarter of it for matrices of 17 to 64 rows beside larger ones.  No gradient; not to be traced."""
     _not_traced("orthogonalize")
     single = isinstance(g, torch.Tensor)
     mats = [g] if single else list(g)
