@@ -17,9 +17,10 @@
 // fp32 matrix instructions take.  Forming A squares the singular values, so a segment of L Gram steps loses the
 // directions whose share of A is below its rounding, amplified a^(2L)-fold.  Measured against 64 bits on a few strong
 // directions over a noise floor (rank 4 and noise of 0.3 to 0.001, 128 x 128 to 2048 x 8192): five steps at once cost
-// 1e-4 to 2e-4 of the result, an eighth of a bf16 result's rounding (1.7e-3) but as much as an fp16 result's (2.1e-4).  So
-// bf16 results take all five at once, fp16 ones two and three (2e-6 to 4e-5, what fp32 products are off by there; 8e-5 at
-// 2048 x 8192, where those are off by 1.3e-4).  For fp32 results the segments are of two and three steps too, or of one for
+// 1e-4 to 2e-4 of the result (rank 1: up to 5e-4 from 129 rows on, 1.4e-3 for 17), a part of a bf16 result's rounding
+// (1.7e-3) but more than an fp16 result's (2.1e-4).  So bf16 results of more than 128 rows take all five at once, smaller
+// ones and fp16 two and three (2e-6 to 4e-5, what fp32 products are off by there; 8e-5 at 2048 x 8192, where those are off
+// by 1.3e-4).  For fp32 results the segments are of two and three steps too, or of one for
 // matrices that are nearly square (n < 2 m, where the smallest singular values sit near zero) and for those of up to 64
 // rows (where the squares saved are cheap): 0.3 to 1.9 times the error of fp32 products on the same inputs (512 x 4608
 // without structure 1.4e-6 against 4.3e-6, 128 x 300 of rank 4 and noise of 0.1 3.8e-6 against 2.6e-6); 64 x 288 2.5e-8
@@ -1219,10 +1220,13 @@ bool scales_of(const Call& k, Scales& s) {
     return true;
 }
 
-// Plan 0 goes through segments of `segment` steps, plan 1 (fp16, and large matrices in fp32) through one of two steps and
-// one of three.
+// Plan 0 goes through segments of `segment` steps, plan 1 through one of two steps and one of three: fp16, large matrices in
+// fp32, and matrices of up to kFew rows in bf16, whose results five steps at once would leave further off than their rounding
+// allows (rank 1 and noise of 0.001, in front of a rounding of 1.7e-3: 17 rows 1.4e-3, 64 6.5e-4, 128 5.1e-4, 256 3.9e-4).
+constexpr int kFew = 128;
 int plan_of(const Call& k, double gain, const Shape& s) {
-    if (gain > kGain || k.steps > 5 || k.out_type == FC3D_BF16) return 0;
+    if (gain > kGain || k.steps > 5) return 0;
+    if (k.out_type == FC3D_BF16) return s.m <= kFew;
     return k.out_type == FC3D_F16 || (s.n >= 2 * s.m && s.m > 64);
 }
 bool starts(int segment, int plan, int step) {
@@ -1499,16 +1503,17 @@ int run_group(const Call& k, const Layout& l, const Scales& sc, int count) {
     a.gain = (float)std::log2(sc.gain);
     a.sums = reinterpret_cast<float*>(k.ws + l.sums_at());
     for (int i = 0; i < launches; ++i) {
-        bool gram = false, exact_gram = false, exact_apply = false;
+        // An input taken as it is has one plane (the other is zero).  It is left out where no product of the launch needs it.
+        bool gram = false;
+        int p1 = 1, p2 = 1;
         for (int p = 0; p < kPlans; ++p)
             for (int j = 0; j < 2; ++j) {
-                a.op[p][j] = i < ops[p].count ? ops[p].op[i][j] : Op{};
-                gram = gram || a.op[p][j].kind == GRAM;
-                exact_gram = exact_gram || (a.op[p][j].kind == GRAM && a.op[p][j].exact);
-                exact_apply = exact_apply || (a.op[p][j].kind == APPLY && a.op[p][j].exact);
+                const Op& o = a.op[p][j] = i < ops[p].count ? ops[p].op[i][j] : Op{};
+                if (o.kind == NONE) continue;
+                gram = gram || o.kind == GRAM;
+                if (!(o.exact && o.kind == GRAM)) p1 = 2;
+                if (!o.exact) p2 = 2;
             }
-        // an input taken as it is has one plane (its plan is the only one: 16-bit results go through one plan, whatever their size)
-        const int p1 = exact_gram ? 1 : 2, p2 = exact_gram || exact_apply ? 1 : 2;
         int64_t groups[kKernelCount], depth = 0;
         for (int c = 0; c < kKernelCount; ++c) groups[c] = groups_of(a, t, kKernels[c].tile);
         for (int j = 0; j < count; ++j) {
@@ -1539,7 +1544,7 @@ bool off_align(const void* p, int type) { return (reinterpret_cast<uintptr_t>(p)
 // Matrices of up to kTiny rows in a list with larger ones go through three launches of their own in 64 bits: a result of a
 // few rows averages little.  Pairs of fp16 values left some fp32 results three times as far off as fp32 products do (2.2e-6
 // against 6e-7), and a bf16 result's five steps at once cost up to 2e-3, as much as its rounding, where its rows were nearly
-// dependent (rank 1 and noise of 0.01, 2 to 8 rows; 4e-4 from 17 rows on).  One tile of rows: 20 us for all of them together.
+// dependent (rank 1 and noise of 0.01, 2 to 8 rows).  One tile of rows: 20 us for all of them together.
 constexpr int kTiny = 16;
 int64_t rows_of(const Call& k, int i) { return k.rows[i] < k.cols[i] ? k.rows[i] : k.cols[i]; }
 bool mixed(const Call& k) {

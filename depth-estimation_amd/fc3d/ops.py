@@ -1444,8 +1444,8 @@ def orthogonalize(g, steps: int = 5, coefficients=NS_COEFFICIENTS, eps: float = 
 
     g: float32, bfloat16 or float16 tensors of two axes or more on one GPU (a convolution's weight is
     [out, in * kh * kw]), any sizes and strides; results in their shapes and types.  What is rounded to the result is
-    about as exact as fp32 products make it; in front of a bf16 rounding an eighth of that rounding may be lost, a
-    quarter of it for matrices of 17 to 64 rows beside larger ones.  No gradient; not to be traced."""
+    about as exact as fp32 products make it; in front of a bf16 rounding up to a third of that rounding may be lost
+    (matrices of more than 128 rows).  No gradient; not to be traced."""
     _not_traced("orthogonalize")
     single = isinstance(g, torch.Tensor)
     mats = [g] if single else list(g)

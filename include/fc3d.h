@@ -465,7 +465,7 @@ int fc3d_layer_norm_bwd(void *stream, const void *dy, const void *x, int x_type,
  *   X = G / (|G|_F + eps), then `steps` times  X <- a X + (b A + c A A) X  with A = X X^T
  * (of the transpose where rows > cols), and out = X.  Evaluated in the Gram form with every
  * operand a pair of fp16 values and fp32 sums: about as exact as fp32 products in front of an
- * fp32 or fp16 rounding, to a quarter of the rounding in front of a bf16 one.  HOST arrays:
+ * fp32 or fp16 rounding, to a third of the rounding in front of a bf16 one.  HOST arrays:
  * g, out (device pointers to dense row-major [rows][cols] tensors of `type`; out[i] may be
  * g[i], nothing else may overlap), rows, cols; they may be freed after the call.  A matrix must
  * have a row and a column.

@@ -760,8 +760,8 @@ DEEP_96 = [(2933, 1964), (74, 11861), (1024, 148), (70, 4139), (312, 133)]
 @gpu
 @pytest.mark.parametrize("op,dt,shapes,kernels", [
     ("orthogonalize", BF16, [(2370, 2019)], {"ns_product_96_1x1", "ns_product_96_2x2", "ns_product_128_2x1"}),
-    ("orthogonalize", BF16, [(135, 10871), (403, 172), (245, 68)], {"ns_product_64_1x1", "ns_gram_sum_64", "ns_product_96_2x1"}),
-    ("orthogonalize", BF16, RAGGED, {"ns_product_128_1x1", "ns_product_128_2x2", "ns_product_64_2x2", "ns_product_128_2x1"}),
+    ("orthogonalize", BF16, [(135, 10871), (403, 172), (245, 130)], {"ns_product_64_1x1", "ns_gram_sum_64", "ns_product_96_2x1"}),
+    ("orthogonalize", BF16, RAGGED, {"ns_product_128_1x1", "ns_product_128_2x2", "ns_product_64_2x2"}),
     ("orthogonalize", F16, RAGGED, {"ns_product_128_1x1", "ns_product_128_2x2", "ns_product_64_2x2", "ns_product_128_2x1"}),
     ("orthogonalize", BF16, [(90, 150)], {"ns_product_64_2x1"}),
     ("orthogonalize", F32, DEEP_96, {"ns_product_96_2x2", "ns_gram_sum_96", "ns_product_128_2x2"}),
@@ -873,3 +873,42 @@ def test_many_steps_lose_no_more_than_their_rounding(dt, steps):
         tol = math.sqrt((r * r + e * e) * (1 + 8 / math.sqrt(m * n)))
         off = float((ops.orthogonalize(g.cuda(), steps=steps).cpu().double() - ref).norm()) / norm
         assert off <= tol, (m, n, off, tol, r, e)
+
+
+@gpu
+@pytest.mark.parametrize("m", [17, 24, 40, 64, 100, 128])
+def test_one_direction_over_little_noise_in_bf16(m):
+    """Matrices of few rows beside a large one, the sum of squares over twenty of them; otherwise as
+    test_half_precision_results_lose_no_more_than_their_rounding."""
+    from fc3d import ops
+    gs = []
+    for i in range(20):
+        n = (m, m + 1, m + 8, 2 * m, 200)[i % 5]
+        gen = torch.Generator().manual_seed(800 + m + i)
+        x = torch.randn(m, 1, generator=gen) @ torch.randn(1, n, generator=gen) + (0.003, 0.001)[i % 2] * torch.randn(m, n, generator=gen)
+        gs.append((x.t() if i % 3 == 0 else x).contiguous().bfloat16())
+    out = ops.orthogonalize([g.cuda() for g in gs] + [update((150, 200), "gauss", 799, BF16).cuda()])
+    off = allowed = count = 0.0
+    for x, g in zip(out, gs):
+        ref = ns(g, torch.float64)
+        x2 = ns(g, torch.float64, 2)
+        x2 = x2.t() if x2.shape[0] > x2.shape[1] else x2
+        r = float((ref.bfloat16().double() - ref).norm())
+        e = 4 * float((ns(g, F32).double() - ref).norm()) + 2.0 ** -20 * float(ref.norm())
+        e += second_segment_slope() * 2.0 ** -22 * float((x2 @ x2.t()).norm())
+        off += float((x.cpu().double() - ref).norm()) ** 2
+        allowed += r * r + e * e
+        count += g.numel()
+    assert off <= allowed * (1 + 8 / math.sqrt(count)), (math.sqrt(off / allowed), count)
+
+
+@gpu
+def test_plans_of_few_and_of_many_rows_side_by_side():
+    """bf16 matrices of up to 128 rows and of more go through other sequences of products in the same launches."""
+    from fc3d import ops
+    gs = [update(s, "gauss", 820 + i, BF16) for i, s in enumerate([(128, 200), (129, 200), (70, 300), (300, 140), (20, 500), (500, 65)])]
+    for g, x in zip(gs, ops.orthogonalize([g.cuda() for g in gs])):
+        near(x, g, f"{tuple(g.shape)}")
+    for steps in (1, 2, 3, 4):
+        for g, x in zip(gs, ops.orthogonalize([g.cuda() for g in gs], steps=steps)):
+            near(x, g, f"{tuple(g.shape)} {steps}", steps)
