@@ -198,3 +198,19 @@ def test_graph_of_a_block_and_its_step(monkeypatch):
         torch.cuda.synchronize()
         for a, b in zip(list(out) + [wg, mg], list(want) + [we, me]):
             assert torch.equal(a, b), k
+
+
+@gpu
+@pytest.mark.timeout(300)
+def test_traced_network(monkeypatch):
+    """A frozen network traced for serving gives what the network gives: the norms are recorded as calls.  Other convolution
+    kernels may be picked in the traced one: sums of up to 9 * 512 products in another order, through 23 convolutions."""
+    monkeypatch.setenv("MIOPEN_FIND_MODE", "FAST")
+    from fc3d import nets
+    torch.manual_seed(7)
+    net = nets.UNet_z(norm="layer").cuda().eval().requires_grad_(False)
+    x = torch.rand(2, 32, 48, 1, device="cuda")
+    traced = torch.jit.trace(net, (torch.rand(2, 32, 48, 1, device="cuda"),), check_trace=False)
+    assert str(traced.inlined_graph).count("^LayerNormFn") == sum(isinstance(m, nets.ChannelNorm) for m in net.modules())
+    want = net(x)
+    assert float((traced(x) - want).abs().max()) <= 23 * (9 * 512) ** 0.5 * 2.0 ** -24 * 16 * float(want.abs().max())
