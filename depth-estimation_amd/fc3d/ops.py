@@ -1249,13 +1249,13 @@ def _norm_forward(x, weight, bias, eps, dim, relu, want_stats):
     p_code = code if p is None or p.dtype == x.dtype else 0
     n = outer * inner
     stats = torch.empty(2 * n, dtype=torch.float32, device=x.device) if want_stats else None
-    at = stats.data_ptr() if want_stats else None
+    x_at, at = xd.data_ptr(), stats.data_ptr() if want_stats else None
     dev = x.get_device()
     ctx = None if dev == _get_device() else _on_device(x.device)
     if ctx is not None:
         ctx.__enter__()
     try:
-        status = _lib.fc3d_layer_norm_fwd(_raw_stream(dev) if _raw_stream is not None else _stream(), xd.data_ptr(), code,
+        status = _lib.fc3d_layer_norm_fwd(_raw_stream(dev) if _raw_stream is not None else _stream(), x_at, code,
                                           weight.data_ptr() if weight is not None else None,
                                           bias.data_ptr() if bias is not None else None, p_code, outer, C, inner, step, eps,
                                           relu, y.data_ptr(), at, at + 4 * n if want_stats else None)
@@ -1264,7 +1264,7 @@ def _norm_forward(x, weight, bias, eps, dim, relu, want_stats):
             ctx.__exit__(None, None, None)
     if status:
         _check(status, "fc3d_layer_norm_fwd")
-    return y, xd, stats, (dim, last, relu, outer, C, inner, step, code, p_code, dev, xd.stride() if want_stats else None)
+    return y, xd, stats, (dim, last, relu, outer, C, inner, step, code, p_code, dev, (x_at, at, xd.stride()) if want_stats else None)
 
 
 class LayerNormFn(torch.autograd.Function):
@@ -1285,14 +1285,16 @@ class LayerNormFn(torch.autograd.Function):
     @staticmethod
     def gradients(ctx, dy):
         xd, weight, bias, stats = ctx.saved_tensors
-        dim, last, relu, outer, C, inner, x_step, code, p_code, dev, strides = ctx.meta
+        dim, last, relu, outer, C, inner, x_step, code, p_code, dev, saved = ctx.meta
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
-        # hooks on saved tensors may hand back a copy in another memory order (save_on_cpu does)
-        if xd.dtype != dy.dtype or stats.dtype != torch.float32 or xd.get_device() != dev or stats.get_device() != dev:
-            raise RuntimeError(f"layer_norm: its saved tensors came back as {xd.dtype} and {stats.dtype} on {xd.device} and "
-                               f"{stats.device}")
-        if xd.stride() != strides:
+        x_at, at = xd.data_ptr(), stats.data_ptr()
+        if x_at != saved[0] or at != saved[1] or xd.stride() != saved[2] or xd.dtype != dy.dtype:
+            # hooks on saved tensors handed back a copy, which may be in another memory order (save_on_cpu's is)
+            if xd.dtype != dy.dtype or stats.dtype != torch.float32 or xd.get_device() != dev or stats.get_device() != dev:
+                raise RuntimeError(f"layer_norm: its saved tensors came back as {xd.dtype} and {stats.dtype} on {xd.device} "
+                                   f"and {stats.device}")
             xd, _, _, _, x_step = _norm_layout(xd, dim, last)
+            x_at = xd.data_ptr()
         if dy.is_contiguous() and (not last or dim == dy.dim() - 1):
             g, g_step = dy, C * inner
         else:
@@ -1300,7 +1302,7 @@ class LayerNormFn(torch.autograd.Function):
         dx = _norm_out(dy, dim, last) if need_x else None
         dw = torch.empty_like(weight) if need_w else None
         db = torch.empty_like(bias) if need_b else None
-        at = ws_at = stats.data_ptr()                            # (some pointer, where no workspace is needed)
+        ws_at = at                                               # (some pointer, where no workspace is needed)
         if need_w or need_b:
             nbytes = _lib.fc3d_layer_norm_bwd_workspace(code, outer, C, inner)
             if nbytes:
@@ -1311,7 +1313,7 @@ class LayerNormFn(torch.autograd.Function):
             other.__enter__()
         try:
             status = _lib.fc3d_layer_norm_bwd(_raw_stream(dev) if _raw_stream is not None else _stream(), g.data_ptr(),
-                                              xd.data_ptr(), code, weight.data_ptr() if weight is not None else None,
+                                              x_at, code, weight.data_ptr() if weight is not None else None,
                                               bias.data_ptr() if bias is not None else None, p_code, at,
                                               at + 4 * outer * inner, outer, C, inner, g_step, x_step, relu,
                                               dx.data_ptr() if need_x else None, dw.data_ptr() if need_w else None,
